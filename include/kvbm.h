@@ -478,6 +478,164 @@ KVBM_API size_t kvbm_design_workspace_bytes(const kvbm_design_args* d);
 KVBM_API int kvbm_design(const kvbm_design_args* d, const kvbm_design_out* out, void* workspace,
                 size_t workspace_bytes, void* stream);
 
+/* Attention over whole prompts (extension; the reference never forms the
+ * attention output):
+ *
+ *   out[b,h,i] = sum_c softmax_c(scale * q[b,h,i] . k[b,h/G,c]) v[b,h/G,c]
+ *   lse[b,h,i] = log(sum_c exp(scale * q[b,h,i] . k[b,h/G,c]))   (natural log)
+ *
+ * over the kept keys c: c < the sequence's length, c <= i with `causal`, and
+ * key_mask[b * key_mask_bstride + c] != 0 where a key mask is given.  A row
+ * that keeps no key gets out 0 and lse -inf.  What a key that is not kept (or
+ * a row past a sequence's end) holds, NaN and infinities included, reaches no
+ * result.  lse is what kvbm_block_mass_lse and kvbm_options.lse take.
+ *
+ * float32, bfloat16 or float16 (out in the same type; sums, maxima and lse in
+ * float32), D <= 256, any strides (elements, dims [B, H, N, D]; lse [B, H, N]).
+ * Layouts as kvbm_options: dense, padded with seq_lens, or packed with
+ * cu_seqlens (q, k, v, out and lse packed alike, [total_tokens, H, D]: strides
+ * {unused, head, row, d}).  fill_outside != 0: rows of `out` and `lse` that
+ * belong to no sequence are written (0, -inf); 0: they are left as they were.
+ * `out` must not overlap the inputs.  No workspace; asynchronous on `stream`;
+ * the same inputs give the same bits. */
+typedef struct kvbm_attention_args {
+  const void* q;
+  int64_t q_stride[4];
+  const void* k;
+  int64_t k_stride[4];
+  const void* v;
+  int64_t v_stride[4];
+  int32_t dtype;
+  int32_t B, Hq, Hkv, N, D;
+  const uint8_t* key_mask;
+  int64_t key_mask_bstride;
+  double scale;
+  int32_t causal;
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens;
+  int64_t total_tokens;
+  int32_t fill_outside;
+  void* out;
+  int64_t out_stride[4];
+  float* lse;
+  int64_t lse_stride[3];
+} kvbm_attention_args;
+
+/* Host-only argument checks. */
+KVBM_API int kvbm_validate_attention(const kvbm_attention_args* a);
+
+KVBM_API int kvbm_attention(const kvbm_attention_args* a, void* stream);
+
+/* Attention of T query tokens per sequence over a paged key/value cache: one
+ * token (T = 1), or a chain or tree of up to 64 drafted tokens.
+ *
+ *   q            [B, H_q, T, D];  k_cache, v_cache [num_pages, page_size, H_kv, D]
+ *                (element strides of those dims)
+ *   block_table  [B, max_pages] as kvbm_paged_kv, or NULL: page
+ *                b * max_pages + i (num_pages >= B * max_pages)
+ *   seq_lens     [B] int32 on the device: cached tokens, the T tokens of this
+ *                call included (they are in the cache already: token u of
+ *                sequence b is slot seq_lens[b] - T + u).  Clamped into
+ *                [0, max_pages * page_size].  With 0 the rows are out 0, lse -inf.
+ *   tree_mask    [B|1, T, T] bytes or NULL: token t keeps drafted token u iff
+ *                tree_mask[b * bstride + t * rstride + u] != 0; NULL: u <= t.
+ *                Every earlier slot is kept by every token.
+ *   log_offsets  [B|1, H_kv|1, max_pages * page_size] float32 or NULL, added
+ *                to the scores (natural log; -log of the inclusion
+ *                probabilities of a thinned cache, evict.py:174-187).  -inf
+ *                drops a key.
+ *   weights, weights_out  [B, H_kv, max_pages * page_size] float32 or both
+ *                NULL, T = 1 only: weights_out = weights + sum over the
+ *                group's heads of the softmax weight of each key (slots past
+ *                the sequence are not written).  They may be one array.
+ *
+ * Types, row and NaN rules as kvbm_attention; a bad block-table entry as
+ * kvbm_block_mass_paged (its keys count as zero vectors, KVBM_ERR_PAGE).
+ * The same inputs give the same bits. */
+typedef struct kvbm_cached_args {
+  const void* q;
+  int64_t q_stride[4];
+  const void* k_cache;
+  int64_t k_stride[4];
+  const void* v_cache;
+  int64_t v_stride[4];
+  int32_t dtype;
+  int32_t B, Hq, Hkv, T, D;
+  int32_t num_pages, page_size, max_pages;
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  const int32_t* seq_lens;
+  const uint8_t* tree_mask;
+  int64_t tree_mask_bstride, tree_mask_rstride;
+  const float* log_offsets;
+  int64_t log_offsets_bstride, log_offsets_hstride;
+  const float* weights;
+  int64_t weights_bstride, weights_hstride;
+  float* weights_out;
+  int64_t weights_out_bstride, weights_out_hstride;
+  double scale;
+  void* out;
+  int64_t out_stride[4];
+  float* lse;
+  int64_t lse_stride[3];
+} kvbm_cached_args;
+
+KVBM_API int kvbm_validate_cached_attention(const kvbm_cached_args* a);
+
+/* Workspace bytes of kvbm_cached_attention (0 on invalid arguments). */
+KVBM_API size_t kvbm_cached_attention_workspace_bytes(const kvbm_cached_args* a);
+
+/* `workspace`: 256-byte aligned device memory; its contents on entry do not
+ * matter.  Calls that can overlap on the GPU need workspaces of their own. */
+KVBM_API int kvbm_cached_attention(const kvbm_cached_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Eviction from a paged cache by accumulated weight.  Per (sequence b, weight
+ * head w): with len = seq_lens[b] <= budget every token stays; otherwise the
+ * first n_sinks, the last `recency` and, of those between, the budget -
+ * n_sinks - recency tokens of the highest weights[b, w, c] (equal weights: the
+ * lower index first; NaN counts as -inf).  Kept tokens keep their order:
+ *
+ *   kept_out     [B, weight_heads, budget] int32, ascending, -1 past the new length
+ *   seq_lens_out [B] int32 = min(len, budget)
+ *   k_out, v_out [B, capacity, H_kv, D] (capacity >= budget): slot j holds
+ *                token kept_out[b, w, j]; rows past the new length are zeros
+ *                with zero_tail, else left as they were
+ *   weights_out  [B, weight_heads, budget] float32 or NULL: the kept weights, then 0
+ *
+ * weight_heads is H_kv (each kv head keeps its own tokens) or 1 (all heads the
+ * same).  Any dtype of kvbm_dtype (rows are moved, not computed on).  The
+ * outputs must not overlap the inputs.  A bad block-table entry gives zero
+ * rows and KVBM_ERR_PAGE at kvbm_check_device_errors. */
+typedef struct kvbm_evict_args {
+  const void* k_cache;
+  int64_t k_stride[4];
+  const void* v_cache;
+  int64_t v_stride[4];
+  int32_t dtype;
+  int32_t B, Hkv, D;
+  int32_t num_pages, page_size, max_pages;
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  const int32_t* seq_lens;
+  const float* weights;
+  int64_t weights_bstride, weights_hstride;
+  int32_t weight_heads;
+  int32_t budget, n_sinks, recency;
+  int32_t capacity;
+  int32_t zero_tail;
+  void* k_out;
+  int64_t k_out_stride[4];
+  void* v_out;
+  int64_t v_out_stride[4];
+  int32_t* seq_lens_out;
+  int32_t* kept_out;
+  float* weights_out;
+} kvbm_evict_args;
+
+KVBM_API int kvbm_validate_evict(const kvbm_evict_args* a);
+
+KVBM_API int kvbm_evict_cache(const kvbm_evict_args* a, void* stream);
+
 /* Queue `height` copies of `width` bytes on `stream`: row i goes from
  * src + i * src_pitch to dst + i * dst_pitch (cudaMemcpy2DAsync, direction
  * from the pointers).  The host-input path of the Python binding moves a

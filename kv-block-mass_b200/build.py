@@ -24,7 +24,7 @@ LIB = PKG_ROOT / "kvblockmass_b200" / "libkvbm.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O2,-fvisibility=hidden", "-shared",
-              "--expt-relaxed-constexpr", "-Xptxas", "-warn-spills"]
+              "--expt-relaxed-constexpr", "-Xptxas", "-warn-spills", "--threads", "0"]
 
 
 def nvcc_path() -> str:

@@ -6,6 +6,7 @@
 
 #include <atomic>
 
+#include "kvbm_attention.cuh"
 #include "kvbm_internal.cuh"
 
 namespace kvbm {
@@ -96,6 +97,9 @@ int device_sms(int dev) {
   }
   return n;
 }
+
+int attention_device_kind(int dev) { return device_kind(dev); }
+int attention_device_sms(int dev) { return device_sms(dev); }
 
 // SM count assumed when the device is unknown (sizes a workspace that fits
 // any sm_100 part).
@@ -663,12 +667,14 @@ int kvbm_copy_2d_async(void* dst, int64_t dst_pitch, const void* src, int64_t sr
 }
 
 int kvbm_check_device_errors(void* stream) {
-  int err = 0, perr = 0;
+  int err = 0, perr = 0, aperr = 0;
   int st = read_and_clear_device_error(static_cast<cudaStream_t>(stream), &err);
   if (st != KVBM_OK) return st;
   st = read_and_clear_page_error(static_cast<cudaStream_t>(stream), &perr);
   if (st != KVBM_OK) return st;
-  return err ? KVBM_ERR_TIMEOUT : (perr ? KVBM_ERR_PAGE : KVBM_OK);
+  st = read_and_clear_attention_page_error(static_cast<cudaStream_t>(stream), &aperr);
+  if (st != KVBM_OK) return st;
+  return err ? KVBM_ERR_TIMEOUT : (perr || aperr ? KVBM_ERR_PAGE : KVBM_OK);
 }
 
 }  // extern "C"

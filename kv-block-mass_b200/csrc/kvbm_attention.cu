@@ -1,0 +1,625 @@
+// Attention by plain FFMA tiles: prompt attention and attention over a paged
+// cache for fp32 inputs, and for 16-bit inputs whose head dim, strides or
+// scale the tensor-core kernels do not take; also the joining of split units
+// and the accumulation of per-key weights, which every cache kernel shares.
+//
+//   x_rc  = scale * q_r . k_c (+ log_offset_c)        for kept (r, c)
+//   lse_r = log sum_c exp(x_rc),  out_r = sum_c exp(x_rc - lse_r) v_c
+//
+// One pass over the keys with a running maximum m and sum l per row:
+// when a key tile raises m, l and the output row are multiplied by
+// exp(m_old - m_new).  A row that keeps no key has l = 0: out 0, lse -inf.
+//
+// Tiles: 16 x 16 threads own RPT x 4 scores each (RPT = 4: 64 rows, for
+// prompts and wide trees; RPT = 1: 16 rows, for single tokens), 64 keys a
+// tile, everything in fp32 registers and shared memory.  Bound by the FFMA
+// pipe (4 shared float4 reads feed 16 FFMAs per thread).
+#include <mutex>
+
+#include "kvbm_attention.cuh"
+
+namespace kvbm {
+namespace {
+
+// Set when a block-table entry lies outside [0, num_pages); the rows it
+// names count as zero vectors.
+__device__ unsigned int g_attention_page_error = 0;
+
+constexpr int kThreads = 256;
+constexpr int BN = 64;
+constexpr int kPad = 4;
+
+// Sign bit set: a masked pair (its value is not to be added, whatever it holds).
+__device__ __forceinline__ bool masked_p(float p) { return __float_as_int(p) < 0; }
+
+template <int RPT, int DP>
+struct Tile {
+  static constexpr int BM = 16 * RPT;
+  static constexpr int kStride = DP + kPad;
+  static constexpr int kPs = BN + kPad;
+  static constexpr size_t kBytes = sizeof(float) * ((size_t)(BM + 2 * BN) * kStride + (size_t)BM * kPs + BN);
+  float o[RPT][DP / 16];
+  float m[RPT], l[RPT];
+
+  __device__ void reset() {
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) o[i][d] = 0.f;
+    }
+  }
+};
+
+// Four consecutive elements of a row from d (zeros past D or for a null row).
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* row, int d, int D, long long ds, bool vec) {
+  float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (row == nullptr || d >= D) return r;
+  if (vec) {  // D % 4 == 0, unit stride, aligned rows
+    if constexpr (sizeof(T) == 4) {
+      r = *reinterpret_cast<const float4*>(row + d);
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(row + d);
+      const T* e = reinterpret_cast<const T*>(&u);
+      r = make_float4(to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3]));
+    }
+    return r;
+  }
+  r.x = to_f32(row[d * ds]);
+  if (d + 1 < D) r.y = to_f32(row[(d + 1) * ds]);
+  if (d + 2 < D) r.z = to_f32(row[(d + 2) * ds]);
+  if (d + 3 < D) r.w = to_f32(row[(d + 3) * ds]);
+  return r;
+}
+
+// The tiles of shared memory: Q [BM], K [BN], V [BN] (fp32, rows of DP + 4),
+// P [BM][BN + 4], bias [BN].
+template <int RPT, int DP>
+struct Smem {
+  using TL = Tile<RPT, DP>;
+  float *q, *k, *v, *p, *bias;
+  __device__ explicit Smem(float* base) {
+    q = base;
+    k = q + TL::BM * TL::kStride;
+    v = k + BN * TL::kStride;
+    p = v + BN * TL::kStride;
+    bias = p + TL::BM * TL::kPs;
+  }
+};
+
+// rows(r) -> const T* of row r of the tile, or null
+template <typename T, int RPT, int DP, class F>
+__device__ __forceinline__ void load_rows(float* dst, int rows, F&& f, int D, long long ds, bool vec) {
+  constexpr int kVecs = DP / 4;
+  for (int i = threadIdx.x; i < rows * kVecs; i += kThreads) {
+    const int r = i / kVecs, d = (i % kVecs) * 4;
+    *reinterpret_cast<float4*>(dst + r * (DP + kPad) + d) = load4<T>(f(r), d, D, ds, vec);
+  }
+}
+
+// One key tile: scores of the tile's 64 keys (K, V, bias already in shared
+// memory), softmax update, output update.  keep(r, j): whether row r keeps
+// key j of the tile.  sink(r, j, x): called for each kept-or-not score.
+// kSelect: some row may drop a key that another keeps, so products of dropped
+// pairs are left out one by one (0 * NaN is not 0).
+template <int RPT, int DP, class Keep, class Sink>
+__device__ __forceinline__ void tile_step(Tile<RPT, DP>& t, const Smem<RPT, DP>& s, float scale, bool has_bias,
+                                          bool select, Keep&& keep, Sink&& sink) {
+  using TL = Tile<RPT, DP>;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  float x[RPT][4];
+#pragma unroll
+  for (int i = 0; i < RPT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[i][j] = 0.f;
+#pragma unroll 4
+  for (int d = 0; d < DP; d += 4) {
+    float4 qv[RPT], kv[4];
+#pragma unroll
+    for (int i = 0; i < RPT; ++i)
+      qv[i] = *reinterpret_cast<const float4*>(s.q + (ty * RPT + i) * TL::kStride + d);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) kv[j] = *reinterpret_cast<const float4*>(s.k + (tx + 16 * j) * TL::kStride + d);
+#pragma unroll
+    for (int i = 0; i < RPT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[i][j] = fmaf(qv[i].x, kv[j].x, x[i][j]);
+        x[i][j] = fmaf(qv[i].y, kv[j].y, x[i][j]);
+        x[i][j] = fmaf(qv[i].z, kv[j].z, x[i][j]);
+        x[i][j] = fmaf(qv[i].w, kv[j].w, x[i][j]);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int r = ty * RPT + i;
+    float top = -INFINITY;
+    bool kp[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = tx + 16 * j;
+      // natural-log domain: an offset of the type's lowest value stays finite
+      x[i][j] = x[i][j] * scale;
+      if (has_bias) x[i][j] += s.bias[c];
+      kp[j] = keep(r, c);
+      if (!kp[j]) x[i][j] = -INFINITY;
+      sink(r, c, x[i][j]);
+      top = fmaxf(top, x[i][j]);
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float mn = fmaxf(t.m[i], top);
+    const float base = mn == -INFINITY ? 0.f : mn;  // nothing kept so far: every exponential below is 0
+    const float corr = exp2f((t.m[i] - base) * kLog2eF);
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float p = exp2f((x[i][j] - base) * kLog2eF);
+      sum += p;
+      s.p[r * TL::kPs + tx + 16 * j] = kp[j] ? p : -0.f;
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    t.l[i] = t.l[i] * corr + sum;
+    t.m[i] = mn;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) t.o[i][d] *= corr;
+  }
+  __syncwarp();  // a row's 64 weights come from its own half warp
+  float acc[RPT][DP / 16];  // this tile's share, added once: short sums lose less
+#pragma unroll
+  for (int i = 0; i < RPT; ++i)
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) acc[i][d] = 0.f;
+  for (int c = 0; c < BN; c += 4) {
+    float4 pv[RPT];
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) pv[i] = *reinterpret_cast<const float4*>(s.p + (ty * RPT + i) * TL::kPs + c);
+#pragma unroll
+    for (int cc = 0; cc < 4; ++cc) {
+#pragma unroll
+      for (int dc = 0; dc < DP / 64; ++dc) {
+        const float4 vv = *reinterpret_cast<const float4*>(s.v + (c + cc) * TL::kStride + dc * 64 + tx * 4);
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+          const float p = cc == 0 ? pv[i].x : cc == 1 ? pv[i].y : cc == 2 ? pv[i].z : pv[i].w;
+          if (select && masked_p(p)) continue;
+          acc[i][dc * 4 + 0] = fmaf(p, vv.x, acc[i][dc * 4 + 0]);
+          acc[i][dc * 4 + 1] = fmaf(p, vv.y, acc[i][dc * 4 + 1]);
+          acc[i][dc * 4 + 2] = fmaf(p, vv.z, acc[i][dc * 4 + 2]);
+          acc[i][dc * 4 + 3] = fmaf(p, vv.w, acc[i][dc * 4 + 3]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < RPT; ++i)
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) t.o[i][d] += acc[i][d];
+}
+
+// Output column of accumulator e of a thread.
+__device__ __forceinline__ int out_col(int e, int tx) { return (e / 4) * 64 + tx * 4 + (e & 3); }
+
+// ------------------------------------------------------------ prompt
+// Grid (row tiles from the last, B * Hq): under causal the longest run first.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) prompt_simt_kernel(PromptArgs a, bool vec) {
+  extern __shared__ float smem[];
+  constexpr int RPT = 4, BM = 64;
+  Smem<RPT, DP> s(smem);
+  const int b = blockIdx.y / a.Hq, h = blockIdx.y % a.Hq, g = h / a.G;
+  const int r0 = (int)(gridDim.x - 1 - blockIdx.x) * BM;
+  const SeqView sv = seq_view(a.lens, a.cu, true, b, a.N, a.total);
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  T* out = static_cast<T*>(a.out) + sv.q_b * a.os[0] + h * a.os[1] + (long long)sv.q_row * a.os[2];
+  float* lse = a.lse + sv.q_b * a.ls[0] + h * a.ls[1] + (long long)sv.q_row * a.ls[2];
+  if (r0 < sv.n) {
+    const T* q = static_cast<const T*>(a.q) + sv.q_b * a.qs[0] + h * a.qs[1] + (long long)sv.q_row * a.qs[2];
+    const T* k = static_cast<const T*>(a.k) + sv.k_b * a.ks[0] + g * a.ks[1] + (long long)sv.k_row * a.ks[2];
+    const T* v = static_cast<const T*>(a.v) + sv.k_b * a.vs[0] + g * a.vs[1] + (long long)sv.k_row * a.vs[2];
+    const uint8_t* km = a.kmask ? a.kmask + b * a.kmb : nullptr;
+    Tile<RPT, DP> t;
+    t.reset();
+    load_rows<T, RPT, DP>(s.q, BM, [&](int r) { return r0 + r < sv.n ? q + (long long)(r0 + r) * a.qs[2] : nullptr; },
+                          a.D, a.qs[3], vec);
+    const int end = a.causal ? min(sv.n, r0 + BM) : sv.n;
+    for (int c0 = 0; c0 < end; c0 += BN) {
+      __syncthreads();
+      // keys past the end and keys the mask drops: zero rows, never products with what they hold
+      auto live = [&](int j) { return c0 + j < end && (km == nullptr || km[c0 + j] != 0); };
+      load_rows<T, RPT, DP>(s.k, BN, [&](int j) { return live(j) ? k + (long long)(c0 + j) * a.ks[2] : nullptr; }, a.D,
+                            a.ks[3], vec);
+      load_rows<T, RPT, DP>(s.v, BN, [&](int j) { return live(j) ? v + (long long)(c0 + j) * a.vs[2] : nullptr; }, a.D,
+                            a.vs[3], vec);
+      if (threadIdx.x < BN) s.bias[threadIdx.x] = live(threadIdx.x) ? 0.f : -INFINITY;
+      __syncthreads();
+      const bool diag = a.causal && c0 + BN - 1 > r0;
+      tile_step<RPT, DP>(
+          t, s, a.scale, false, diag,
+          [&](int r, int j) { return s.bias[j] == 0.f && (!a.causal || c0 + j <= r0 + r); },
+          [](int, int, float) {});
+    }
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+      const int r = r0 + ty * RPT + i;
+      if (r >= sv.n) continue;
+      const float inv = t.l[i] > 0.f ? 1.f / t.l[i] : (t.l[i] == 0.f ? 0.f : t.l[i]);
+#pragma unroll
+      for (int e = 0; e < DP / 16; ++e) {
+        const int d = out_col(e, tx);
+        if (d < a.D) out[r * a.os[2] + d * a.os[3]] = from_f32<T>(t.l[i] == 0.f ? 0.f : t.o[i][e] * inv);
+      }
+      if (tx == 0) lse[r * a.ls[2]] = t.l[i] == 0.f ? -INFINITY : t.m[i] + logf(t.l[i]);
+    }
+  }
+  if (a.fill && a.cu == nullptr) {
+    for (int i = threadIdx.x; i < BM; i += kThreads) {
+      const int r = r0 + i;
+      if (r >= sv.n && r < a.N) lse[r * a.ls[2]] = -INFINITY;
+    }
+    for (int i = threadIdx.x; i < BM * a.D; i += kThreads) {
+      const int r = r0 + i / a.D;
+      if (r >= sv.n && r < a.N) out[r * a.os[2] + (i % a.D) * a.os[3]] = from_f32<T>(0.f);
+    }
+  }
+}
+
+// Rows of a packed output that belong to no sequence (before the first
+// offset, past the last, or past a sequence's first N rows): out 0, lse -inf.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) prompt_fill_kernel(PromptArgs a) {
+  const long long row = (long long)blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
+  if (row >= a.total) return;
+  const int lane = threadIdx.x & 31;
+  bool inside = false;
+  for (int b0 = 0; b0 < a.B && !inside; b0 += 32) {
+    const int b = b0 + lane;
+    bool in = false;
+    if (b < a.B) {
+      const SeqView sv = seq_view(nullptr, a.cu, true, b, a.N, a.total);
+      in = row >= sv.q_row && row < (long long)sv.q_row + sv.n;
+    }
+    inside = __any_sync(0xffffffffu, in);
+  }
+  if (inside) return;
+  for (int h = 0; h < a.Hq; ++h) {
+    T* out = static_cast<T*>(a.out) + h * a.os[1] + row * a.os[2];
+    for (int d = lane; d < a.D; d += 32) out[d * a.os[3]] = from_f32<T>(0.f);
+    if (lane == 0) a.lse[h * a.ls[1] + row * a.ls[2]] = -INFINITY;
+  }
+}
+
+// ------------------------------------------------------------ cache
+// The linear list of (sequence, kv head, row tile, key tile), key tile
+// fastest, is cut into C equal ranges, one per CTA: every SM gets the same
+// number of key tiles however the lengths differ.  A unit (sequence, kv head,
+// row tile) inside one range is finished by its CTA; a unit that crosses a
+// border leaves one partial (m, l, unnormalised output) per CTA, in slot 0
+// when it is the CTA's first unit and slot 1 when a later one, which
+// cached_merge_kernel joins in CTA order.
+template <typename T, int RPT, int DP>
+__global__ void __launch_bounds__(kThreads) cached_simt_kernel(CachedArgs a, bool vec) {
+  extern __shared__ float smem[];
+  constexpr int BM = 16 * RPT;
+  Smem<RPT, DP> s(smem);
+  __shared__ long long sh_first, sh_total;
+  __shared__ int sh_b;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  if (threadIdx.x < 32) {
+    long long pre, total, first = 0;
+    warp_tile_prefix(a, 0, &pre, &total);
+    const int b = warp_find_seq(a, split_begin(blockIdx.x, total, a.C), &first);
+    if (threadIdx.x == 0) {
+      sh_total = total;
+      sh_first = first;
+      sh_b = b;
+    }
+  }
+  __syncthreads();
+  const long long total = sh_total;
+  const long long begin = split_begin(blockIdx.x, total, a.C), end = split_begin(blockIdx.x + 1, total, a.C);
+  int b = sh_b;
+  long long bfirst = sh_first;
+  const int per = a.Hkv * a.RT;
+  for (long long at = begin; at < end;) {
+    int len = cached_len(a, b), nt = (len + BN - 1) / BN;
+    while (at >= bfirst + (long long)nt * per) {
+      bfirst += (long long)nt * per;
+      ++b;
+      len = cached_len(a, b);
+      nt = (len + BN - 1) / BN;
+    }
+    const int u = (int)((at - bfirst) / nt), g = u / a.RT, rt = u % a.RT;
+    const long long ufirst = bfirst + (long long)u * nt;
+    const int k0 = (int)(at - ufirst);
+    const int k1 = (int)min((long long)nt, end - ufirst);
+    const int pre = len - a.T;  // keys before the drafted tokens
+    const T* qb = static_cast<const T*>(a.q) + b * a.qs[0];
+    const float* off = a.off ? a.off + b * a.ob + g * a.oh : nullptr;
+    const uint8_t* tree = a.tree ? a.tree + b * a.tb : nullptr;
+    Tile<RPT, DP> t;
+    t.reset();
+    __syncthreads();
+    load_rows<T, RPT, DP>(
+        s.q, BM,
+        [&](int i) -> const T* {
+          const int r = rt * BM + i;
+          return r < a.R ? qb + (long long)(g * a.G + r / a.T) * a.qs[1] + (long long)(r % a.T) * a.qs[2] : nullptr;
+        },
+        a.D, a.qs[3], vec);
+    for (int kt = k0; kt < k1; ++kt) {
+      const int c0 = kt * BN;
+      __syncthreads();
+      auto at_slot = [&](const void* base, const long long* st, int j) -> const T* {
+        const int c = c0 + j;
+        if (c >= len || (off != nullptr && off[c] == -INFINITY)) return nullptr;
+        const int pi = c / a.pg.page_size;
+        const int page = a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
+        if (page < 0 || page >= a.pg.num_pages) {
+          atomicOr(&g_attention_page_error, 1u);
+          return nullptr;
+        }
+        return static_cast<const T*>(base) + (long long)page * st[0] + (long long)(c - pi * a.pg.page_size) * st[1] +
+               g * st[2];
+      };
+      load_rows<T, RPT, DP>(s.k, BN, [&](int j) { return at_slot(a.k, a.ks, j); }, a.D, a.ks[3], vec);
+      load_rows<T, RPT, DP>(s.v, BN, [&](int j) { return at_slot(a.v, a.vs, j); }, a.D, a.vs[3], vec);
+      if (off != nullptr && threadIdx.x < BN) {
+        const int c = c0 + threadIdx.x;
+        s.bias[threadIdx.x] = c < len ? off[c] : -INFINITY;
+      }
+      __syncthreads();
+      const bool drafts = c0 + BN > pre;  // some key of the tile is a drafted token or past the end
+      float* sc = a.scores ? a.scores + ((long long)(b * a.Hkv + g) * a.G) * a.Lmax + c0 : nullptr;
+      tile_step<RPT, DP>(
+          t, s, a.scale, off != nullptr, drafts,
+          [&](int i, int j) {
+            const int c = c0 + j, r = rt * BM + i;
+            if (c >= len || r >= a.R) return false;
+            if (off != nullptr && s.bias[j] == -INFINITY) return false;
+            if (c < pre) return true;
+            const int tok = r % a.T;
+            return tree ? tree[tok * a.tr + (c - pre)] != 0 : c - pre <= tok;
+          },
+          [&](int i, int j, float x) {
+            if (sc != nullptr && rt * BM + i < a.R && c0 + j < len) sc[(long long)(rt * BM + i) * a.Lmax + j] = x;
+          });
+    }
+    const bool whole = k0 == 0 && k1 == nt;
+    const int slot = begin >= ufirst ? 0 : 1;
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+      const int rl = ty * RPT + i, r = rt * BM + rl;
+      if (whole) {
+        if (r >= a.R) continue;
+        const int h = g * a.G + r / a.T, tok = r % a.T;
+        const float inv = 1.f / t.l[i];
+        T* out = static_cast<T*>(a.out) + b * a.os[0] + h * a.os[1] + tok * a.os[2];
+#pragma unroll
+        for (int e = 0; e < DP / 16; ++e) {
+          const int d = out_col(e, tx);
+          if (d < a.D) out[d * a.os[3]] = from_f32<T>(t.l[i] == 0.f ? 0.f : t.o[i][e] * inv);
+        }
+        if (tx == 0) {
+          a.lse[b * a.ls[0] + h * a.ls[1] + tok * a.ls[2]] = t.l[i] == 0.f ? -INFINITY : t.m[i] + logf(t.l[i]);
+          if (a.stats) a.stats[(long long)(b * a.Hkv + g) * a.R + r] = make_float2(t.m[i], t.l[i] == 0.f ? 0.f : inv);
+        }
+      } else {
+        const long long pr = ((long long)blockIdx.x * 2 + slot) * BM + rl;
+#pragma unroll
+        for (int e = 0; e < DP / 16; ++e) a.part_o[pr * DP + out_col(e, tx)] = t.o[i][e];
+        if (tx == 0) a.part_ml[pr] = make_float2(t.m[i], t.l[i]);
+      }
+    }
+    at = ufirst + k1;
+  }
+}
+
+// Joins the partials of every split unit, and writes the rows of sequences
+// with no keys (out 0, lse -inf).  One warp per row, grid (B * Hkv * RT, BM / 8);
+// partials in CTA order: the same bits on every run.
+template <typename T>
+__global__ void __launch_bounds__(256) cached_merge_kernel(CachedArgs a) {
+  const int unit = blockIdx.x, b = unit / (a.Hkv * a.RT), u = unit % (a.Hkv * a.RT), g = u / a.RT, rt = u % a.RT;
+  const int rl = blockIdx.y * 8 + threadIdx.x / 32, r = rt * a.BM + rl, lane = threadIdx.x & 31;
+  if (rl >= a.BM || r >= a.R) return;
+  long long pre, total;
+  warp_tile_prefix(a, b, &pre, &total);
+  const int nt = (cached_len(a, b) + a.KT - 1) / a.KT;
+  const int h = g * a.G + r / a.T, tok = r % a.T;
+  T* out = static_cast<T*>(a.out) + b * a.os[0] + h * a.os[1] + tok * a.os[2];
+  float* lse = a.lse + b * a.ls[0] + h * a.ls[1] + tok * a.ls[2];
+  if (nt == 0) {
+    for (int d = lane; d < a.D; d += 32) out[d * a.os[3]] = from_f32<T>(0.f);
+    if (lane == 0) *lse = -INFINITY;
+    return;
+  }
+  const long long t0 = pre + (long long)u * nt, t1 = t0 + nt;
+  const int i0 = (int)split_owner(t0, total, a.C), i1 = (int)split_owner(t1 - 1, total, a.C);
+  if (i0 == i1) return;  // finished by its CTA
+  auto row_of = [&](int i) {
+    const int slot = split_begin(i, total, a.C) >= t0 ? 0 : 1;
+    return ((long long)i * 2 + slot) * a.BM + rl;
+  };
+  float m = -INFINITY;
+  bool bad = false;  // a NaN maximum can only come with a NaN sum
+  for (int i = i0 + lane; i <= i1; i += 32) {
+    if (split_begin(i, total, a.C) == split_begin(i + 1, total, a.C)) continue;  // a CTA without tiles
+    m = fmaxf(m, a.part_ml[row_of(i)].x);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  (void)bad;
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f, acc[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+  for (int i = i0; i <= i1; ++i) {
+    if (split_begin(i, total, a.C) == split_begin(i + 1, total, a.C)) continue;
+    const long long pr = row_of(i);
+    const float2 ml = a.part_ml[pr];
+    const float f = exp2f((ml.x - base) * kLog2eF);
+    if (ml.y == 0.f) continue;  // kept nothing
+    l += ml.y * f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int d = lane + 32 * e;
+      if (d < a.D) acc[e] = fmaf(a.part_o[pr * a.DP + d], f, acc[e]);
+    }
+  }
+  const float inv = 1.f / l;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int d = lane + 32 * e;
+    if (d < a.D) out[d * a.os[3]] = from_f32<T>(l == 0.f ? 0.f : acc[e] * inv);
+  }
+  if (lane == 0) {
+    *lse = l == 0.f ? -INFINITY : m + logf(l);
+    if (a.stats) a.stats[(long long)(b * a.Hkv + g) * a.R + r] = make_float2(m, l == 0.f ? 0.f : inv);
+  }
+}
+
+// weights_out[b, g, c] = weights[b, g, c] + sum over the group's heads of
+// exp(x - m) / l, c < len.  From the stored scores (G * 4 bytes a key next to
+// the 4 D bytes of its k and v rows) rather than from a second pass over k.
+__global__ void __launch_bounds__(256) cached_weights_kernel(CachedArgs a) {
+  const int b = blockIdx.y / a.Hkv, g = blockIdx.y % a.Hkv;
+  const int len = cached_len(a, b);
+  const float* sc = a.scores + (long long)blockIdx.y * a.G * a.Lmax;
+  const float2* st = a.stats + (long long)blockIdx.y * a.R;
+  for (int c = blockIdx.x * 256 + threadIdx.x; c < len; c += gridDim.x * 256) {
+    float sum = 0.f;
+    for (int hh = 0; hh < a.G; ++hh) {
+      const float2 ml = st[hh];
+      const float base = ml.x == -INFINITY ? 0.f : ml.x;
+      sum = fmaf(exp2f((sc[(long long)hh * a.Lmax + c] - base) * kLog2eF), ml.y, sum);
+    }
+    a.wout[b * a.wob + g * a.woh + c] = a.w[b * a.wb + g * a.wh + c] + sum;
+  }
+}
+
+template <typename K>
+int set_smem(K kernel, size_t bytes) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess
+             ? KVBM_OK
+             : KVBM_ERR_CUDA;
+}
+
+bool rows_aligned(const void* p, const long long* st, int D, int es) {
+  return st[3] == 1 && D % 4 == 0 && (uintptr_t)p % (4 * es) == 0 && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
+}
+
+template <typename T, int DP>
+int prompt_simt(const PromptArgs& a, cudaStream_t s) {
+  const bool vec = rows_aligned(a.q, a.qs, a.D, sizeof(T)) && rows_aligned(a.k, a.ks, a.D, sizeof(T)) &&
+                   rows_aligned(a.v, a.vs, a.D, sizeof(T));
+  auto kern = prompt_simt_kernel<T, DP>;
+  constexpr size_t bytes = Tile<4, DP>::kBytes;
+  if (set_smem(kern, bytes) != KVBM_OK) return KVBM_ERR_CUDA;
+  kern<<<dim3((unsigned)((a.N + 63) / 64), (unsigned)(a.B * a.Hq)), kThreads, bytes, s>>>(a, vec);
+  return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
+}
+
+template <typename T>
+int prompt_simt_d(const PromptArgs& a, cudaStream_t s) {
+  if (a.D <= 64) return prompt_simt<T, 64>(a, s);
+  if (a.D <= 128) return prompt_simt<T, 128>(a, s);
+  return prompt_simt<T, 256>(a, s);
+}
+
+template <typename T, int RPT, int DP>
+int cached_simt(const CachedArgs& a, cudaStream_t s) {
+  const bool vec = rows_aligned(a.q, a.qs, a.D, sizeof(T)) && rows_aligned(a.k, a.ks, a.D, sizeof(T)) &&
+                   rows_aligned(a.v, a.vs, a.D, sizeof(T));
+  auto kern = cached_simt_kernel<T, RPT, DP>;
+  constexpr size_t bytes = Tile<RPT, DP>::kBytes;
+  if (set_smem(kern, bytes) != KVBM_OK) return KVBM_ERR_CUDA;
+  kern<<<(unsigned)a.C, kThreads, bytes, s>>>(a, vec);
+  return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
+}
+
+template <typename T>
+int cached_simt_d(const CachedArgs& a, cudaStream_t s) {
+  if (a.BM == 16) {
+    if (a.DP == 64) return cached_simt<T, 1, 64>(a, s);
+    if (a.DP == 128) return cached_simt<T, 1, 128>(a, s);
+    return cached_simt<T, 1, 256>(a, s);
+  }
+  if (a.DP == 64) return cached_simt<T, 4, 64>(a, s);
+  if (a.DP == 128) return cached_simt<T, 4, 128>(a, s);
+  return cached_simt<T, 4, 256>(a, s);
+}
+
+}  // namespace
+
+int launch_prompt_simt(const PromptArgs& a, int dtype, cudaStream_t s) {
+  if (dtype == KVBM_F32) return prompt_simt_d<float>(a, s);
+  if (dtype == KVBM_BF16) return prompt_simt_d<__nv_bfloat16>(a, s);
+  return prompt_simt_d<__half>(a, s);
+}
+
+int launch_prompt_fill(const PromptArgs& a, int dtype, cudaStream_t s) {
+  if (a.cu == nullptr || a.total == 0) return KVBM_OK;
+  const unsigned grid = (unsigned)((a.total + kThreads / 32 - 1) / (kThreads / 32));
+  if (dtype == KVBM_F32)
+    prompt_fill_kernel<float><<<grid, kThreads, 0, s>>>(a);
+  else if (dtype == KVBM_BF16)
+    prompt_fill_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(a);
+  else
+    prompt_fill_kernel<__half><<<grid, kThreads, 0, s>>>(a);
+  return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
+}
+
+int launch_cached_simt(const CachedArgs& a, int dtype, cudaStream_t s) {
+  if (dtype == KVBM_F32) return cached_simt_d<float>(a, s);
+  if (dtype == KVBM_BF16) return cached_simt_d<__nv_bfloat16>(a, s);
+  return cached_simt_d<__half>(a, s);
+}
+
+int launch_cached_merge(const CachedArgs& a, int dtype, cudaStream_t s) {
+  const int rows = a.R < a.BM ? a.R : a.BM;
+  const dim3 grid((unsigned)(a.B * a.Hkv * a.RT), (unsigned)((rows + 7) / 8));
+  if (dtype == KVBM_F32)
+    cached_merge_kernel<float><<<grid, 256, 0, s>>>(a);
+  else if (dtype == KVBM_BF16)
+    cached_merge_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
+  else
+    cached_merge_kernel<__half><<<grid, 256, 0, s>>>(a);
+  return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
+}
+
+int launch_cached_weights(const CachedArgs& a, cudaStream_t s) {
+  const int blocks = (a.Lmax + 255) / 256;
+  cached_weights_kernel<<<dim3((unsigned)(blocks < 1024 ? blocks : 1024), (unsigned)(a.B * a.Hkv)), 256, 0, s>>>(a);
+  return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
+}
+
+int read_and_clear_attention_page_error(cudaStream_t s, int* err) {
+  unsigned int v = 0;
+  if (cudaMemcpyFromSymbolAsync(&v, g_attention_page_error, sizeof(v), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
+      cudaStreamSynchronize(s) != cudaSuccess)
+    return KVBM_ERR_CUDA;
+  *err = v != 0;
+  if (v != 0) {
+    const unsigned int zero = 0;
+    if (cudaMemcpyToSymbolAsync(g_attention_page_error, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s) !=
+            cudaSuccess ||
+        cudaStreamSynchronize(s) != cudaSuccess)
+      return KVBM_ERR_CUDA;
+  }
+  return KVBM_OK;
+}
+
+unsigned int* attention_page_error_word() {
+  void* p = nullptr;
+  if (cudaGetSymbolAddress(&p, g_attention_page_error) != cudaSuccess) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  return static_cast<unsigned int*>(p);
+}
+
+}  // namespace kvbm

@@ -1,0 +1,166 @@
+// Arguments and device helpers shared by the attention kernels (prompt
+// attention, attention over a paged cache) and the cache eviction.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "kvbm.h"
+#include "kvbm_internal.cuh"
+
+namespace kvbm {
+
+constexpr float kLog2eF = 1.44269504088896340736f;
+constexpr float kLn2F = 0.69314718055994530942f;
+// Drafted tokens of one cached call: a row of the tree mask fits a 64-bit word.
+constexpr int kMaxTreeTokens = 64;
+
+// Prompt attention as the kernels see it (strides in elements, dims [B, H, N, D]).
+struct PromptArgs {
+  const void *q, *k, *v;
+  long long qs[4], ks[4], vs[4];
+  int B, Hq, Hkv, G, N, D;
+  const uint8_t* kmask;  // [B|1, N] or null
+  long long kmb;
+  int causal;
+  float scale;
+  const int32_t* lens;  // [B] or null
+  const int32_t* cu;    // [B + 1] or null
+  long long total;
+  int fill;             // 1: rows past a sequence's end get out 0, lse -inf
+  void* out;
+  long long os[4];
+  float* lse;
+  long long ls[3];
+};
+
+// A paged cache: row c of sequence b is slot c % page_size of page
+// table[b * ts + c / page_size] (table == null: page b * max_pages + c / page_size).
+struct PagedView {
+  const int32_t* table;
+  long long ts;
+  int num_pages, page_size, max_pages;
+};
+
+// Attention over a cache: unit (b, g) has R = G * T rows, row r = hh * T + t.
+struct CachedArgs {
+  const void *q, *k, *v;
+  long long qs[4];          // [B, Hq, T, D]
+  long long ks[4], vs[4];   // [num_pages, page_size, Hkv, D]
+  PagedView pg;
+  int B, Hq, Hkv, G, T, D, R;
+  int Lmax;                 // max_pages * page_size
+  const int32_t* lens;
+  const uint8_t* tree;      // [B|1, T, T] or null (u <= t)
+  long long tb, tr;
+  const float* off;         // [B|1, Hkv|1, Lmax] or null
+  long long ob, oh;
+  float scale;
+  void* out;
+  long long os[4];
+  float* lse;
+  long long ls[3];
+  // weights (T == 1)
+  const float* w;
+  long long wb, wh;
+  float* wout;
+  long long wob, woh;
+  // scratch
+  float* scores;            // [B * Hkv, G, Lmax] or null
+  float2* stats;            // [B * Hkv, R]: (max, 1 / sum) per row
+  float* part_o;            // [C][2][BM][DP] unnormalised outputs of split units
+  float2* part_ml;          // [C][2][BM]
+  int C;                    // CTAs of the split kernel
+  int BM, RT, KT, DP;       // rows per row tile, row tiles, keys per tile, padded D
+};
+
+// Length of sequence b, inside the table.
+__device__ __forceinline__ int cached_len(const CachedArgs& a, int b) {
+  const int n = a.lens[b];
+  return n < 0 ? 0 : (n < a.Lmax ? n : a.Lmax);
+}
+
+// First CTA-linear tile of CTA i, and the CTA that holds tile t, when `total`
+// tiles are cut into C ranges [i * total / C, (i + 1) * total / C).
+__device__ __forceinline__ long long split_begin(long long i, long long total, long long C) { return i * total / C; }
+__device__ __forceinline__ long long split_owner(long long t, long long total, long long C) {
+  return ((t + 1) * C + total - 1) / total - 1;
+}
+
+// Key tiles of sequences [0, b) (times units per sequence) by one warp:
+// prefix of b, and the total over all B.
+__device__ __forceinline__ void warp_tile_prefix(const CachedArgs& a, int b_end, long long* prefix, long long* total) {
+  const int lane = threadIdx.x & 31;
+  long long pre = 0, all = 0;
+  for (int b = lane; b < a.B; b += 32) {
+    const long long n = (cached_len(a, b) + a.KT - 1) / a.KT;
+    all += n;
+    if (b < b_end) pre += n;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    pre += __shfl_xor_sync(0xffffffffu, pre, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+  }
+  const long long per = (long long)a.Hkv * a.RT;
+  *prefix = pre * per;
+  *total = all * per;
+}
+
+// The sequence that holds linear tile t: first b with prefix(b + 1) > t, and prefix(b).  One warp.
+__device__ __forceinline__ int warp_find_seq(const CachedArgs& a, long long t, long long* first) {
+  const int lane = threadIdx.x & 31;
+  const long long per = (long long)a.Hkv * a.RT;
+  long long carry = 0;
+  for (int base = 0; base < a.B; base += 32) {
+    const int b = base + lane;
+    const long long n = b < a.B ? (long long)((cached_len(a, b) + a.KT - 1) / a.KT) * per : 0;
+    long long incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, carry + incl > t);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      *first = carry + __shfl_sync(0xffffffffu, incl - n, l);
+      return base + l;
+    }
+    carry += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  *first = carry;
+  return a.B;
+}
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+
+// Launchers (kvbm_status).
+int launch_prompt_simt(const PromptArgs& a, int dtype, cudaStream_t s);
+int launch_prompt_fill(const PromptArgs& a, int dtype, cudaStream_t s);
+bool prompt_tc_supported(const PromptArgs& a, int dtype);
+int launch_prompt_tc(const PromptArgs& a, int dtype, cudaStream_t s);
+int launch_cached_simt(const CachedArgs& a, int dtype, cudaStream_t s);
+int launch_cached_merge(const CachedArgs& a, int dtype, cudaStream_t s);
+int launch_cached_weights(const CachedArgs& a, cudaStream_t s);
+int read_and_clear_attention_error(cudaStream_t s, int* err);         // waits that ran out
+int read_and_clear_attention_page_error(cudaStream_t s, int* err);    // bad table entries (attention, eviction)
+unsigned int* attention_page_error_word();                            // its device address (or null)
+
+int attention_device_kind(int dev);  // 1: sm_100
+int attention_device_sms(int dev);
+
+}  // namespace kvbm

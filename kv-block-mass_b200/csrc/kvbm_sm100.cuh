@@ -11,9 +11,9 @@ namespace kvbm {
 namespace sm100 {
 
 // Device-wide error word: nonzero once a bounded wait gave up (see kvbm.h,
-// kvbm_check_device_errors).  Only kvbm_tc.cu includes this header, so the
-// library holds exactly one copy.
-__device__ unsigned int g_kvbm_device_error = 0;
+// kvbm_check_device_errors).  Every source file that includes this header
+// holds a copy of its own and a reader for it.
+static __device__ unsigned int g_kvbm_device_error = 0;
 
 // A wait on an mbarrier gives up after this many nanoseconds of %globaltimer.
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s

@@ -13,6 +13,11 @@ Beyond the reference's entry points:
 * ``block_mass_varlen``: packed (varlen) batches with ``cu_seqlens``;
 * ``block_mass_paged``: keys from a paged KV cache and block table;
 * ``design_from_mass``: the reference's eviction design (evict.py) on the GPU;
+* ``attention_b200`` / ``attention_varlen``: the attention of a prompt and its
+  row log-sum-exp (what ``lse=`` takes);
+* ``attention_cached``: one token, or a tree of drafted tokens, over a paged
+  cache, with the accumulated weight of each key;
+* ``evict_cache``: a paged cache cut down to its heaviest tokens;
 * ``kvblockmass_b200.distributed``: (batch, kv-head) shards over ranks.
 """
 
@@ -36,6 +41,13 @@ from .ops import (  # noqa: F401
     run_prepared,
     workspace_bytes,
 )
+from .attention import (  # noqa: F401
+    attention_b200,
+    attention_cached,
+    attention_varlen,
+    cached_attention_workspace_bytes,
+)
+from .evict import EvictedCache, evict_cache  # noqa: F401
 from .design import DeviceDesign, design_from_mass  # noqa: F401
 from .workloads import WORKLOADS, Workload, make_inputs, pairs  # noqa: F401
 
@@ -53,6 +65,12 @@ __all__ = [
     "check_device_errors",
     "design_from_mass",
     "DeviceDesign",
+    "attention_b200",
+    "attention_varlen",
+    "attention_cached",
+    "cached_attention_workspace_bytes",
+    "evict_cache",
+    "EvictedCache",
     "kernel_path",
     "method_of",
     "make_problem",

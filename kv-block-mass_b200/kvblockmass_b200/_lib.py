@@ -68,6 +68,13 @@ EXPORTED = [
     "kvbm_design",
     "kvbm_copy_2d_async",
     "kvbm_method",
+    "kvbm_validate_attention",
+    "kvbm_attention",
+    "kvbm_validate_cached_attention",
+    "kvbm_cached_attention_workspace_bytes",
+    "kvbm_cached_attention",
+    "kvbm_validate_evict",
+    "kvbm_evict_cache",
 ]
 
 
@@ -174,6 +181,116 @@ class DesignOut(ctypes.Structure):
     ]
 
 
+class AttentionArgs(ctypes.Structure):
+    """Mirror of ``struct kvbm_attention_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 4),
+        ("k", ctypes.c_void_p),
+        ("k_stride", ctypes.c_int64 * 4),
+        ("v", ctypes.c_void_p),
+        ("v_stride", ctypes.c_int64 * 4),
+        ("dtype", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("Hq", ctypes.c_int32),
+        ("Hkv", ctypes.c_int32),
+        ("N", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("key_mask", ctypes.c_void_p),
+        ("key_mask_bstride", ctypes.c_int64),
+        ("scale", ctypes.c_double),
+        ("causal", ctypes.c_int32),
+        ("seq_lens", ctypes.c_void_p),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("total_tokens", ctypes.c_int64),
+        ("fill_outside", ctypes.c_int32),
+        ("out", ctypes.c_void_p),
+        ("out_stride", ctypes.c_int64 * 4),
+        ("lse", ctypes.c_void_p),
+        ("lse_stride", ctypes.c_int64 * 3),
+    ]
+
+
+class CachedArgs(ctypes.Structure):
+    """Mirror of ``struct kvbm_cached_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 4),
+        ("k_cache", ctypes.c_void_p),
+        ("k_stride", ctypes.c_int64 * 4),
+        ("v_cache", ctypes.c_void_p),
+        ("v_stride", ctypes.c_int64 * 4),
+        ("dtype", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("Hq", ctypes.c_int32),
+        ("Hkv", ctypes.c_int32),
+        ("T", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_stride", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p),
+        ("tree_mask", ctypes.c_void_p),
+        ("tree_mask_bstride", ctypes.c_int64),
+        ("tree_mask_rstride", ctypes.c_int64),
+        ("log_offsets", ctypes.c_void_p),
+        ("log_offsets_bstride", ctypes.c_int64),
+        ("log_offsets_hstride", ctypes.c_int64),
+        ("weights", ctypes.c_void_p),
+        ("weights_bstride", ctypes.c_int64),
+        ("weights_hstride", ctypes.c_int64),
+        ("weights_out", ctypes.c_void_p),
+        ("weights_out_bstride", ctypes.c_int64),
+        ("weights_out_hstride", ctypes.c_int64),
+        ("scale", ctypes.c_double),
+        ("out", ctypes.c_void_p),
+        ("out_stride", ctypes.c_int64 * 4),
+        ("lse", ctypes.c_void_p),
+        ("lse_stride", ctypes.c_int64 * 3),
+    ]
+
+
+class EvictArgs(ctypes.Structure):
+    """Mirror of ``struct kvbm_evict_args``."""
+
+    _fields_ = [
+        ("k_cache", ctypes.c_void_p),
+        ("k_stride", ctypes.c_int64 * 4),
+        ("v_cache", ctypes.c_void_p),
+        ("v_stride", ctypes.c_int64 * 4),
+        ("dtype", ctypes.c_int32),
+        ("B", ctypes.c_int32),
+        ("Hkv", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_stride", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p),
+        ("weights", ctypes.c_void_p),
+        ("weights_bstride", ctypes.c_int64),
+        ("weights_hstride", ctypes.c_int64),
+        ("weight_heads", ctypes.c_int32),
+        ("budget", ctypes.c_int32),
+        ("n_sinks", ctypes.c_int32),
+        ("recency", ctypes.c_int32),
+        ("capacity", ctypes.c_int32),
+        ("zero_tail", ctypes.c_int32),
+        ("k_out", ctypes.c_void_p),
+        ("k_out_stride", ctypes.c_int64 * 4),
+        ("v_out", ctypes.c_void_p),
+        ("v_out_stride", ctypes.c_int64 * 4),
+        ("seq_lens_out", ctypes.c_void_p),
+        ("kept_out", ctypes.c_void_p),
+        ("weights_out", ctypes.c_void_p),
+    ]
+
+
 _lib = None
 
 
@@ -250,6 +367,16 @@ def load() -> ctypes.CDLL:
                                        ctypes.c_int64, ctypes.c_void_p]
     lib.kvbm_method.restype = ctypes.c_int
     lib.kvbm_method.argtypes = [P, O]
+    # Prompt attention, attention over a paged cache, cache eviction.
+    A, W, E = ctypes.POINTER(AttentionArgs), ctypes.POINTER(CachedArgs), ctypes.POINTER(EvictArgs)
+    for name, args in (("kvbm_validate_attention", [A]), ("kvbm_attention", [A, ctypes.c_void_p]),
+                       ("kvbm_validate_cached_attention", [W]),
+                       ("kvbm_cached_attention", [W, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+                       ("kvbm_validate_evict", [E]), ("kvbm_evict_cache", [E, ctypes.c_void_p])):
+        getattr(lib, name).restype = ctypes.c_int
+        getattr(lib, name).argtypes = args
+    lib.kvbm_cached_attention_workspace_bytes.restype = ctypes.c_size_t
+    lib.kvbm_cached_attention_workspace_bytes.argtypes = [W]
     lib.kvbm_check_device_errors.restype = ctypes.c_int
     lib.kvbm_check_device_errors.argtypes = [ctypes.c_void_p]
     if lib.kvbm_abi_version() != ABI_VERSION:
