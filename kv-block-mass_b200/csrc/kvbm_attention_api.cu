@@ -179,6 +179,7 @@ extern "C" int kvbm_attention(const kvbm_attention_args* p, void* stream) {
   const PromptArgs a = prompt_args(p);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a.cu != nullptr && a.total == 0) return KVBM_OK;
+  if (prompt_tc_supported(a, p->dtype)) return launch_prompt_tc(a, p->dtype, s);
   if (a.fill && a.cu != nullptr) {
     const int f = launch_prompt_fill(a, p->dtype, s);
     if (f != KVBM_OK) return f;

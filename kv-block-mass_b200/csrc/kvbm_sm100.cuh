@@ -183,6 +183,18 @@ __device__ __forceinline__ void mma_tf32(uint32_t d_tmem, uint64_t a_desc, uint6
       : "memory");
 }
 
+// D[tmem] (+)= A[tmem] * B[smem desc], kind::f16: A's row i in lane i, two
+// 16-bit elements of K per 32-bit column.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // Arrive (once) on `bar` when all tcgen05.mma previously issued by this thread complete.
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
@@ -242,6 +254,24 @@ __device__ __forceinline__ void tmem_ld16x256_x4(uint32_t taddr, float (&v)[16])
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// 32 lanes x 16 / 32 consecutive 32-bit columns, the layout of tmem_ld32.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
+  uint32_t r[2][16];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) r[i / 16][i % 16] = __float_as_uint(v[i]);
+  tmem_st16(taddr, r[0]);
+  tmem_st16(taddr + 16, r[1]);
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Shared-memory matrix descriptor for a K-major operand stored in the
@@ -265,6 +295,16 @@ __device__ __forceinline__ uint64_t k16_interleaved_desc(uint32_t addr) {
          | ((uint64_t)(256 >> 4) << 32)        // stride byte offset: next 8-row group
          | ((uint64_t)1 << 46);                // descriptor version (sm_100); swizzle: none
 }
+
+// Shared-memory matrix descriptor for an MN-major operand in the same
+// layout: rows of K hold 64 16-bit elements of MN (128 bytes), 8 K rows to an
+// atom, atoms of later K rows 1024 bytes apart, the next 64 elements of MN
+// `mn_stride` bytes apart.  (kTransposeB in the instruction descriptor.)
+__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t addr, uint32_t mn_stride) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(mn_stride >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+constexpr uint32_t kTransposeB = 1u << 16;  // B is MN-major
 
 // Instruction descriptor, kind::f16 / kind::tf32: fp32 accumulate, A and B of
 // the same input format (0 = fp16, 1 = bf16, 2 = tf32), both K-major, shape M x N.
@@ -310,6 +350,38 @@ __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pk(a)), "l"(pk(b)));
   return upk(d);
 }
+// max that returns NaN if either input is one.
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Two floats as a pair of 16-bit values, the first in the low half.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  uint32_t r;
+  if constexpr (kBf16)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+template <int kRegs>
+__device__ __forceinline__ void reg_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void reg_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
 // Flush-to-zero add: denormal inputs count as 0 (matches ex2.approx.ftz).
 __device__ __forceinline__ float2 fadd2_ftz(float2 a, float2 b) {
   unsigned long long d;

@@ -1722,6 +1722,12 @@ int launch_km(const kvbm_problem* p, const WsLayout& L, void* ws, cudaStream_t s
 
 bool tc_path_enabled() { return encode_fn() != nullptr; }
 
+// The same map for the attention kernels (16-bit operands).
+bool make_attention_map(CUtensorMap* map, const void* base, bool bf16, int B, int H, int N, int D, const int64_t* st) {
+  return make_map(map, base, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, B, H, N, D,
+                  st);
+}
+
 namespace {
 __device__ int g_selftest_result = -1;
 
