@@ -14,7 +14,7 @@
 // prompts and wide trees; RPT = 1: 16 rows, for single tokens), 64 keys a
 // tile, everything in fp32 registers and shared memory.  Bound by the FFMA
 // pipe (4 shared float4 reads feed 16 FFMAs per thread).
-#include <mutex>
+#include <atomic>
 
 #include "kvbm_attention.cuh"
 
@@ -613,13 +613,25 @@ int read_and_clear_attention_page_error(cudaStream_t s, int* err) {
   return KVBM_OK;
 }
 
+// Looked up once per device (every device has a copy of the word).
 unsigned int* attention_page_error_word() {
+  constexpr int kMaxDevices = 64;
+  static std::atomic<unsigned int*> words[kMaxDevices] = {};
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  unsigned int* w = words[dev].load(std::memory_order_acquire);
+  if (w != nullptr) return w;
   void* p = nullptr;
   if (cudaGetSymbolAddress(&p, g_attention_page_error) != cudaSuccess) {
     cudaGetLastError();
     return nullptr;
   }
-  return static_cast<unsigned int*>(p);
+  w = static_cast<unsigned int*>(p);
+  words[dev].store(w, std::memory_order_release);
+  return w;
 }
 
 }  // namespace kvbm

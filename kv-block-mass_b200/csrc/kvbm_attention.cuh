@@ -18,6 +18,9 @@ constexpr float kLn2F = 0.69314718055994530942f;
 // Drafted tokens of one cached call: a row of the tree mask fits a 64-bit word.
 constexpr int kMaxTreeTokens = 64;
 
+// Keys of one tile of the cache kernels.
+constexpr int kCachedKeyTile = 64;
+
 // Prompt attention as the kernels see it (strides in elements, dims [B, H, N, D]).
 struct PromptArgs {
   const void *q, *k, *v;
@@ -75,6 +78,7 @@ struct CachedArgs {
   float2* part_ml;          // [C][2][BM]
   int C;                    // CTAs of the split kernel
   int BM, RT, KT, DP;       // rows per row tile, row tiles, keys per tile, padded D
+  unsigned int* page_error; // set when a table entry is no page
 };
 
 // Length of sequence b, inside the table.
@@ -148,12 +152,37 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 
+// The non-finite v elements of drafted tokens [lo, hi) that token `tok` keeps,
+// added to four output columns from d (the matrix products took them as zeros).
+template <typename T>
+__device__ __noinline__ void add_draft_nonfinite(const CachedArgs& a, int b, int g, int tok, int lo, int hi, int pre,
+                                                 int d, float4& acc) {
+  const uint8_t* tree = a.tree ? a.tree + b * a.tb : nullptr;
+  const float* off = a.off ? a.off + b * a.ob + g * a.oh : nullptr;
+  for (int c = lo; c < hi; ++c) {
+    if (!(tree ? tree[tok * a.tr + (c - pre)] != 0 : c - pre <= tok)) continue;
+    if (off != nullptr && off[c] == -INFINITY) continue;
+    const int pi = c / a.pg.page_size;
+    const int page = a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
+    if (page < 0 || page >= a.pg.num_pages) continue;
+    const T* v = static_cast<const T*>(a.v) + (long long)page * a.vs[0] +
+                 (long long)(c - pi * a.pg.page_size) * a.vs[1] + g * a.vs[2];
+    float* o = &acc.x;
+    for (int e = 0; e < 4; ++e) {
+      if (d + e >= a.D) continue;
+      const float x = to_f32(v[(d + e) * a.vs[3]]);
+      if (!(fabsf(x) < INFINITY)) o[e] += x;
+    }
+  }
+}
+
 // Launchers (kvbm_status).
 int launch_prompt_simt(const PromptArgs& a, int dtype, cudaStream_t s);
 int launch_prompt_fill(const PromptArgs& a, int dtype, cudaStream_t s);
 bool prompt_tc_supported(const PromptArgs& a, int dtype);
 int launch_prompt_tc(const PromptArgs& a, int dtype, cudaStream_t s);
 int launch_cached_simt(const CachedArgs& a, int dtype, cudaStream_t s);
+int launch_cached_mma(const CachedArgs& a, int dtype, cudaStream_t s);  // R <= 16 rows a tile, 16-bit types
 int launch_cached_merge(const CachedArgs& a, int dtype, cudaStream_t s);
 int launch_cached_weights(const CachedArgs& a, cudaStream_t s);
 int read_and_clear_attention_error(cudaStream_t s, int* err);         // waits that ran out

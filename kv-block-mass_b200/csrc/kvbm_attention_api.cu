@@ -86,8 +86,19 @@ int check_cached(const kvbm_cached_args* p) {
   return KVBM_OK;
 }
 
+// The mma.sync kernel reads rows in 16-byte pieces.
+bool cached_mma_supported(const kvbm_cached_args* p) {
+  if (p->dtype == KVBM_F32 || p->D % 8 != 0) return false;
+  auto rows16 = [](const void* base, const int64_t* st) {
+    return (uintptr_t)base % 16 == 0 && st[3] == 1 && st[0] % 8 == 0 && st[1] % 8 == 0 && st[2] % 8 == 0;
+  };
+  return rows16(p->q, p->q_stride) && rows16(p->k_cache, p->k_stride) && rows16(p->v_cache, p->v_stride) &&
+         rows16(p->out, p->out_stride);
+}
+
 struct CachedPlan {
   CachedArgs a;
+  bool mma = false;
   size_t part_o = 0, part_ml = 0, stats = 0, scores = 0, total = 0;
 };
 
@@ -131,8 +142,9 @@ void plan_cached(const kvbm_cached_args* p, int sms, CachedPlan* pl) {
   a.wob = p->weights_out_bstride;
   a.woh = p->weights_out_hstride;
   a.DP = a.D <= 64 ? 64 : a.D <= 128 ? 128 : 256;
-  a.BM = a.R <= 16 ? 16 : 64;
-  a.KT = 64;
+  pl->mma = cached_mma_supported(p);
+  a.BM = a.R <= 16 || pl->mma ? 16 : 64;
+  a.KT = kCachedKeyTile;
   a.RT = (a.R + a.BM - 1) / a.BM;
   // no more CTAs than key tiles of full-length sequences
   const long long tiles = (long long)a.B * a.Hkv * a.RT * ((a.Lmax + a.KT - 1) / a.KT);
@@ -217,8 +229,10 @@ extern "C" int kvbm_cached_attention(const kvbm_cached_args* p, void* workspace,
     a.stats = reinterpret_cast<float2*>(w + pl.stats);
     a.scores = reinterpret_cast<float*>(w + pl.scores);
   }
+  a.page_error = attention_page_error_word();
+  if (a.page_error == nullptr) return KVBM_ERR_CUDA;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  st = launch_cached_simt(a, p->dtype, s);
+  st = pl.mma ? launch_cached_mma(a, p->dtype, s) : launch_cached_simt(a, p->dtype, s);
   if (st != KVBM_OK) return st;
   st = launch_cached_merge(a, p->dtype, s);
   if (st != KVBM_OK) return st;
