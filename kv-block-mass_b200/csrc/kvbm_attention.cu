@@ -501,13 +501,6 @@ __global__ void __launch_bounds__(256) cached_weights_kernel(CachedArgs a) {
   }
 }
 
-template <typename K>
-int set_smem(K kernel, size_t bytes) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess
-             ? KVBM_OK
-             : KVBM_ERR_CUDA;
-}
-
 bool rows_aligned(const void* p, const long long* st, int D, int es) {
   return st[3] == 1 && D % 4 == 0 && (uintptr_t)p % (4 * es) == 0 && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
 }
@@ -518,7 +511,7 @@ int prompt_simt(const PromptArgs& a, cudaStream_t s) {
                    rows_aligned(a.v, a.vs, a.D, sizeof(T));
   auto kern = prompt_simt_kernel<T, DP>;
   constexpr size_t bytes = Tile<4, DP>::kBytes;
-  if (set_smem(kern, bytes) != KVBM_OK) return KVBM_ERR_CUDA;
+  if (allow_smem(kern, bytes) != KVBM_OK) return KVBM_ERR_CUDA;
   kern<<<dim3((unsigned)((a.N + 63) / 64), (unsigned)(a.B * a.Hq)), kThreads, bytes, s>>>(a, vec);
   return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
 }
@@ -536,7 +529,7 @@ int cached_simt(const CachedArgs& a, cudaStream_t s) {
                    rows_aligned(a.v, a.vs, a.D, sizeof(T));
   auto kern = cached_simt_kernel<T, RPT, DP>;
   constexpr size_t bytes = Tile<RPT, DP>::kBytes;
-  if (set_smem(kern, bytes) != KVBM_OK) return KVBM_ERR_CUDA;
+  if (allow_smem(kern, bytes) != KVBM_OK) return KVBM_ERR_CUDA;
   kern<<<(unsigned)a.C, kThreads, bytes, s>>>(a, vec);
   return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
 }

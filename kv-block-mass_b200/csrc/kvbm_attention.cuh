@@ -189,6 +189,14 @@ int read_and_clear_attention_error(cudaStream_t s, int* err);         // waits t
 int read_and_clear_attention_page_error(cudaStream_t s, int* err);    // bad table entries (attention, eviction)
 unsigned int* attention_page_error_word();                            // its device address (or null)
 
+// Allows a kernel its dynamic shared memory (kvbm_attention_api.cu): set once
+// per kernel and device, 4 us of a call otherwise.
+int allow_smem_of(const void* kernel, size_t bytes);
+template <typename K>
+int allow_smem(K* kernel, size_t bytes) {
+  return allow_smem_of(reinterpret_cast<const void*>(kernel), bytes);
+}
+
 int attention_device_kind(int dev);  // 1: sm_100
 int attention_device_sms(int dev);
 

@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "kvbm_attention.cuh"
 
@@ -176,6 +177,24 @@ int this_device(int* dev) {
 }
 
 }  // namespace
+
+int allow_smem_of(const void* kernel, size_t bytes) {
+  // the last (kernel, device) pair set in each slot; two that share one only set it again
+  constexpr int kSlots = 256;
+  static std::atomic<uintptr_t> done[kSlots] = {};
+  int dev = -1;
+  if (this_device(&dev) != KVBM_OK) return KVBM_ERR_CUDA;
+  const uintptr_t key = (uintptr_t)kernel * 64 + (uintptr_t)dev + 1;
+  const int at = (int)((key * 0x9E3779B97F4A7C15ull) >> 56);
+  if (dev < 63 && done[at].load(std::memory_order_acquire) == key) return KVBM_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
+    cudaGetLastError();
+    return KVBM_ERR_CUDA;
+  }
+  if (dev < 63) done[at].store(key, std::memory_order_release);
+  return KVBM_OK;
+}
+
 }  // namespace kvbm
 
 using namespace kvbm;

@@ -583,8 +583,7 @@ int launch(const PromptArgs& a, cudaStream_t s) {
     return KVBM_ERR_CUDA;
   auto kern = prompt_tc_kernel<DP, kBf16>;
   constexpr size_t smem = Cfg<DP>::kSmem;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return KVBM_ERR_CUDA;
+  if (allow_smem(kern, smem) != KVBM_OK) return KVBM_ERR_CUDA;
   long long tiles = (long long)a.B * ((a.N + ROWS - 1) / ROWS);
   // packed rows make at most ceil(T / 256) + B tiles; one more CTA row for the rows of no sequence
   if (packed) tiles = std::min(tiles, (a.total + ROWS - 1) / ROWS + a.B) + 1;

@@ -451,8 +451,7 @@ template <int DP, bool kBf16>
 int launch(const CachedArgs& a, cudaStream_t s) {
   auto kern = cached_mma_kernel<DP, kBf16>;
   constexpr size_t bytes = Cfg<DP>::kSmem;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess)
-    return KVBM_ERR_CUDA;
+  if (allow_smem(kern, bytes) != KVBM_OK) return KVBM_ERR_CUDA;
   kern<<<(unsigned)a.C, kThreads, bytes, s>>>(a);
   return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
 }

@@ -24,7 +24,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _VALUE_ERRORS, _as_mask, _int32_on
+from .ops import _DTYPES, _VALUE_ERRORS, _as_mask
 
 __all__ = ["attention_b200", "attention_varlen", "attention_cached", "cached_attention_workspace_bytes"]
 
@@ -34,6 +34,28 @@ MAX_TREE_TOKENS = 64
 def _fail(code: int, what: str):
     msg = f"{what}: kvbm error {code}: {_lib.status_string(code)}"
     raise ValueError(msg) if code in _VALUE_ERRORS else RuntimeError(msg)
+
+
+_I3, _I4 = ctypes.c_int64 * 3, ctypes.c_int64 * 4
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _on_device(dev: torch.device, call):
+    """``call(stream)`` with ``dev`` current, on its current stream."""
+    if torch.cuda.current_device() == dev.index:
+        return call(torch.cuda.current_stream(dev).cuda_stream)
+    with torch.cuda.device(dev):
+        return call(torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _int32_on(t: torch.Tensor, dev, name: str) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dim() != 1:
+        raise ValueError(f"{name} must be a 1-D integer tensor")
+    if t.dtype == torch.int32 and t.device == dev and t.is_contiguous():
+        return t
+    if t.dtype.is_floating_point or t.dtype == torch.bool:
+        raise ValueError(f"{name} must hold integers, got {t.dtype}")
+    return t.to(device=dev, dtype=torch.int32).contiguous()
 
 
 def _same(name: str, t: torch.Tensor, like: torch.Tensor) -> None:
@@ -67,11 +89,11 @@ def _check_out(name: str, t: torch.Tensor, shape, dtype, device) -> None:
 
 
 def _check_qkv(q, k, v, what):
-    if not all(isinstance(t, torch.Tensor) for t in (q, k, v)):
+    if not (isinstance(q, torch.Tensor) and isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)):
         raise TypeError(f"{what}: q, k and v must be torch tensors")
     if not q.is_cuda:
         raise ValueError(f"{what} needs CUDA tensors (there is no CPU path)")
-    if q.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    if q.dtype not in _FLOATS:
         raise ValueError(f"unsupported dtype {q.dtype}; expected float32, bfloat16 or float16")
     _same("k", k, q)
     _same("v", v, q)
@@ -88,11 +110,8 @@ def _prompt(q, k, v, dims, strides, attn_mask, causal, scale, out, out_strides, 
     dev = q.device
     a = _lib.AttentionArgs()
     a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    for i in range(4):
-        a.q_stride[i], a.k_stride[i], a.v_stride[i] = strides[0][i], strides[1][i], strides[2][i]
-        a.out_stride[i] = out_strides[i]
-    for i in range(3):
-        a.lse_stride[i] = lse_strides[i]
+    a.q_stride, a.k_stride, a.v_stride = _I4(*strides[0]), _I4(*strides[1]), _I4(*strides[2])
+    a.out_stride, a.lse_stride = _I4(*out_strides), _I3(*lse_strides)
     a.dtype = _DTYPES[q.dtype]
     a.B, a.Hq, a.Hkv, a.N, a.D = B, Hq, Hkv, N, D
     keep = []
@@ -113,8 +132,7 @@ def _prompt(q, k, v, dims, strides, attn_mask, causal, scale, out, out_strides, 
         a.cu_seqlens, a.total_tokens = cu.data_ptr(), total
     a.fill_outside = int(fill)
     a.out, a.lse = out.data_ptr(), lse.data_ptr()
-    with torch.cuda.device(dev):
-        code = _lib.load().kvbm_attention(ctypes.byref(a), torch.cuda.current_stream(dev).cuda_stream)
+    code = _on_device(dev, lambda stream: _lib.load().kvbm_attention(ctypes.byref(a), stream))
     if code != _lib.KVBM_OK:
         _fail(code, "attention")
 
@@ -226,7 +244,7 @@ def _table(block_table, B, k_cache, q):
         raise ValueError("q, the caches and block_table must be on one device")
     if block_table.shape[1] == 0:
         raise ValueError("block_table names no pages")
-    t = block_table.to(torch.int32)
+    t = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)
     return (t if t.stride(1) == 1 else t.contiguous()), t.shape[1]
 
 
@@ -274,8 +292,7 @@ def _cached_args(q, k_cache, v_cache, block_table, seq_lens, tree_mask, log_offs
     a = _lib.CachedArgs()
     keep = [q, k_cache, v_cache, table, lens]
     a.q, a.k_cache, a.v_cache = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
-    for i in range(4):
-        a.q_stride[i], a.k_stride[i], a.v_stride[i] = q.stride(i), k_cache.stride(i), v_cache.stride(i)
+    a.q_stride, a.k_stride, a.v_stride = _I4(*q.stride()), _I4(*k_cache.stride()), _I4(*v_cache.stride())
     a.dtype = _DTYPES[q.dtype]
     a.B, a.Hq, a.Hkv, a.T, a.D = B, Hq, Hkv, T, D
     a.num_pages, a.page_size, a.max_pages = num_pages, page_size, max_pages
@@ -318,7 +335,8 @@ def _cached_args(q, k_cache, v_cache, block_table, seq_lens, tree_mask, log_offs
         _no_overlap("weights_out", wo, ins)
         keep += [w, wo]
     a.scale = float(1.0 / D ** 0.5 if scale is None else scale)
-    ins = {"q": q, "k_cache": k_cache, "v_cache": v_cache}
+    if out is not None or lse_out is not None:
+        ins = {"q": q, "k_cache": k_cache, "v_cache": v_cache}
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     else:
@@ -330,13 +348,7 @@ def _cached_args(q, k_cache, v_cache, block_table, seq_lens, tree_mask, log_offs
         _check_out("lse_out", lse_out, (B, Hq, T), torch.float32, q.device)
         _no_overlap("lse_out", lse_out, ins)
     a.out, a.lse = out.data_ptr(), lse_out.data_ptr()
-    for i in range(4):
-        a.out_stride[i] = out.stride(i)
-    for i in range(3):
-        a.lse_stride[i] = lse_out.stride(i)
-    code = _lib.load().kvbm_validate_cached_attention(ctypes.byref(a))
-    if code != _lib.KVBM_OK:
-        _fail(code, "attention_cached")
+    a.out_stride, a.lse_stride = _I4(*out.stride()), _I3(*lse_out.stride())
     return a, keep, out, lse_out, weights_out
 
 
@@ -345,8 +357,7 @@ def cached_attention_workspace_bytes(q, k_cache, v_cache, block_table, seq_lens,
     args = dict(tree_mask=None, log_offsets=None, weights=None, weights_out=None, scale=None, out=None, lse_out=None)
     args.update(kwargs)
     a, keep, *_ = _cached_args(q, k_cache, v_cache, block_table, seq_lens, **args)
-    with torch.cuda.device(q.device):
-        n = int(_lib.load().kvbm_cached_attention_workspace_bytes(ctypes.byref(a)))
+    n = int(_on_device(q.device, lambda _: _lib.load().kvbm_cached_attention_workspace_bytes(ctypes.byref(a))))
     del keep
     return n
 
@@ -385,15 +396,17 @@ def attention_cached(q, k_cache, v_cache, block_table, seq_lens, *, tree_mask=No
                                                       log_offsets, weights, weights_out, scale, out, lse_out)
     dev = q.device
     lib = _lib.load()
-    with torch.cuda.device(dev):
-        need = int(lib.kvbm_cached_attention_workspace_bytes(ctypes.byref(a)))
-        if workspace is None:
-            workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=dev)
-        elif workspace.device != dev or workspace.dtype != torch.uint8 or not workspace.is_contiguous() or \
-                workspace.numel() < need:
+
+    def launch(stream):
+        need = lib.kvbm_cached_attention_workspace_bytes(ctypes.byref(a))
+        ws = workspace
+        if ws is None:
+            ws = torch.empty(max(need, 256), dtype=torch.uint8, device=dev)
+        elif ws.device != dev or ws.dtype != torch.uint8 or not ws.is_contiguous() or ws.numel() < need:
             raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes on {dev}")
-        code = lib.kvbm_cached_attention(ctypes.byref(a), workspace.data_ptr(), workspace.numel(),
-                                         torch.cuda.current_stream(dev).cuda_stream)
+        return lib.kvbm_cached_attention(ctypes.byref(a), ws.data_ptr(), ws.numel(), stream)
+
+    code = _on_device(dev, launch)
     del keep
     if code != _lib.KVBM_OK:
         _fail(code, "attention_cached")

@@ -18,8 +18,8 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .attention import _check_out, _fail, _no_overlap, _per_key, _table
-from .ops import _DTYPES, _int32_on
+from .attention import _I4, _check_out, _fail, _int32_on, _no_overlap, _on_device, _per_key, _table
+from .ops import _DTYPES
 
 __all__ = ["EvictedCache", "evict_cache"]
 
@@ -78,7 +78,8 @@ def evict_cache(k_cache, v_cache, block_table, seq_lens, weights, budget, *, n_s
         if cap < budget:
             raise ValueError(f"capacity={cap} < budget={budget}")
         # a head's slots one after another: the next reader streams them
-        ko, vo = (torch.empty(B, Hkv, cap, D, dtype=k_cache.dtype, device=dev).transpose(1, 2) for _ in range(2))
+        both = torch.empty(2, B, Hkv, cap, D, dtype=k_cache.dtype, device=dev).transpose(2, 3)
+        ko, vo = both.unbind(0)
     else:
         ko, vo = out
         if not isinstance(ko, torch.Tensor) or ko.dim() != 4:
@@ -92,9 +93,8 @@ def evict_cache(k_cache, v_cache, block_table, seq_lens, weights, budget, *, n_s
         _no_overlap("out v", vo, {"out k": ko})
     a = _lib.EvictArgs()
     a.k_cache, a.v_cache, a.k_out, a.v_out = k_cache.data_ptr(), v_cache.data_ptr(), ko.data_ptr(), vo.data_ptr()
-    for i in range(4):
-        a.k_stride[i], a.v_stride[i] = k_cache.stride(i), v_cache.stride(i)
-        a.k_out_stride[i], a.v_out_stride[i] = ko.stride(i), vo.stride(i)
+    a.k_stride, a.v_stride = _I4(*k_cache.stride()), _I4(*v_cache.stride())
+    a.k_out_stride, a.v_out_stride = _I4(*ko.stride()), _I4(*vo.stride())
     a.dtype = _DTYPES[k_cache.dtype]
     a.B, a.Hkv, a.D = B, Hkv, D
     a.num_pages, a.page_size, a.max_pages = num_pages, page_size, max_pages
@@ -103,15 +103,14 @@ def evict_cache(k_cache, v_cache, block_table, seq_lens, weights, budget, *, n_s
     a.seq_lens = lens.data_ptr()
     a.weights, a.weights_bstride, a.weights_hstride, a.weight_heads = w.data_ptr(), wb, wh, Hw
     a.budget, a.n_sinks, a.recency, a.capacity, a.zero_tail = budget, n_sinks, recency, cap, int(out is None)
-    code = _lib.load().kvbm_validate_evict(ctypes.byref(a))  # k_out and the rest below are set when it passes
-    if code not in (_lib.KVBM_OK, _lib.KVBM_ERR_NULL):
-        _fail(code, "evict_cache")
-    with torch.cuda.device(dev):
-        new_lens = torch.empty(B, dtype=torch.int32, device=dev)
-        kept = torch.empty(B, Hw, budget, dtype=torch.int32, device=dev)
-        wout = torch.empty(B, Hw, budget, dtype=torch.float32, device=dev)
-        a.seq_lens_out, a.kept_out, a.weights_out = new_lens.data_ptr(), kept.data_ptr(), wout.data_ptr()
-        code = _lib.load().kvbm_evict_cache(ctypes.byref(a), torch.cuda.current_stream(dev).cuda_stream)
+    # one block of memory for the three small results: slots and lengths are int32, weights float32
+    n = B * Hw * budget
+    small = torch.empty(2 * n + B, dtype=torch.int32, device=dev)
+    kept, new_lens = small[:n].view(B, Hw, budget), small[2 * n:]
+    wout = small[n:2 * n].view(torch.float32).view(B, Hw, budget)
+    a.kept_out = small.data_ptr()
+    a.weights_out, a.seq_lens_out = a.kept_out + 4 * n, a.kept_out + 8 * n
+    code = _on_device(dev, lambda stream: _lib.load().kvbm_evict_cache(ctypes.byref(a), stream))
     if code != _lib.KVBM_OK:
         _fail(code, "evict_cache")
     return EvictedCache(k=ko, v=vo, seq_lens=new_lens, kept=kept, weights=wout)
