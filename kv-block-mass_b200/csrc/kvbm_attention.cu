@@ -420,9 +420,10 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(CachedArgs a, boo
 
 // Joins the partials of every split unit, and writes the rows of sequences
 // with no keys (out 0, lse -inf).  One warp per row, grid (B * Hkv * RT, BM / 8);
-// partials in CTA order: the same bits on every run.
+// partials in CTA order: the same bits on every run.  Lanes read 32 partials'
+// (m, l) at once and then stream their output rows, four loads in flight.
 template <typename T>
-__global__ void __launch_bounds__(256) cached_merge_kernel(CachedArgs a) {
+__global__ void __launch_bounds__(256) cached_merge_kernel(const __grid_constant__ CachedArgs a) {
   const int unit = blockIdx.x, b = unit / (a.Hkv * a.RT), u = unit % (a.Hkv * a.RT), g = u / a.RT, rt = u % a.RT;
   const int rl = blockIdx.y * 8 + threadIdx.x / 32, r = rt * a.BM + rl, lane = threadIdx.x & 31;
   if (rl >= a.BM || r >= a.R) return;
@@ -440,41 +441,61 @@ __global__ void __launch_bounds__(256) cached_merge_kernel(CachedArgs a) {
   const long long t0 = pre + (long long)u * nt, t1 = t0 + nt;
   const int i0 = (int)split_owner(t0, total, a.C), i1 = (int)split_owner(t1 - 1, total, a.C);
   if (i0 == i1) return;  // finished by its CTA
-  auto row_of = [&](int i) {
-    const int slot = split_begin(i, total, a.C) >= t0 ? 0 : 1;
-    return ((long long)i * 2 + slot) * a.BM + rl;
+  auto load_ml = [&](int i, long long* pr) {
+    *pr = 0;
+    if (i > i1) return make_float2(-INFINITY, 0.f);
+    const long long s0 = split_begin(i, total, a.C), s1 = split_begin(i + 1, total, a.C);
+    if (s0 == s1) return make_float2(-INFINITY, 0.f);  // a CTA without tiles
+    *pr = ((long long)i * 2 + (s0 >= t0 ? 0 : 1)) * a.BM + rl;
+    return a.part_ml[*pr];
   };
-  float m = -INFINITY;
-  bool bad = false;  // a NaN maximum can only come with a NaN sum
-  for (int i = i0 + lane; i <= i1; i += 32) {
-    if (split_begin(i, total, a.C) == split_begin(i + 1, total, a.C)) continue;  // a CTA without tiles
-    m = fmaxf(m, a.part_ml[row_of(i)].x);
+  long long pr;
+  float2 ml = load_ml(i0 + lane, &pr);
+  float m = ml.x;
+  for (int base = i0 + 32; base <= i1; base += 32) {
+    long long p2;
+    m = fmaxf(m, load_ml(base + lane, &p2).x);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  (void)bad;
-  const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f, acc[8];
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  const int lanes = a.DP < 128 ? a.DP / 4 : 32;  // lanes that hold four columns each (DP = 256: twice four)
+  for (int base = i0; base <= i1; base += 32) {
+    if (base > i0) ml = load_ml(base + lane, &pr);
+    // (a partial that kept nothing has l = 0; a NaN maximum gives a NaN factor)
+    const float f = ml.y == 0.f ? 0.f : exp2f((ml.x - ref) * kLog2eF);
+    float lp = ml.y * f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-  for (int i = i0; i <= i1; ++i) {
-    if (split_begin(i, total, a.C) == split_begin(i + 1, total, a.C)) continue;
-    const long long pr = row_of(i);
-    const float2 ml = a.part_ml[pr];
-    const float f = exp2f((ml.x - base) * kLog2eF);
-    if (ml.y == 0.f) continue;  // kept nothing
-    l += ml.y * f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int d = lane + 32 * e;
-      if (d < a.D) acc[e] = fmaf(a.part_o[pr * a.DP + d], f, acc[e]);
+    for (int o = 16; o > 0; o >>= 1) lp += __shfl_xor_sync(0xffffffffu, lp, o);
+    l += lp;
+    const int n = min(32, i1 - base + 1);
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {
+      const float fk = __shfl_sync(0xffffffffu, f, k);
+      const long long pk = __shfl_sync(0xffffffffu, pr, k);
+      if (fk == 0.f || lane >= lanes) continue;
+      const float4* src = reinterpret_cast<const float4*>(a.part_o + pk * a.DP) + lane;
+      const float4 x = src[0];
+      acc[0] = make_float4(fmaf(x.x, fk, acc[0].x), fmaf(x.y, fk, acc[0].y), fmaf(x.z, fk, acc[0].z),
+                           fmaf(x.w, fk, acc[0].w));
+      if (a.DP > 128) {
+        const float4 y = src[32];
+        acc[1] = make_float4(fmaf(y.x, fk, acc[1].x), fmaf(y.y, fk, acc[1].y), fmaf(y.z, fk, acc[1].z),
+                             fmaf(y.w, fk, acc[1].w));
+      }
     }
   }
   const float inv = 1.f / l;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int d = lane + 32 * e;
-    if (d < a.D) out[d * a.os[3]] = from_f32<T>(l == 0.f ? 0.f : acc[e] * inv);
+  for (int half = 0; half < 2; ++half) {
+    const float v[4] = {acc[half].x, acc[half].y, acc[half].z, acc[half].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = half * 128 + lane * 4 + e;
+      if (lane < lanes && d < a.D) out[d * a.os[3]] = from_f32<T>(l == 0.f ? 0.f : v[e] * inv);
+    }
   }
   if (lane == 0) {
     *lse = l == 0.f ? -INFINITY : m + logf(l);

@@ -99,7 +99,7 @@ struct Cfg {
   static constexpr int kPasses = KT / kRowsPerPass;
   static constexpr int kPitch = DP + 4;               // floats of a row of the joining buffer
   static constexpr size_t kRing = (size_t)kStages * 2 * kTileBytes;
-  static constexpr size_t kSmem = kRing + 2 * KT * 16 + BM * DP * 2 + 4 * BM * 8 + 64;
+  static constexpr size_t kSmem = kRing + (kStages + 1) * KT * 16 + BM * DP * 2 + 4 * BM * 8 + 64;
   static_assert(kRing >= sizeof(float) * 4 * BM * kPitch, "the joining buffer reuses the ring");
 };
 
@@ -109,8 +109,8 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) cached_mma_kernel
   using T = std::conditional_t<kBf16, __nv_bfloat16, __half>;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* ring = smem;
-  longlong2* offs = reinterpret_cast<longlong2*>(smem + CF::kRing);     // [2][KT] element offsets of k, v rows (-1: zeros)
-  uint8_t* qs = reinterpret_cast<uint8_t*>(offs + 2 * KT);              // [BM][DP] swizzled
+  longlong2* offs = reinterpret_cast<longlong2*>(smem + CF::kRing);     // [kStages + 1][KT] element offsets of k, v rows (-1: zeros)
+  uint8_t* qs = reinterpret_cast<uint8_t*>(offs + (CF::kStages + 1) * KT);              // [BM][DP] swizzled
   float2* ml_s = reinterpret_cast<float2*>(qs + BM * DP * 2);           // [4][BM]
   long long* sched = reinterpret_cast<long long*>(ml_s + 4 * BM);       // total, first, b
   volatile int* bad_flag = reinterpret_cast<volatile int*>(sched + 3);
@@ -149,16 +149,16 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) cached_mma_kernel
     const float* off = a.off ? a.off + b * a.ob + g * a.oh : nullptr;
     const uint8_t* tree = a.tree ? a.tree + b * a.tb : nullptr;
 
-    // ---- offsets of a tile's rows (threads 0 .. 63, one row each)
-    auto page_of = [&](int tile) -> int {  // the page id of this thread's row (-1: not in the cache)
-      const int c = tile * KT + tid;
-      if (tid >= KT || tile >= k1 || c >= len) return -1;
+    // ---- element offsets of a tile's rows, kStages tiles ahead of their use
+    auto page_of = [&](int tile, int i) -> int {  // the page id of row i of a tile (-1: none)
+      const int c = tile * KT + i;
+      if (tile >= k1 || c >= len) return -1;
       const int pi = c / a.pg.page_size;
       return a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
     };
-    auto put_offsets = [&](int tile, int page) {
-      if (tid >= KT || tile >= k1) return;
-      const int c = tile * KT + tid;
+    auto put_offsets = [&](int tile, int i, int page) {
+      if (tile >= k1) return;
+      const int c = tile * KT + i;
       longlong2 o = make_longlong2(-1, -1);
       if (c < len && !(off != nullptr && off[c] == -INFINITY)) {
         if (page >= 0 && page < a.pg.num_pages) {
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) cached_mma_kernel
           atomicOr(a.page_error, 1u);
         }
       }
-      offs[(tile & 1) * KT + tid] = o;
+      offs[((tile - k0) % (CF::kStages + 1)) * KT + i] = o;
     };
     auto load_tile = [&](int tile) {
       if (tile < k1) {
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) cached_mma_kernel
 #pragma unroll
         for (int i = 0; i < CF::kPasses; ++i) {
           const int r = tid / CF::kChunks + i * CF::kRowsPerPass;
-          const longlong2 o = offs[(tile & 1) * KT + r];
+          const longlong2 o = offs[((tile - k0) % (CF::kStages + 1)) * KT + r];
           const bool live = in && o.x >= 0;
           const uint32_t d = r * (DP * 2) + ((ch ^ (r & 7)) << 4);
           cp16(kd + d, live ? kbase + o.x + ch * 8 : kbase, live);
@@ -189,7 +189,19 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) cached_mma_kernel
       cp_commit();
     };
 
-    // ---- queries
+    // the first kStages tiles at once (their table reads overlap), then the queries
+    {
+      constexpr int kEach = (CF::kStages * KT + kThreads - 1) / kThreads;
+      int page[kEach];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) page[i] = page_of(k0 + (tid + i * kThreads) / KT, tid % KT);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (tid + i * kThreads < CF::kStages * KT) put_offsets(k0 + (tid + i * kThreads) / KT, tid % KT, page[i]);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = 0; i < CF::kStages - 1; ++i) load_tile(k0 + i);
     for (int i = tid; i < BM * CF::kChunks; i += kThreads) {
       const int r = i / CF::kChunks, ch = i % CF::kChunks, rr = rt * BM + r;
       uint4 w = make_uint4(0u, 0u, 0u, 0u);
@@ -199,16 +211,8 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) cached_mma_kernel
                                             (long long)(rr % a.T) * a.qs[2] + ch * 8);
       *reinterpret_cast<uint4*>(qs + r * (DP * 2) + ((ch ^ (r & 7)) << 4)) = w;
     }
-    // ---- fill the pipeline: offsets of tiles are written one step before their loads
-    put_offsets(k0, page_of(k0));
+    int next_page = tid < KT ? page_of(k0 + CF::kStages, tid) : -1;
     __syncthreads();
-#pragma unroll 1
-    for (int i = 0; i < CF::kStages - 1; ++i) {
-      load_tile(k0 + i);
-      put_offsets(k0 + i + 1, page_of(k0 + i + 1));
-      __syncthreads();
-    }
-    int next_page = page_of(k0 + CF::kStages);
 
     uint32_t qf[DP <= 128 ? DP / 16 : 1][4];
     const uint32_t q_row = (lane & 7) + ((lane >> 3) & 1) * 8, q_ch = lane >> 4;
@@ -242,8 +246,10 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) cached_mma_kernel
       cp_wait<CF::kStages - 2>();
       __syncthreads();
       load_tile(tile + CF::kStages - 1);
-      put_offsets(tile + CF::kStages, next_page);
-      next_page = page_of(tile + CF::kStages + 1);
+      if (tid < KT) {
+        put_offsets(tile + CF::kStages, tid, next_page);
+        next_page = page_of(tile + CF::kStages + 1, tid);
+      }
       const uint32_t kt = ring_a + ((tile - k0) % CF::kStages) * 2 * CF::kTileBytes + warp * 16 * (DP * 2);
       const uint32_t vt = kt + CF::kTileBytes;
       if (a.T > 1 && c0 + 16 > pre && c0 < len) {

@@ -18,7 +18,8 @@ namespace kvbm {
 namespace {
 
 constexpr int kSelThreads = 1024;
-constexpr int kGatherThreads = 256;
+constexpr int kGatherThreads = 512;  // one element a thread at D = 256: 2 * 256 threads a slot
+constexpr int kSmemKeys = 48 * 1024;
 constexpr int kGatherUnroll = 4;
 
 struct EvictArgs {
@@ -50,12 +51,20 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) {
-  __shared__ unsigned int hist[256];
-  __shared__ int scan_buf[kSelThreads / 32];
+// One CTA per (sequence, weight head).  The row's keys are read once into
+// shared memory (rows past kSmemKeys: re-read from L2 in every pass).
+// Threshold: three histogram passes of 11, 11 and 10 bits over the candidates;
+// in each warp the lanes that share the first lane's bin add once together,
+// since many weights are alike (keys nothing attended to).  Slots: each warp
+// takes a run of the row and counts its ties and kept tokens with ballots, one
+// scan over the warps, and a second walk writes.
+__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a, int smem_keys) {
+  extern __shared__ uint32_t keys_s[];
+  __shared__ unsigned int hist[2048];
+  __shared__ int scan_buf[kSelThreads / 32], warp_ties[kSelThreads / 32], warp_gt[kSelThreads / 32];
   __shared__ unsigned int s_prefix;
   __shared__ int s_left;
-  const int row = blockIdx.x, b = row / a.Hw, hw = row % a.Hw, t = threadIdx.x;
+  const int row = blockIdx.x, b = row / a.Hw, hw = row % a.Hw, t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int len = evict_len(a, b);
   const float* w = a.w + b * a.wb + hw * a.wh;
   int32_t* kept = a.kept + (long long)row * a.budget;
@@ -75,118 +84,142 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a) 
   }
   const int lo = a.n_sinks, hi = len - a.recency;  // the candidates; budget >= n_sinks + recency, so lo <= hi
   const int take = a.budget - a.n_sinks - a.recency;
+  const bool cached = len <= smem_keys;
+  if (cached) {
+#pragma unroll 8
+    for (int c = t; c < len; c += kSelThreads) keys_s[c] = weight_key(w[c]);
+  }
+  auto key_at = [&](int c) { return cached ? keys_s[c] : weight_key(w[c]); };
   // 1. threshold key of the `take` highest candidates, and how many of its
   //    ties are taken (from the lowest index)
   if (t == 0) {
     s_prefix = 0;
     s_left = take;
   }
-  __syncthreads();
   if (take > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = t; i < 256; i += kSelThreads) hist[i] = 0;
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+      for (int i = t; i < 2048; i += kSelThreads) hist[i] = 0;
       __syncthreads();
-      const uint32_t pre = s_prefix, high = shift == 24 ? 0u : ~0u << (shift + 8);
-      for (int c = lo + t; c < hi; c += kSelThreads) {
-        const uint32_t key = weight_key(w[c]);
-        if (((key ^ pre) & high) == 0) atomicAdd(&hist[(key >> shift) & 255u], 1u);
+      const uint32_t pre = s_prefix, high = pass == 0 ? 0u : ~0u << (shift + bits), mask = (1u << bits) - 1u;
+#pragma unroll 4
+      for (int c0 = lo + warp * 32; c0 < hi; c0 += kSelThreads) {
+        const int c = c0 + lane;
+        const uint32_t key = c < hi ? key_at(c) : 0u;
+        const bool in = c < hi && ((key ^ pre) & high) == 0;
+        const unsigned act = __ballot_sync(0xffffffffu, in);
+        if (act == 0) continue;
+        const uint32_t bin = (key >> shift) & mask;
+        const int first = __ffs(act) - 1;
+        const uint32_t bin0 = __shfl_sync(0xffffffffu, bin, first);
+        const unsigned same = __ballot_sync(0xffffffffu, in && bin == bin0);
+        if (lane == first) atomicAdd(&hist[bin0], (unsigned)__popc(same));
+        if (in && bin != bin0) atomicAdd(&hist[bin], 1u);
       }
       __syncthreads();
-      if (t < 32) {
-        // lane l owns bins [248 - 8l, 256 - 8l), counted from the top
-        const int left = s_left;
-        int mine = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) mine += hist[255 - 8 * t - j];
-        int incl = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, incl, o);
-          if (t >= o) incl += y;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, incl >= left);
-        if (t == __ffs(hit) - 1) {
-          int above = incl - mine, v = 255 - 8 * t;
-          for (int j = 0; j < 7 && above + (int)hist[v] < left; ++j, --v) above += hist[v];
-          s_left = left - above;
-          s_prefix = pre | ((uint32_t)v << shift);
-        }
+      // thread t owns bins 2047 - 2t and 2046 - 2t, counted from the top (1024 threads, 2048 bins)
+      const int left = s_left;
+      const int h0 = (int)hist[2047 - 2 * t], h1 = (int)hist[2046 - 2 * t];
+      int all;
+      const int above = block_exclusive_scan<int, kSelThreads>(h0 + h1, scan_buf, &all);
+      if (above < left && above + h0 + h1 >= left) {
+        const bool second = above + h0 < left;
+        s_left = left - above - (second ? h0 : 0);
+        s_prefix = pre | ((uint32_t)(second ? 2046 - 2 * t : 2047 - 2 * t) << shift);
       }
       __syncthreads();
     }
+  } else {
+    __syncthreads();
   }
   const uint32_t thr = s_prefix;
   const int ties = s_left;
-  // 2. slots in index order
-  int out = 0, seen = 0;  // kept before this chunk, ties met before it
-  for (int base = 0; base < len; base += kSelThreads) {
-    const int c = base + t;
+  // 2. slots in index order: warp i walks tokens [i * run, (i + 1) * run)
+  const int run = ((len + kSelThreads - 1) / kSelThreads) * 32;
+  const int c_lo = warp * run, c_hi = min(len, c_lo + run);
+  int ngt = 0, ntie = 0;
+#pragma unroll 4
+  for (int c0 = c_lo; c0 < c_hi; c0 += 32) {
+    const int c = c0 + lane;
     const bool cand = c >= lo && c < hi && take > 0;
-    float wc = c < len ? w[c] : 0.f;
-    const uint32_t key = cand ? weight_key(wc) : 0u;
-    const bool tie = cand && key == thr;
-    int ntie = 0, nkeep = 0;
-    const int before = seen + block_exclusive_scan<int, kSelThreads>(tie ? 1 : 0, scan_buf, &ntie);
-    const bool keep = c < len && (c < lo || c >= hi || (cand && (key > thr || (tie && before < ties))));
-    const int slot = out + block_exclusive_scan<int, kSelThreads>(keep ? 1 : 0, scan_buf, &nkeep);
+    const uint32_t key = cand && c < c_hi ? key_at(c) : 0u;
+    ngt += __popc(__ballot_sync(0xffffffffu, c < c_hi && (c < lo || c >= hi || (cand && key > thr))));
+    ntie += __popc(__ballot_sync(0xffffffffu, cand && c < c_hi && key == thr));
+  }
+  if (lane == 0) {
+    warp_ties[warp] = ntie;
+    warp_gt[warp] = ngt;
+  }
+  __syncthreads();
+  int seen = 0, out = 0;
+  for (int i = 0; i < warp; ++i) {
+    out += warp_gt[i] + max(0, min(warp_ties[i], ties - seen));
+    seen += warp_ties[i];
+  }
+#pragma unroll 2
+  for (int c0 = c_lo; c0 < c_hi; c0 += 32) {
+    const int c = c0 + lane;
+    const bool cand = c >= lo && c < hi && take > 0 && c < c_hi;
+    const uint32_t key = cand ? key_at(c) : 0u;
+    const unsigned below = (1u << lane) - 1u;
+    const unsigned tie = __ballot_sync(0xffffffffu, cand && key == thr);
+    const bool keep = c < c_hi && (c < lo || c >= hi ||
+                                   (cand && (key > thr || (key == thr && seen + __popc(tie & below) < ties))));
+    const unsigned km = __ballot_sync(0xffffffffu, keep);
     if (keep) {
+      const int slot = out + __popc(km & below);
       kept[slot] = c;
-      if (wout) wout[slot] = wc;
+      if (wout) wout[slot] = w[c];
     }
-    out += nkeep;
-    seen += ntie;
+    out += __popc(km);
+    seen += __popc(tie);
   }
 }
 
-// One thread moves one V (16 bytes, or one element) of the k and of the v row
-// of one slot; strides in V units.
+// Grid (slot groups, B * Hkv).  2 * dv threads move one slot: the first dv
+// its k row, the others its v row, one V (16 bytes, or one element) each;
+// kGatherUnroll slots a thread, all their loads before the stores.  Strides in
+// V units.
 template <typename V>
-__global__ void __launch_bounds__(kGatherThreads) evict_gather_kernel(EvictArgs a, int dv) {
-  const int rpb = kGatherThreads / dv;
-  const int t = threadIdx.x;
-  if (t >= rpb * dv) return;
-  const int d = t % dv;
-  const long long rows = (long long)a.B * a.capacity * a.Hkv, step = (long long)gridDim.x * rpb;
-  const V *k = reinterpret_cast<const V*>(a.k), *v = reinterpret_cast<const V*>(a.v);
-  V *ko = reinterpret_cast<V*>(a.ko), *vo = reinterpret_cast<V*>(a.vo);
-  for (long long r0 = (long long)blockIdx.x * rpb + t / dv; r0 < rows; r0 += kGatherUnroll * step) {
-    V kv[kGatherUnroll], vv[kGatherUnroll];
-    long long dk[kGatherUnroll], dvv[kGatherUnroll];
-    bool put[kGatherUnroll];
+__global__ void __launch_bounds__(kGatherThreads) evict_gather_kernel(EvictArgs a, int dv, int rows) {
+  const int spb = kGatherThreads / (2 * dv);  // slots a step
+  const int t = threadIdx.x, s = t / (2 * dv), e = t % (2 * dv);
+  if (s >= spb) return;
+  const bool isv = e >= dv;
+  const int d = isv ? e - dv : e;
+  const int b = blockIdx.y / a.Hkv, g = blockIdx.y % a.Hkv;
+  const int new_len = min(evict_len(a, b), a.budget);
+  const int32_t* kept = a.kept + ((long long)b * a.Hw + (a.Hw > 1 ? g : 0)) * a.budget;
+  const long long* st = isv ? a.vs : a.ks;
+  const long long* ot = isv ? a.vos : a.kos;
+  const V* src = reinterpret_cast<const V*>(isv ? a.v : a.k) + g * st[2] + d * st[3];
+  V* dst = reinterpret_cast<V*>(isv ? a.vo : a.ko) + b * ot[0] + g * ot[2] + d * ot[3];
+  const int j0 = blockIdx.x * spb * kGatherUnroll + s;
+  int c[kGatherUnroll], page[kGatherUnroll];
 #pragma unroll
-    for (int i = 0; i < kGatherUnroll; ++i) {
-      const long long r = r0 + i * step;
-      kv[i] = V{};
-      vv[i] = V{};
-      put[i] = false;
-      if (r >= rows) continue;
-      const int g = (int)(r % a.Hkv);
-      const long long bj = r / a.Hkv;
-      const int j = (int)(bj % a.capacity), b = (int)(bj / a.capacity);
-      dk[i] = b * a.kos[0] + j * a.kos[1] + g * a.kos[2] + d * a.kos[3];
-      dvv[i] = b * a.vos[0] + j * a.vos[1] + g * a.vos[2] + d * a.vos[3];
-      if (j >= min(evict_len(a, b), a.budget)) {
-        put[i] = a.zero_tail != 0;
-        continue;
-      }
-      put[i] = true;
-      const int c = a.kept[((long long)b * a.Hw + (a.Hw > 1 ? g : 0)) * a.budget + j];
-      const int pi = c / a.pg.page_size;
-      const int page = a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
-      if (page >= 0 && page < a.pg.num_pages) {
-        const long long in = c - pi * a.pg.page_size;
-        kv[i] = k[page * a.ks[0] + in * a.ks[1] + g * a.ks[2] + d * a.ks[3]];
-        vv[i] = v[page * a.vs[0] + in * a.vs[1] + g * a.vs[2] + d * a.vs[3]];
-      } else if (d == 0) {
-        atomicOr(a.page_error, 1u);
-      }
-    }
+  for (int i = 0; i < kGatherUnroll; ++i) {
+    const int j = j0 + i * spb;
+    c[i] = j < new_len ? kept[j] : -1;
+  }
 #pragma unroll
-    for (int i = 0; i < kGatherUnroll; ++i) {
-      if (!put[i]) continue;
-      ko[dk[i]] = kv[i];
-      vo[dvv[i]] = vv[i];
-    }
+  for (int i = 0; i < kGatherUnroll; ++i) {
+    const int pi = c[i] / a.pg.page_size;
+    page[i] = c[i] < 0 ? -1 : a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
+  }
+  V v[kGatherUnroll];
+#pragma unroll
+  for (int i = 0; i < kGatherUnroll; ++i) {
+    v[i] = V{};
+    if (c[i] < 0) continue;
+    if (page[i] >= 0 && page[i] < a.pg.num_pages)
+      v[i] = src[page[i] * st[0] + (long long)(c[i] % a.pg.page_size) * st[1]];
+    else if (d == 0)
+      atomicOr(a.page_error, 1u);
+  }
+#pragma unroll
+  for (int i = 0; i < kGatherUnroll; ++i) {
+    const int j = j0 + i * spb;
+    if (j < new_len || (a.zero_tail && j < rows)) dst[j * ot[1]] = v[i];
   }
 }
 
@@ -203,11 +236,10 @@ int launch_gather(EvictArgs a, int es, cudaStream_t s) {
       a.vos[i] = i == 3 ? 1 : a.vos[i] / per;
     }
   const int dv = a.D / per;
-  const long long rows = (long long)a.B * (a.zero_tail ? a.capacity : a.budget) * a.Hkv;
-  const int rpb = kGatherThreads / dv;
-  long long blocks = (rows + rpb - 1) / rpb;
-  if (blocks > 148LL * 8) blocks = 148LL * 8;
-  evict_gather_kernel<V><<<(unsigned)blocks, kGatherThreads, 0, s>>>(a, dv);
+  const int rows = a.zero_tail ? a.capacity : a.budget;
+  const int per_block = kGatherThreads / (2 * dv) * kGatherUnroll;
+  const long long blocks = ((long long)rows + per_block - 1) / per_block;
+  evict_gather_kernel<V><<<dim3((unsigned)blocks, (unsigned)(a.B * a.Hkv)), kGatherThreads, 0, s>>>(a, dv, rows);
   return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
 }
 
@@ -285,7 +317,9 @@ extern "C" int kvbm_evict_cache(const kvbm_evict_args* e, void* stream) {
   a.wout = e->weights_out;
   a.page_error = attention_page_error_word();
   if (a.page_error == nullptr) return KVBM_ERR_CUDA;
-  evict_select_kernel<<<(unsigned)(a.B * a.Hw), kSelThreads, 0, s>>>(a);
+  const int smem_keys = a.Lmax < kSmemKeys ? a.Lmax : kSmemKeys;
+  if (allow_smem(evict_select_kernel, kSmemKeys * sizeof(uint32_t)) != KVBM_OK) return KVBM_ERR_CUDA;
+  evict_select_kernel<<<(unsigned)(a.B * a.Hw), kSelThreads, smem_keys * sizeof(uint32_t), s>>>(a, smem_keys);
   if (cudaGetLastError() != cudaSuccess) return KVBM_ERR_CUDA;
   const int es = esize(e->dtype);
   if ((a.D * es) % 16 == 0 && vec16(e->k_cache, e->k_stride, es) && vec16(e->v_cache, e->v_stride, es) &&
