@@ -93,6 +93,7 @@ struct Smem {
 template <typename T, int RPT, int DP, class F>
 __device__ __forceinline__ void load_rows(float* dst, int rows, F&& f, int D, long long ds, bool vec) {
   constexpr int kVecs = DP / 4;
+#pragma unroll 4
   for (int i = threadIdx.x; i < rows * kVecs; i += kThreads) {
     const int r = i / kVecs, d = (i % kVecs) * 4;
     *reinterpret_cast<float4*>(dst + r * (DP + kPad) + d) = load4<T>(f(r), d, D, ds, vec);
@@ -301,13 +302,15 @@ __global__ void __launch_bounds__(kThreads) prompt_fill_kernel(PromptArgs a) {
 // when it is the CTA's first unit and slot 1 when a later one, which
 // cached_merge_kernel joins in CTA order.
 template <typename T, int RPT, int DP>
-__global__ void __launch_bounds__(kThreads) cached_simt_kernel(CachedArgs a, bool vec) {
+__global__ void __launch_bounds__(kThreads) cached_simt_kernel(const __grid_constant__ CachedArgs a, bool vec) {
   extern __shared__ float smem[];
   constexpr int BM = 16 * RPT;
   Smem<RPT, DP> s(smem);
   __shared__ long long sh_first, sh_total;
   __shared__ int sh_b;
+  __shared__ longlong2 offs[BN];  // element offsets of the tile's k and v rows (-1: a zero row)
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  cudaTriggerProgrammaticLaunchCompletion();  // the joining kernel may be set up beside this one
   if (threadIdx.x < 32) {
     long long pre, total, first = 0;
     warp_tile_prefix(a, 0, &pre, &total);
@@ -352,21 +355,27 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(CachedArgs a, boo
         a.D, a.qs[3], vec);
     for (int kt = k0; kt < k1; ++kt) {
       const int c0 = kt * BN;
-      __syncthreads();
-      auto at_slot = [&](const void* base, const long long* st, int j) -> const T* {
-        const int c = c0 + j;
-        if (c >= len || (off != nullptr && off[c] == -INFINITY)) return nullptr;
-        const int pi = c / a.pg.page_size;
-        const int page = a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
-        if (page < 0 || page >= a.pg.num_pages) {
-          atomicOr(&g_attention_page_error, 1u);
-          return nullptr;
+      if (threadIdx.x < BN) {
+        const int c = c0 + threadIdx.x;
+        longlong2 o = make_longlong2(-1, -1);
+        if (c < len && !(off != nullptr && off[c] == -INFINITY)) {
+          const int pi = c / a.pg.page_size, in = c - pi * a.pg.page_size;
+          const int page = a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
+          if (page >= 0 && page < a.pg.num_pages) {
+            o.x = (long long)page * a.ks[0] + (long long)in * a.ks[1] + g * a.ks[2];
+            o.y = (long long)page * a.vs[0] + (long long)in * a.vs[1] + g * a.vs[2];
+          } else {
+            atomicOr(&g_attention_page_error, 1u);
+          }
         }
-        return static_cast<const T*>(base) + (long long)page * st[0] + (long long)(c - pi * a.pg.page_size) * st[1] +
-               g * st[2];
-      };
-      load_rows<T, RPT, DP>(s.k, BN, [&](int j) { return at_slot(a.k, a.ks, j); }, a.D, a.ks[3], vec);
-      load_rows<T, RPT, DP>(s.v, BN, [&](int j) { return at_slot(a.v, a.vs, j); }, a.D, a.vs[3], vec);
+        offs[threadIdx.x] = o;
+      }
+      __syncthreads();
+      const T *kp = static_cast<const T*>(a.k), *vp = static_cast<const T*>(a.v);
+      load_rows<T, RPT, DP>(s.k, BN, [&](int j) { return offs[j].x >= 0 ? kp + offs[j].x : nullptr; }, a.D, a.ks[3],
+                            vec);
+      load_rows<T, RPT, DP>(s.v, BN, [&](int j) { return offs[j].y >= 0 ? vp + offs[j].y : nullptr; }, a.D, a.vs[3],
+                            vec);
       if (off != nullptr && threadIdx.x < BN) {
         const int c = c0 + threadIdx.x;
         s.bias[threadIdx.x] = c < len ? off[c] : -INFINITY;
@@ -421,15 +430,18 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(CachedArgs a, boo
 // Joins the partials of every split unit, and writes the rows of sequences
 // with no keys (out 0, lse -inf).  One warp per row, grid (B * Hkv * RT, BM / 8);
 // partials in CTA order: the same bits on every run.  Lanes read 32 partials'
-// (m, l) at once and then stream their output rows, four loads in flight.
+// (m, l) at once and then stream their output rows, eight loads in flight.
 template <typename T>
 __global__ void __launch_bounds__(256) cached_merge_kernel(const __grid_constant__ CachedArgs a) {
   const int unit = blockIdx.x, b = unit / (a.Hkv * a.RT), u = unit % (a.Hkv * a.RT), g = u / a.RT, rt = u % a.RT;
   const int rl = blockIdx.y * 8 + threadIdx.x / 32, r = rt * a.BM + rl, lane = threadIdx.x & 31;
-  if (rl >= a.BM || r >= a.R) return;
   long long pre, total;
   warp_tile_prefix(a, b, &pre, &total);
   const int nt = (cached_len(a, b) + a.KT - 1) / a.KT;
+  // launched while the split kernel runs: what is above overlaps it, and every
+  // thread waits here for its results
+  cudaGridDependencySynchronize();
+  if (rl >= a.BM || r >= a.R) return;
   const int h = g * a.G + r / a.T, tok = r % a.T;
   T* out = static_cast<T*>(a.out) + b * a.os[0] + h * a.os[1] + tok * a.os[2];
   float* lse = a.lse + b * a.ls[0] + h * a.ls[1] + tok * a.ls[2];
@@ -471,19 +483,25 @@ __global__ void __launch_bounds__(256) cached_merge_kernel(const __grid_constant
     for (int o = 16; o > 0; o >>= 1) lp += __shfl_xor_sync(0xffffffffu, lp, o);
     l += lp;
     const int n = min(32, i1 - base + 1);
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) {
-      const float fk = __shfl_sync(0xffffffffu, f, k);
-      const long long pk = __shfl_sync(0xffffffffu, pr, k);
-      if (fk == 0.f || lane >= lanes) continue;
-      const float4* src = reinterpret_cast<const float4*>(a.part_o + pk * a.DP) + lane;
-      const float4 x = src[0];
-      acc[0] = make_float4(fmaf(x.x, fk, acc[0].x), fmaf(x.y, fk, acc[0].y), fmaf(x.z, fk, acc[0].z),
-                           fmaf(x.w, fk, acc[0].w));
-      if (a.DP > 128) {
-        const float4 y = src[32];
-        acc[1] = make_float4(fmaf(y.x, fk, acc[1].x), fmaf(y.y, fk, acc[1].y), fmaf(y.z, fk, acc[1].z),
-                             fmaf(y.w, fk, acc[1].w));
+    for (int k0 = 0; k0 < n; k0 += 8) {
+      float4 x[8], y[8];
+      float fk[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        fk[i] = __shfl_sync(0xffffffffu, f, (k0 + i) & 31);
+        const long long pk = __shfl_sync(0xffffffffu, pr, (k0 + i) & 31);
+        const bool in = k0 + i < n && fk[i] != 0.f && lane < lanes;
+        const float4* src = reinterpret_cast<const float4*>(a.part_o + pk * a.DP) + lane;
+        x[i] = y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (in) x[i] = src[0];
+        if (in && a.DP > 128) y[i] = src[32];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        acc[0] = make_float4(fmaf(x[i].x, fk[i], acc[0].x), fmaf(x[i].y, fk[i], acc[0].y),
+                             fmaf(x[i].z, fk[i], acc[0].z), fmaf(x[i].w, fk[i], acc[0].w));
+        acc[1] = make_float4(fmaf(y[i].x, fk[i], acc[1].x), fmaf(y[i].y, fk[i], acc[1].y),
+                             fmaf(y[i].z, fk[i], acc[1].z), fmaf(y[i].w, fk[i], acc[1].w));
       }
     }
   }
@@ -506,20 +524,68 @@ __global__ void __launch_bounds__(256) cached_merge_kernel(const __grid_constant
 // weights_out[b, g, c] = weights[b, g, c] + sum over the group's heads of
 // exp(x - m) / l, c < len.  From the stored scores (G * 4 bytes a key next to
 // the 4 D bytes of its k and v rows) rather than from a second pass over k.
-__global__ void __launch_bounds__(256) cached_weights_kernel(CachedArgs a) {
+// kVec: four keys a thread (aligned rows).
+template <int kVec>
+__global__ void __launch_bounds__(256) cached_weights_kernel(const __grid_constant__ CachedArgs a) {
   const int b = blockIdx.y / a.Hkv, g = blockIdx.y % a.Hkv;
   const int len = cached_len(a, b);
-  const float* sc = a.scores + (long long)blockIdx.y * a.G * a.Lmax;
-  const float2* st = a.stats + (long long)blockIdx.y * a.R;
-  for (int c = blockIdx.x * 256 + threadIdx.x; c < len; c += gridDim.x * 256) {
-    float sum = 0.f;
-    for (int hh = 0; hh < a.G; ++hh) {
-      const float2 ml = st[hh];
-      const float base = ml.x == -INFINITY ? 0.f : ml.x;
-      sum = fmaf(exp2f((sc[(long long)hh * a.Lmax + c] - base) * kLog2eF), ml.y, sum);
+  const int c = (blockIdx.x * 256 + threadIdx.x) * kVec;
+  const float* w = a.w + b * a.wb + g * a.wh + c;
+  float* wo = a.wout + b * a.wob + g * a.woh + c;
+  float sum[kVec];
+  alignas(16) float old[kVec];
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) sum[e] = old[e] = 0.f;
+  if (c < len) {
+    if (kVec == 4 && c + 4 <= len) {
+      *reinterpret_cast<float4*>(old) = *reinterpret_cast<const float4*>(w);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e)
+        if (c + e < len) old[e] = w[e];
     }
-    a.wout[b * a.wob + g * a.woh + c] = a.w[b * a.wb + g * a.wh + c] + sum;
   }
+  cudaGridDependencySynchronize();  // the weights were there before; scores and row statistics are now
+  if (c >= len) return;
+  const float* sc = a.scores + (long long)blockIdx.y * a.G * a.Lmax + c;
+  const float2* st = a.stats + (long long)blockIdx.y * a.R;
+#pragma unroll 4
+  for (int hh = 0; hh < a.G; ++hh) {
+    const float2 ml = st[hh];
+    const float base = ml.x == -INFINITY ? 0.f : ml.x;
+    float x[kVec];
+    if constexpr (kVec == 4) {
+      // (inside the row: Lmax % 4 == 0)
+      const float4 v = *reinterpret_cast<const float4*>(sc + (long long)hh * a.Lmax);
+      x[0] = v.x;
+      x[1] = v.y;
+      x[2] = v.z;
+      x[3] = v.w;
+    } else {
+      x[0] = sc[(long long)hh * a.Lmax];
+    }
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) sum[e] = fmaf(exp2f((x[e] - base) * kLog2eF), ml.y, sum[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < kVec; ++e)
+    if (c + e < len) wo[e] = old[e] + sum[e];
+}
+
+// Launches a kernel that may start before the one ahead of it on the stream
+// has ended (it waits for it itself, in cudaGridDependencySynchronize).
+template <typename... P, typename... A>
+int launch_dependent(void (*kernel)(P...), dim3 grid, unsigned threads, cudaStream_t s, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
 }
 
 bool rows_aligned(const void* p, const long long* st, int D, int es) {
@@ -596,19 +662,17 @@ int launch_cached_simt(const CachedArgs& a, int dtype, cudaStream_t s) {
 int launch_cached_merge(const CachedArgs& a, int dtype, cudaStream_t s) {
   const int rows = a.R < a.BM ? a.R : a.BM;
   const dim3 grid((unsigned)(a.B * a.Hkv * a.RT), (unsigned)((rows + 7) / 8));
-  if (dtype == KVBM_F32)
-    cached_merge_kernel<float><<<grid, 256, 0, s>>>(a);
-  else if (dtype == KVBM_BF16)
-    cached_merge_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
-  else
-    cached_merge_kernel<__half><<<grid, 256, 0, s>>>(a);
-  return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
+  if (dtype == KVBM_F32) return launch_dependent(cached_merge_kernel<float>, grid, 256, s, a);
+  if (dtype == KVBM_BF16) return launch_dependent(cached_merge_kernel<__nv_bfloat16>, grid, 256, s, a);
+  return launch_dependent(cached_merge_kernel<__half>, grid, 256, s, a);
 }
 
 int launch_cached_weights(const CachedArgs& a, cudaStream_t s) {
-  const int blocks = (a.Lmax + 255) / 256;
-  cached_weights_kernel<<<dim3((unsigned)(blocks < 1024 ? blocks : 1024), (unsigned)(a.B * a.Hkv)), 256, 0, s>>>(a);
-  return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
+  const bool vec = a.Lmax % 4 == 0 && (uintptr_t)a.w % 16 == 0 && a.wb % 4 == 0 && a.wh % 4 == 0;
+  const int per = vec ? 1024 : 256;
+  const dim3 grid((unsigned)((a.Lmax + per - 1) / per), (unsigned)(a.B * a.Hkv));
+  return vec ? launch_dependent(cached_weights_kernel<4>, grid, 256, s, a)
+             : launch_dependent(cached_weights_kernel<1>, grid, 256, s, a);
 }
 
 int read_and_clear_attention_page_error(cudaStream_t s, int* err) {

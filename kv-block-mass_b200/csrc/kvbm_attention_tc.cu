@@ -361,12 +361,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int s = j % kStages;
         if (!mbar_wait(&v_raw[s], ((j - js) / kStages) & 1, abort_flag)) break;
         uint8_t* tile = v_ring + s * CF::kTileBytes;
-        for (int i = st; i < CF::kBlocks * TILE * 8; i += kScrubThreads) {
-          const int row = (i >> 3) & (TILE - 1), c = j * TILE + row;
-          uint4* p = reinterpret_cast<uint4*>(tile + i * 16);
-          if (c >= n || (km != nullptr && km[c] == 0)) {
-            *p = make_uint4(0u, 0u, 0u, 0u);
-          } else if (a.causal && j >= 2 * qt) {
+        // rows that nobody keeps: zeros (a row is whole 128-byte pieces, however swizzled inside)
+        for (int row = st; row < TILE; row += kScrubThreads) {
+          const int c = j * TILE + row;
+          if (c < n && (km == nullptr || km[c] != 0)) continue;
+#pragma unroll
+          for (int i = 0; i < CF::kBlocks * 8; ++i)
+            *reinterpret_cast<uint4*>(tile + (i >> 3) * CF::kBlockBytes + row * 128 + (i & 7) * 16) =
+                make_uint4(0u, 0u, 0u, 0u);
+        }
+        // diagonal tiles: rows keep different keys
+        if (a.causal && j >= 2 * qt) {
+          for (int i = st; i < CF::kBlocks * TILE * 8; i += kScrubThreads) {
+            uint4* p = reinterpret_cast<uint4*>(tile + i * 16);
             const uint4 w = *p;
             uint32_t x[4] = {w.x, w.y, w.z, w.w};
             bool bad = false;
@@ -381,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 bad = true;
               }
             }
-            if (bad) {
+            if (bad && j * TILE + ((i >> 3) & (TILE - 1)) < n) {
               *p = make_uint4(x[0], x[1], x[2], x[3]);
               *bad_flag = 1;
             }

@@ -115,6 +115,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) cached_mma_kernel
   long long* sched = reinterpret_cast<long long*>(ml_s + 4 * BM);       // total, first, b
   volatile int* bad_flag = reinterpret_cast<volatile int*>(sched + 3);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  cudaTriggerProgrammaticLaunchCompletion();  // the joining kernel may be set up beside this one
   if (warp == 0) {
     long long pre, total, first = 0;
     warp_tile_prefix(a, 0, &pre, &total);

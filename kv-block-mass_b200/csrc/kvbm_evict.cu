@@ -10,6 +10,7 @@
 // turns the choice into slots with one scan: 4 * len bytes of weights are all
 // it reads from DRAM.  evict_gather_kernel moves the kept k and v rows, 16
 // bytes a thread: 4 * budget * D elements a head, bound by DRAM.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include "kvbm_attention.cuh"
@@ -51,32 +52,45 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// One CTA per (sequence, weight head).  The row's keys are read once into
-// shared memory (rows past kSmemKeys: re-read from L2 in every pass).
-// Threshold: three histogram passes of 11, 11 and 10 bits over the candidates;
-// in each warp the lanes that share the first lane's bin add once together,
-// since many weights are alike (keys nothing attended to).  Slots: each warp
-// takes a run of the row and counts its ties and kept tokens with ballots, one
-// scan over the warps, and a second walk writes.
+// A cluster of kCluster CTAs per (sequence, weight head); each takes a run of
+// the row and reads its keys once into shared memory (runs past kSmemKeys:
+// re-read from L2 in every pass).  Threshold: three histogram passes of 11, 11
+// and 10 bits over the candidates; in each warp the lanes that share the first
+// lane's bin add once together, since many weights are alike (keys nothing
+// attended to); the CTAs' histograms meet in the first CTA's shared memory.
+// Slots: each warp takes a part of its CTA's run and counts its ties and kept
+// tokens with ballots; sums over the warps and CTAs before it give its first
+// slot, and a second walk writes.
+template <int kCluster>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a, int smem_keys) {
+  namespace cg = cooperative_groups;
   extern __shared__ uint32_t keys_s[];
   __shared__ unsigned int hist[2048];
   __shared__ int scan_buf[kSelThreads / 32], warp_ties[kSelThreads / 32], warp_gt[kSelThreads / 32];
   __shared__ unsigned int s_prefix;
-  __shared__ int s_left;
-  const int row = blockIdx.x, b = row / a.Hw, hw = row % a.Hw, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  __shared__ int s_left, cta_ties, cta_gt;
+  cg::cluster_group cl = cg::this_cluster();
+  const int rank = kCluster > 1 ? (int)cl.block_rank() : 0;
+  auto all_ctas = [&] {
+    if constexpr (kCluster > 1)
+      cl.sync();
+    else
+      __syncthreads();
+  };
+  const int row = blockIdx.x / kCluster, b = row / a.Hw, hw = row % a.Hw;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int len = evict_len(a, b);
   const float* w = a.w + b * a.wb + hw * a.wh;
   int32_t* kept = a.kept + (long long)row * a.budget;
   float* wout = a.wout ? a.wout + (long long)row * a.budget : nullptr;
   const int new_len = min(len, a.budget);
-  if (hw == 0 && t == 0) a.lens_out[b] = new_len;
-  for (int j = new_len + t; j < a.budget; j += kSelThreads) {
+  if (hw == 0 && t == 0 && rank == 0) a.lens_out[b] = new_len;
+  for (int j = new_len + rank * kSelThreads + t; j < a.budget; j += kCluster * kSelThreads) {
     kept[j] = -1;
     if (wout) wout[j] = 0.f;
   }
-  if (len <= a.budget) {
-    for (int j = t; j < len; j += kSelThreads) {
+  if (len <= a.budget) {  // the same for every CTA of the cluster
+    for (int j = rank * kSelThreads + t; j < len; j += kCluster * kSelThreads) {
       kept[j] = j;
       if (wout) wout[j] = w[j];
     }
@@ -84,29 +98,31 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a, 
   }
   const int lo = a.n_sinks, hi = len - a.recency;  // the candidates; budget >= n_sinks + recency, so lo <= hi
   const int take = a.budget - a.n_sinks - a.recency;
-  const bool cached = len <= smem_keys;
+  // this CTA's tokens [r_lo, r_hi), and the candidates among them
+  const int cta_run = (len + kCluster * kSelThreads - 1) / (kCluster * kSelThreads) * kSelThreads;
+  const int r_lo = min(len, rank * cta_run), r_hi = min(len, r_lo + cta_run);
+  const int d_lo = max(lo, r_lo), d_hi = min(hi, r_hi);
+  const bool cached = cta_run <= smem_keys;
   if (cached) {
-#pragma unroll 8
-    for (int c = t; c < len; c += kSelThreads) keys_s[c] = weight_key(w[c]);
+#pragma unroll 4
+    for (int c = r_lo + t; c < r_hi; c += kSelThreads) keys_s[c - r_lo] = weight_key(w[c]);
   }
-  auto key_at = [&](int c) { return cached ? keys_s[c] : weight_key(w[c]); };
+  auto key_at = [&](int c) { return cached ? keys_s[c - r_lo] : weight_key(w[c]); };
   // 1. threshold key of the `take` highest candidates, and how many of its
   //    ties are taken (from the lowest index)
-  if (t == 0) {
-    s_prefix = 0;
-    s_left = take;
-  }
+  uint32_t pre = 0;
+  int left = take;
   if (take > 0) {
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
       for (int i = t; i < 2048; i += kSelThreads) hist[i] = 0;
       __syncthreads();
-      const uint32_t pre = s_prefix, high = pass == 0 ? 0u : ~0u << (shift + bits), mask = (1u << bits) - 1u;
+      const uint32_t high = pass == 0 ? 0u : ~0u << (shift + bits), mask = (1u << bits) - 1u;
 #pragma unroll 4
-      for (int c0 = lo + warp * 32; c0 < hi; c0 += kSelThreads) {
+      for (int c0 = d_lo + warp * 32; c0 < d_hi; c0 += kSelThreads) {
         const int c = c0 + lane;
-        const uint32_t key = c < hi ? key_at(c) : 0u;
-        const bool in = c < hi && ((key ^ pre) & high) == 0;
+        const uint32_t key = c < d_hi ? key_at(c) : 0u;
+        const bool in = c < d_hi && ((key ^ pre) & high) == 0;
         const unsigned act = __ballot_sync(0xffffffffu, in);
         if (act == 0) continue;
         const uint32_t bin = (key >> shift) & mask;
@@ -116,46 +132,75 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a, 
         if (lane == first) atomicAdd(&hist[bin0], (unsigned)__popc(same));
         if (in && bin != bin0) atomicAdd(&hist[bin], 1u);
       }
-      __syncthreads();
-      // thread t owns bins 2047 - 2t and 2046 - 2t, counted from the top (1024 threads, 2048 bins)
-      const int left = s_left;
-      const int h0 = (int)hist[2047 - 2 * t], h1 = (int)hist[2046 - 2 * t];
-      int all;
-      const int above = block_exclusive_scan<int, kSelThreads>(h0 + h1, scan_buf, &all);
-      if (above < left && above + h0 + h1 >= left) {
-        const bool second = above + h0 < left;
-        s_left = left - above - (second ? h0 : 0);
-        s_prefix = pre | ((uint32_t)(second ? 2046 - 2 * t : 2047 - 2 * t) << shift);
+      all_ctas();
+      if constexpr (kCluster > 1) {
+        if (rank != 0) {
+          unsigned int* root = cl.map_shared_rank(hist, 0);
+          for (int i = t; i < 2048; i += kSelThreads)
+            if (hist[i] != 0) atomicAdd(&root[i], hist[i]);
+        }
+        all_ctas();
       }
-      __syncthreads();
+      if (rank == 0) {
+        // thread t owns bins 2047 - 2t and 2046 - 2t, counted from the top (1024 threads, 2048 bins)
+        const int h0 = (int)hist[2047 - 2 * t], h1 = (int)hist[2046 - 2 * t];
+        int all;
+        const int above = block_exclusive_scan<int, kSelThreads>(h0 + h1, scan_buf, &all);
+        if (above < left && above + h0 + h1 >= left) {
+          const bool second = above + h0 < left;
+          s_left = left - above - (second ? h0 : 0);
+          s_prefix = pre | ((uint32_t)(second ? 2046 - 2 * t : 2047 - 2 * t) << shift);
+        }
+      }
+      all_ctas();
+      if constexpr (kCluster > 1) {
+        pre = *cl.map_shared_rank(&s_prefix, 0);
+        left = *cl.map_shared_rank(&s_left, 0);
+      } else {
+        pre = s_prefix;
+        left = s_left;
+      }
     }
   } else {
     __syncthreads();
   }
-  const uint32_t thr = s_prefix;
-  const int ties = s_left;
-  // 2. slots in index order: warp i walks tokens [i * run, (i + 1) * run)
-  const int run = ((len + kSelThreads - 1) / kSelThreads) * 32;
-  const int c_lo = warp * run, c_hi = min(len, c_lo + run);
+  const uint32_t thr = pre;
+  const int ties = left;
+  // 2. slots in index order: warp i walks its CTA's tokens [i * run, (i + 1) * run)
+  const int run = cta_run / (kSelThreads / 32);
+  const int c_lo = min(r_hi, r_lo + warp * run), c_hi = min(r_hi, c_lo + run);
   int ngt = 0, ntie = 0;
 #pragma unroll 4
   for (int c0 = c_lo; c0 < c_hi; c0 += 32) {
     const int c = c0 + lane;
-    const bool cand = c >= lo && c < hi && take > 0;
-    const uint32_t key = cand && c < c_hi ? key_at(c) : 0u;
+    const bool cand = c >= lo && c < hi && take > 0 && c < c_hi;
+    const uint32_t key = cand ? key_at(c) : 0u;
     ngt += __popc(__ballot_sync(0xffffffffu, c < c_hi && (c < lo || c >= hi || (cand && key > thr))));
-    ntie += __popc(__ballot_sync(0xffffffffu, cand && c < c_hi && key == thr));
+    ntie += __popc(__ballot_sync(0xffffffffu, cand && key == thr));
   }
   if (lane == 0) {
     warp_ties[warp] = ntie;
     warp_gt[warp] = ngt;
   }
   __syncthreads();
-  int seen = 0, out = 0;
+  int seen = 0, gt = 0;  // ties and others before this warp
   for (int i = 0; i < warp; ++i) {
-    out += warp_gt[i] + max(0, min(warp_ties[i], ties - seen));
+    gt += warp_gt[i];
     seen += warp_ties[i];
   }
+  if constexpr (kCluster > 1) {
+    if (t == kSelThreads - 1) {
+      cta_ties = seen + ntie;
+      cta_gt = gt + ngt;
+    }
+    all_ctas();
+    for (int i = 0; i < rank; ++i) {
+      gt += *cl.map_shared_rank(&cta_gt, i);
+      seen += *cl.map_shared_rank(&cta_ties, i);
+    }
+    all_ctas();  // no CTA leaves while another reads its counts
+  }
+  int out = gt + min(seen, ties);
 #pragma unroll 2
   for (int c0 = c_lo; c0 < c_hi; c0 += 32) {
     const int c = c0 + lane;
@@ -224,6 +269,27 @@ __global__ void __launch_bounds__(kGatherThreads) evict_gather_kernel(EvictArgs 
 }
 
 int esize(int dtype) { return dtype == KVBM_F64 ? 8 : dtype == KVBM_F32 ? 4 : 2; }
+
+template <int kCluster>
+int launch_select(const EvictArgs& a, cudaStream_t s) {
+  auto kern = evict_select_kernel<kCluster>;
+  const long long per = ((long long)a.Lmax + kCluster * kSelThreads - 1) / (kCluster * kSelThreads) * kSelThreads;
+  const int keys = (int)(per < kSmemKeys ? per : kSmemKeys);
+  if (allow_smem(kern, kSmemKeys * sizeof(uint32_t)) != KVBM_OK) return KVBM_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.B * a.Hw * kCluster));
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = keys * sizeof(uint32_t);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kCluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = kCluster > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, a, keys) == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
+}
 
 template <typename V>
 int launch_gather(EvictArgs a, int es, cudaStream_t s) {
@@ -317,10 +383,15 @@ extern "C" int kvbm_evict_cache(const kvbm_evict_args* e, void* stream) {
   a.wout = e->weights_out;
   a.page_error = attention_page_error_word();
   if (a.page_error == nullptr) return KVBM_ERR_CUDA;
-  const int smem_keys = a.Lmax < kSmemKeys ? a.Lmax : kSmemKeys;
-  if (allow_smem(evict_select_kernel, kSmemKeys * sizeof(uint32_t)) != KVBM_OK) return KVBM_ERR_CUDA;
-  evict_select_kernel<<<(unsigned)(a.B * a.Hw), kSelThreads, smem_keys * sizeof(uint32_t), s>>>(a, smem_keys);
-  if (cudaGetLastError() != cudaSuccess) return KVBM_ERR_CUDA;
+  // CTAs per row: as many as fill the SMs, while each has a few thousand keys
+  const int rows = a.B * a.Hw, sms = attention_device_sms(dev);
+  int cluster = 1;
+  while (cluster < 8 && rows * cluster * 2 <= sms && a.Lmax >= cluster * 4096) cluster *= 2;
+  const int st2 = cluster == 1   ? launch_select<1>(a, s)
+                  : cluster == 2 ? launch_select<2>(a, s)
+                  : cluster == 4 ? launch_select<4>(a, s)
+                                 : launch_select<8>(a, s);
+  if (st2 != KVBM_OK) return st2;
   const int es = esize(e->dtype);
   if ((a.D * es) % 16 == 0 && vec16(e->k_cache, e->k_stride, es) && vec16(e->v_cache, e->v_stride, es) &&
       vec16(e->k_out, e->k_out_stride, es) && vec16(e->v_out, e->v_out_stride, es))
