@@ -667,16 +667,18 @@ int kvbm_copy_2d_async(void* dst, int64_t dst_pitch, const void* src, int64_t sr
 }
 
 int kvbm_check_device_errors(void* stream) {
-  int err = 0, aerr = 0, perr = 0, aperr = 0;
+  int err = 0, aerr = 0, cerr = 0, perr = 0, aperr = 0;
   int st = read_and_clear_device_error(static_cast<cudaStream_t>(stream), &err);
   if (st != KVBM_OK) return st;
   st = read_and_clear_attention_error(static_cast<cudaStream_t>(stream), &aerr);
+  if (st != KVBM_OK) return st;
+  st = read_and_clear_cached_error(static_cast<cudaStream_t>(stream), &cerr);
   if (st != KVBM_OK) return st;
   st = read_and_clear_page_error(static_cast<cudaStream_t>(stream), &perr);
   if (st != KVBM_OK) return st;
   st = read_and_clear_attention_page_error(static_cast<cudaStream_t>(stream), &aperr);
   if (st != KVBM_OK) return st;
-  return err || aerr ? KVBM_ERR_TIMEOUT : (perr || aperr ? KVBM_ERR_PAGE : KVBM_OK);
+  return err || aerr || cerr ? KVBM_ERR_TIMEOUT : (perr || aperr ? KVBM_ERR_PAGE : KVBM_OK);
 }
 
 }  // extern "C"

@@ -183,9 +183,11 @@ bool prompt_tc_supported(const PromptArgs& a, int dtype);
 int launch_prompt_tc(const PromptArgs& a, int dtype, cudaStream_t s);
 int launch_cached_simt(const CachedArgs& a, int dtype, cudaStream_t s);
 int launch_cached_mma(const CachedArgs& a, int dtype, cudaStream_t s);  // R <= 16 rows a tile, 16-bit types
+int launch_cached_tc(const CachedArgs& a, int dtype, cudaStream_t s);   // row tiles of 128 or 256, 16-bit types, D <= 128
 int launch_cached_merge(const CachedArgs& a, int dtype, cudaStream_t s);
 int launch_cached_weights(const CachedArgs& a, cudaStream_t s);
 int read_and_clear_attention_error(cudaStream_t s, int* err);         // waits that ran out
+int read_and_clear_cached_error(cudaStream_t s, int* err);
 int read_and_clear_attention_page_error(cudaStream_t s, int* err);    // bad table entries (attention, eviction)
 unsigned int* attention_page_error_word();                            // its device address (or null)
 

@@ -97,9 +97,12 @@ bool cached_mma_supported(const kvbm_cached_args* p) {
          rows16(p->out, p->out_stride);
 }
 
+// Rows up to which the mma.sync kernel runs.
+constexpr int kMmaRows = 32;
+
 struct CachedPlan {
   CachedArgs a;
-  bool mma = false;
+  int kernel = 0;  // 0: FFMA tiles, 1: mma.sync (16 rows a tile), 2: tcgen05 (128 or 256)
   size_t part_o = 0, part_ml = 0, stats = 0, scores = 0, total = 0;
 };
 
@@ -143,13 +146,16 @@ void plan_cached(const kvbm_cached_args* p, int sms, CachedPlan* pl) {
   a.wob = p->weights_out_bstride;
   a.woh = p->weights_out_hstride;
   a.DP = a.D <= 64 ? 64 : a.D <= 128 ? 128 : 256;
-  pl->mma = cached_mma_supported(p);
-  a.BM = a.R <= 16 || pl->mma ? 16 : 64;
-  a.KT = kCachedKeyTile;
+  // 16-bit types: up to 32 rows, mma.sync, which reads the cache once per 16
+  // rows; above, tcgen05, whose tiles of 128 rows cost a 16-row unit eight
+  // times its tensor work.
+  pl->kernel = !cached_mma_supported(p) ? 0 : (a.R > kMmaRows && a.D <= 128 && a.w == nullptr && p->scale > 0.0) ? 2 : 1;
+  a.BM = pl->kernel == 2 ? (a.R > 128 ? 256 : 128) : pl->kernel == 1 || a.R <= 16 ? 16 : 64;
+  a.KT = pl->kernel == 2 ? 128 : kCachedKeyTile;
   a.RT = (a.R + a.BM - 1) / a.BM;
   // no more CTAs than key tiles of full-length sequences
   const long long tiles = (long long)a.B * a.Hkv * a.RT * ((a.Lmax + a.KT - 1) / a.KT);
-  a.C = (int)std::min<long long>(tiles, (long long)sms * 2);
+  a.C = (int)std::min<long long>(tiles, (long long)sms * (pl->kernel == 2 ? 1 : 2));
   size_t o = 0;
   auto take = [&](size_t bytes) {
     const size_t at = o;
@@ -251,7 +257,9 @@ extern "C" int kvbm_cached_attention(const kvbm_cached_args* p, void* workspace,
   a.page_error = attention_page_error_word();
   if (a.page_error == nullptr) return KVBM_ERR_CUDA;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  st = pl.mma ? launch_cached_mma(a, p->dtype, s) : launch_cached_simt(a, p->dtype, s);
+  st = pl.kernel == 2   ? launch_cached_tc(a, p->dtype, s)
+       : pl.kernel == 1 ? launch_cached_mma(a, p->dtype, s)
+                        : launch_cached_simt(a, p->dtype, s);
   if (st != KVBM_OK) return st;
   st = launch_cached_merge(a, p->dtype, s);
   if (st != KVBM_OK) return st;

@@ -34,7 +34,7 @@
 #include <algorithm>
 
 #include "kvbm_attention.cuh"
-#include "kvbm_sm100.cuh"
+#include "kvbm_attention_tile.cuh"
 
 namespace kvbm {
 
@@ -49,12 +49,6 @@ constexpr int kThreads = 384;
 constexpr int kMmaWarp = 8, kTmaWarp = 9;
 constexpr int kScrubThreads = 64;
 constexpr int kStages = 2;  // K ring, V ring
-constexpr float kGrow = 8.f;  // base-2 growth of a row's maximum that makes it the new reference
-// Of 8 groups of four columns, kEmu take their exp2 from the FMA pipe.
-#ifndef KVBM_ATT_EMU
-#define KVBM_ATT_EMU 2
-#endif
-constexpr int kEmu = KVBM_ATT_EMU;
 // Registers a thread after the split: 2 softmax warpgroups + 1 of the rest;
 // the launch holds 384 x 168.
 constexpr int kRegsSoftmax = 208, kRegsRest = 88;
@@ -178,16 +172,6 @@ __device__ void fill_rows(const PromptArgs& a, long long who, long long of) {
   }
 }
 
-__device__ __forceinline__ bool exp_group_emulated(int g) {
-  return ((g + 1) * kEmu) / 8 != (g * kEmu) / 8;
-}
-
-template <bool kBf16>
-__device__ __forceinline__ bool finite16(uint32_t half) {
-  const uint32_t e = kBf16 ? 0x7F80u : 0x7C00u;
-  return (half & e) != e;
-}
-
 template <int DP, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -304,20 +288,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t idesc_o = idesc_mma(TILE, DP, kBf16 ? 1u : 0u) | kTransposeB;
         const uint32_t qs = smem_u32(q_tile), ks = smem_u32(k_ring), vs = smem_u32(v_ring);
         auto issue_s = [&](int t, int j) {
-          const uint32_t qa = qs + t * CF::kTileBytes, kb = ks + (j % kStages) * CF::kTileBytes;
-#pragma unroll
-          for (int i = 0; i < CF::kBlocks; ++i)
-#pragma unroll
-            for (int k4 = 0; k4 < 4; ++k4)
-              mma_f16(tmem + t * TILE, sw128_desc(qa + i * CF::kBlockBytes + k4 * 32),
-                      sw128_desc(kb + i * CF::kBlockBytes + k4 * 32), idesc_s, (i | k4) != 0);
+          issue_scores<DP>(tmem + t * TILE, qs + t * CF::kTileBytes, ks + (j % kStages) * CF::kTileBytes, idesc_s);
         };
         auto issue_o = [&](int t, int j) {
-          const uint32_t vb = vs + (j % kStages) * CF::kTileBytes;
-#pragma unroll
-          for (int k = 0; k < 8; ++k)  // 16 keys a step
-            mma_f16_ts(tmem + 256 + t * TILE, tmem + t * TILE + k * 8, sw128_mn_desc(vb + k * 2048, CF::kBlockBytes),
-                       idesc_o, (j | k) != 0);
+          issue_output<DP>(tmem + 256 + t * TILE, tmem + t * TILE, vs + (j % kStages) * CF::kTileBytes, idesc_o, j > 0);
         };
         const int cnt[2] = {nA, nB};
         bool ok = mbar_wait(&k_full[0], 0, abort_flag);
@@ -373,25 +347,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         // diagonal tiles: rows keep different keys
         if (a.causal && j >= 2 * qt) {
           for (int i = st; i < CF::kBlocks * TILE * 8; i += kScrubThreads) {
-            uint4* p = reinterpret_cast<uint4*>(tile + i * 16);
-            const uint4 w = *p;
-            uint32_t x[4] = {w.x, w.y, w.z, w.w};
-            bool bad = false;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (!finite16<kBf16>(x[e])) {
-                x[e] &= 0xFFFF0000u;
-                bad = true;
-              }
-              if (!finite16<kBf16>(x[e] >> 16)) {
-                x[e] &= 0x0000FFFFu;
-                bad = true;
-              }
-            }
-            if (bad && j * TILE + ((i >> 3) & (TILE - 1)) < n) {
-              *p = make_uint4(x[0], x[1], x[2], x[3]);
+            if (j * TILE + ((i >> 3) & (TILE - 1)) < n && drop_nonfinite<kBf16>(reinterpret_cast<uint4*>(tile + i * 16)))
               *bad_flag = 1;
-            }
           }
         }
         fence_proxy_async_smem();
@@ -439,62 +396,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < TILE; ++c) v[c] = c <= lim ? v[c] : -INFINITY;
       }
-      // a NaN among the kept scores makes the maximum, and with it the row, NaN
-      float mx[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mx[e] = fmax_nan(v[e], v[e + 4]);
-#pragma unroll
-      for (int c = 8; c < TILE; c += 8)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx[e] = fmax3_nan(mx[e], v[c + e], v[c + e + 4]);
-      const float mt = fmax3_nan(fmax_nan(mx[0], mx[1]), mx[2], mx[3]) * C;
-      const bool grow = !(mt <= m + kGrow);  // (true from -inf to anything finite, and for NaN)
+      const float mt = row_max_nan(v) * C;
+      const bool grow = !(mt <= m + kAttGrow);  // (true from -inf to anything finite, and for NaN)
       if (__any_sync(0xffffffffu, grow)) {
         const float mn = grow ? mt : m;
         const float f = m == mn ? 1.f : ex2(m - mn);
         l *= f;
         m = mn;
-        if (j > 0) {
-#pragma unroll
-          for (int w = 0; w < DP / 32; ++w) {
-            float o[32];
-            tmem_ld32(to + 32 * w, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] *= f;
-            tmem_st32(to + 32 * w, o);
-          }
-        }
+        if (j > 0) scale_output<DP>(to, f);
       }
-      const float nm = m == -INFINITY ? 0.f : -m;
-      const float2 C2 = make_float2(C, C), N2 = make_float2(nm, nm);
-      float2 s0 = make_float2(0.f, 0.f), s1 = s0;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t pk16[16];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int c = 32 * w + 4 * e;
-          const float2 x0 = ffma2(make_float2(v[c], v[c + 1]), C2, N2);
-          const float2 x1 = ffma2(make_float2(v[c + 2], v[c + 3]), C2, N2);
-          float2 p0, p1;
-          if (exp_group_emulated(e)) {
-            p0 = exp2_fma2<4>(x0);
-            p1 = exp2_fma2<4>(x1);
-          } else {
-            p0 = make_float2(ex2(x0.x), ex2(x0.y));
-            p1 = make_float2(ex2(x1.x), ex2(x1.y));
-          }
-          s0 = fadd2_ftz(s0, p0);
-          s1 = fadd2_ftz(s1, p1);
-          // the weights are rounded to the inputs' type for the product with v; the row sum keeps all of them
-          pk16[2 * e] = pack16<kBf16>(p0.x, p0.y);
-          pk16[2 * e + 1] = pack16<kBf16>(p1.x, p1.y);
-        }
-        tmem_st16(ts + 16 * w, pk16);
-      }
-      s0 = fadd2(s0, s1);
-      l += s0.x + s0.y;
+      l += put_weights<kBf16, false>(v, C, m == -INFINITY ? 0.f : -m, ts);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&p_ready[t]);

@@ -1,0 +1,140 @@
+// The softmax of one row of a 128-key tile, shared by the tcgen05 attention
+// kernels: the row's 128 scores are in registers, its weights go to TMEM as
+// the A operand of P V, its output accumulator is in TMEM.
+#pragma once
+
+#include "kvbm_sm100.cuh"
+
+namespace kvbm {
+namespace sm100 {
+
+constexpr int kAttTile = 128;
+// Growth of a row's maximum (base 2) that makes it the new reference: weights
+// stay below 2^8, which both 16-bit types hold at full precision.
+constexpr float kAttGrow = 8.f;
+// Of 8 groups of four columns, kAttEmu take their exp2 from the FMA pipe
+// (degree 4, 2.7e-6 relative: far below a 16-bit weight's step, and the row
+// sums' float32 results stay within 1e-6).
+#ifndef KVBM_ATT_EMU
+#define KVBM_ATT_EMU 2
+#endif
+constexpr int kAttEmu = KVBM_ATT_EMU;
+__host__ __device__ constexpr bool att_emulated(int g) { return ((g + 1) * kAttEmu) / 8 != (g * kAttEmu) / 8; }
+
+// A NaN among the values makes the maximum NaN (and with it the row).
+__device__ __forceinline__ float row_max_nan(const float (&v)[kAttTile]) {
+  float mx[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) mx[e] = fmax_nan(v[e], v[e + 4]);
+#pragma unroll
+  for (int c = 8; c < kAttTile; c += 8)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mx[e] = fmax3_nan(mx[e], v[c + e], v[c + e + 4]);
+  return fmax3_nan(fmax_nan(mx[0], mx[1]), mx[2], mx[3]);
+}
+
+// Multiplies the row's DP accumulator columns at `to` by f (whole warp).
+template <int DP>
+__device__ __forceinline__ void scale_output(uint32_t to, float f) {
+#pragma unroll
+  for (int w = 0; w < DP / 32; ++w) {
+    float o[32];
+    tmem_ld32(to + 32 * w, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 32; ++e) o[e] *= f;
+    tmem_st32(to + 32 * w, o);
+  }
+}
+
+// Weights of the row, rounded to 16 bits, to the 64 columns at `ts`; returns
+// their float32 sum (of the unrounded values).
+//   kShift false: 2^(v C + shift), shift = -(reference in base 2)
+//   kShift true:  2^((v + shift) C), shift = -(reference), so that a score of
+//                 float32's lowest value less itself is 0
+template <bool kBf16, bool kShift>
+__device__ __forceinline__ float put_weights(const float (&v)[kAttTile], float C, float shift, uint32_t ts) {
+  const float2 C2 = make_float2(C, C), N2 = make_float2(shift, shift);
+  float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+  auto arg = [&](float a, float b) {
+    if constexpr (kShift) {
+      const float2 d = fadd2(make_float2(a, b), N2);
+      return ffma2(d, C2, make_float2(0.f, 0.f));
+    } else {
+      return ffma2(make_float2(a, b), C2, N2);
+    }
+  };
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint32_t p16[16];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = 32 * w + 4 * e;
+      const float2 x0 = arg(v[c], v[c + 1]), x1 = arg(v[c + 2], v[c + 3]);
+      float2 p0, p1;
+      if (att_emulated(e)) {
+        p0 = exp2_fma2<4>(x0);
+        p1 = exp2_fma2<4>(x1);
+      } else {
+        p0 = make_float2(ex2(x0.x), ex2(x0.y));
+        p1 = make_float2(ex2(x1.x), ex2(x1.y));
+      }
+      s0 = fadd2_ftz(s0, p0);
+      s1 = fadd2_ftz(s1, p1);
+      p16[2 * e] = pack16<kBf16>(p0.x, p0.y);
+      p16[2 * e + 1] = pack16<kBf16>(p1.x, p1.y);
+    }
+    tmem_st16(ts + 16 * w, p16);
+  }
+  s0 = fadd2(s0, s1);
+  return s0.x + s0.y;
+}
+
+template <bool kBf16>
+__device__ __forceinline__ bool finite16(uint32_t half) {
+  const uint32_t e = kBf16 ? 0x7F80u : 0x7C00u;
+  return (half & e) != e;
+}
+
+// Zeroes the non-finite 16-bit elements of a 16-byte piece; true if any was.
+template <bool kBf16>
+__device__ __forceinline__ bool drop_nonfinite(uint4* p) {
+  const uint4 w = *p;
+  uint32_t x[4] = {w.x, w.y, w.z, w.w};
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (!finite16<kBf16>(x[e])) {
+      x[e] &= 0xFFFF0000u;
+      bad = true;
+    }
+    if (!finite16<kBf16>(x[e] >> 16)) {
+      x[e] &= 0x0000FFFFu;
+      bad = true;
+    }
+  }
+  if (bad) *p = make_uint4(x[0], x[1], x[2], x[3]);
+  return bad;
+}
+
+// S (+)= Q K^T of a 128 x 128 tile, both K-major with 128-byte swizzle.
+template <int DP>
+__device__ __forceinline__ void issue_scores(uint32_t d_tmem, uint32_t q, uint32_t k, uint32_t idesc) {
+#pragma unroll
+  for (int i = 0; i < DP / 64; ++i)
+#pragma unroll
+    for (int k4 = 0; k4 < 4; ++k4)
+      mma_f16(d_tmem, sw128_desc(q + i * kAttTile * 128 + k4 * 32), sw128_desc(k + i * kAttTile * 128 + k4 * 32),
+              idesc, (i | k4) != 0);
+}
+
+// O (+)= P V: P (128 x 128, 16 bit) in TMEM, V [128 keys][DP] MN-major.
+template <int DP>
+__device__ __forceinline__ void issue_output(uint32_t d_tmem, uint32_t p_tmem, uint32_t v, uint32_t idesc, bool add) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k)  // 16 keys a step
+    mma_f16_ts(d_tmem, p_tmem + k * 8, sw128_mn_desc(v + k * 2048, kAttTile * 128), idesc, (add || k > 0) ? 1u : 0u);
+}
+
+}  // namespace sm100
+}  // namespace kvbm

@@ -1,0 +1,604 @@
+// Attention of many rows per kv head (drafted trees: R = G * T > 32) over a
+// paged cache on the tensor cores (tcgen05), bf16 / fp16, D <= 128, split over
+// the keys (kvbm_attention.cu describes the split and the joining).
+//
+// One CTA an SM.  warps 0-3 and 4-7: softmax of two streams, as in prompt
+// attention; warp 8: MMA issuer; warps 9-11: loaders, which read the rows of a
+// key tile wherever the pages lie with 16-byte cp.async (any page size, rows
+// of 128 keys, swizzled as the MMA wants them), looking page ids up one tile
+// ahead.
+//   kPair (R > 128): the streams are two tiles of 128 rows that share every
+//                    key tile;
+//   else:            one tile of rows, the streams take the even and the odd
+//                    key tiles and are joined from TMEM at the end.
+// Either way the tensor pipe works for one stream while the other's softmax
+// runs.  With 256 rows a key tile of 64 KB takes 2048 tensor cycles, about as
+// long as its bytes take from DRAM.
+//
+// Log offsets are added in the natural-log domain, and subtracted from before
+// the conversion to base 2, so that offsets of float32's lowest value act like
+// any other.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <type_traits>
+
+#include "kvbm_attention.cuh"
+#include "kvbm_attention_tile.cuh"
+
+namespace kvbm {
+namespace {
+using namespace sm100;
+
+constexpr int TILE = kAttTile;
+constexpr int kThreads = 384;
+constexpr int kMmaWarp = 8;
+constexpr int kLoaders = 96;  // warps 9-11
+constexpr int kLoaderBarrier = 2, kSoftmaxBarrier = 3;
+// Registers a thread after the split: 2 softmax warpgroups + 1 of the rest; the launch holds 384 x 168.
+constexpr int kRegsSoftmax = 208, kRegsRest = 88;
+static_assert(2 * kRegsSoftmax + kRegsRest <= 3 * 168, "the split draws on the launch's registers");
+
+template <int DP, bool kPair>
+struct Cfg {
+  static constexpr int kChunks = DP / 8;
+  static constexpr int kTileBytes = TILE * DP * 2;
+  static constexpr int kQTiles = kPair ? 2 : 1;
+  // k and v tiles in one ring, in the order k0 v0 k1 v1 ...  Four slots are
+  // enough for the order in which the MMA warp frees them (entry i is handed
+  // over when entry i + kLag is issued, and waits for entry i + kLag - kSlots,
+  // which an MMA issued before the wait for entry i frees); more hide latency.
+  static constexpr int kSlots = DP == 128 ? (kPair ? 4 : 5) : 6;
+  static constexpr int kLag = 2;  // copies still in flight when a tile is handed over
+  static constexpr int kBars = 1 + 2 * kSlots + 4 + 1;
+  static constexpr size_t kRing = (size_t)kTileBytes * (kQTiles + kSlots);
+  static constexpr size_t kSmem = 1024 + kRing + 2 * TILE * 16 + 8 * TILE * 4 + 2 * TILE * 8 + 8 * kBars + 64;
+  static_assert(kSmem <= 227 * 1024, "one CTA's shared memory");
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
+  const int n = live ? 16 : 0;  // 0: zero-filled, nothing is read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+template <int kId, int kCount>
+__device__ __forceinline__ void bar_sync() {
+  asm volatile("bar.sync %0, %1;" ::"n"(kId), "n"(kCount) : "memory");
+}
+
+// The same barrier, with one answer for every thread: whether any came with `stop`.
+// (A role whose wait gave up leaves together: nobody stays behind at a barrier.)
+template <int kId, int kCount>
+__device__ __forceinline__ bool bar_any(bool stop) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)stop), "n"(kId), "n"(kCount)
+      : "memory");
+  return r != 0;
+}
+
+// The segments of a CTA: parts [k0, k1) of units (b, g, rt), in order.
+struct Segments {
+  long long at, begin, end, bfirst;
+  int b;
+  // the current segment
+  int len, nt, g, rt, k0, k1;
+  long long ufirst;
+  __device__ bool next(const CachedArgs& a) {
+    if (at >= end) return false;
+    len = cached_len(a, b);
+    nt = (len + TILE - 1) / TILE;
+    while (at >= bfirst + (long long)nt * a.Hkv * a.RT) {
+      bfirst += (long long)nt * a.Hkv * a.RT;
+      ++b;
+      len = cached_len(a, b);
+      nt = (len + TILE - 1) / TILE;
+    }
+    const int u = (int)((at - bfirst) / nt);
+    g = u / a.RT;
+    rt = u % a.RT;
+    ufirst = bfirst + (long long)u * nt;
+    k0 = (int)(at - ufirst);
+    k1 = (int)min((long long)nt, end - ufirst);
+    at = ufirst + k1;
+    return true;
+  }
+};
+
+template <int DP, bool kBf16, bool kPair, bool kBias>
+__global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_constant__ CachedArgs a) {
+  using CF = Cfg<DP, kPair>;
+  using T = std::conditional_t<kBf16, __nv_bfloat16, __half>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* q_tile = smem;
+  uint8_t* ring = q_tile + CF::kQTiles * CF::kTileBytes;
+  longlong2* offs = reinterpret_cast<longlong2*>(smem + CF::kRing);       // [2][TILE]
+  float* bias_s = reinterpret_cast<float*>(offs + 2 * TILE);              // [8 warps][TILE]
+  float2* ml_s = reinterpret_cast<float2*>(bias_s + 8 * TILE);            // [2][TILE]
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(ml_s + 2 * TILE);
+  uint64_t *full = q_full + 1, *empty = full + CF::kSlots, *s_full = empty + CF::kSlots, *p_ready = s_full + 2;
+  uint64_t* seg_done = p_ready + 2;
+  long long* sched = reinterpret_cast<long long*>(seg_done + 1);  // total, first
+  int* sched_b = reinterpret_cast<int*>(sched + 2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sched_b + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* bad_flag = abort_flag + 1;
+
+  cudaTriggerProgrammaticLaunchCompletion();  // the joining kernel may be set up beside this one
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0) {
+    long long pre, total, first = 0;
+    warp_tile_prefix(a, 0, &pre, &total);
+    const int b = warp_find_seq(a, split_begin(blockIdx.x, total, a.C), &first);
+    if (lane == 0) {
+      sched[0] = total;
+      sched[1] = first;
+      *sched_b = b;
+      *abort_flag = 0;
+      *bad_flag = 0;
+      mbar_init(q_full, kLoaders);
+      for (int i = 0; i < CF::kSlots; ++i) {
+        mbar_init(&full[i], kLoaders);
+        mbar_init(&empty[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&s_full[i], 1);
+        mbar_init(&p_ready[i], TILE);
+      }
+      mbar_init(seg_done, 2 * TILE);
+      fence_mbar_init();
+    }
+  } else if (warp == kMmaWarp) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // columns: S/P of stream t at t * 128, O of stream t at 256 + t * 128
+  Segments sg;
+  sg.begin = split_begin(blockIdx.x, sched[0], a.C);
+  sg.end = split_begin(blockIdx.x + 1, sched[0], a.C);
+  sg.at = sg.begin;
+  sg.bfirst = sched[1];
+  sg.b = *sched_b;
+
+  if (warp >= kMmaWarp) {
+    reg_dec<kRegsRest>();
+    if (warp == kMmaWarp) {
+      if (lane == 0) {
+        const uint32_t idesc_s = idesc_mma(TILE, TILE, kBf16 ? 1u : 0u);
+        const uint32_t idesc_o = idesc_mma(TILE, DP, kBf16 ? 1u : 0u) | kTransposeB;
+        const uint32_t qa = smem_u32(q_tile), ra = smem_u32(ring);
+        long long idx = 0;             // ring index of this segment's k0
+        uint32_t pn[2] = {0, 0};       // p_ready phases used
+        uint32_t sn[2] = {0, 0};       // s_full commits made
+        bool ok = true;
+        for (uint32_t seg = 0; ok && sg.next(a); ++seg) {
+          const int nk = sg.k1 - sg.k0;
+          auto slot_of = [&](long long i) { return (int)(i % CF::kSlots); };
+          auto wait_full = [&](long long i) {
+            return mbar_wait(&full[slot_of(i)], (uint32_t)(i / CF::kSlots) & 1u, abort_flag);
+          };
+          auto issue_s = [&](int t, int j) {
+            issue_scores<DP>(tmem + t * TILE, qa + (kPair ? t : 0) * CF::kTileBytes,
+                             ra + slot_of(idx + 2 * j) * CF::kTileBytes, idesc_s);
+          };
+          auto commit_s = [&](int t) {
+            mma_commit(&s_full[t]);
+            ++sn[t];
+          };
+          ok = mbar_wait(q_full, seg & 1u, abort_flag);
+          if constexpr (kPair) {
+            ok = ok && wait_full(idx);
+            if (ok) {
+              tc_fence_after();
+              fence_proxy_async_smem();
+              for (int t = 0; t < 2; ++t) {
+                issue_s(t, 0);
+                commit_s(t);
+              }
+              mma_commit(&empty[slot_of(idx)]);
+            }
+            for (int j = 0; ok && j < nk; ++j) {
+              ok = wait_full(idx + 2 * j + 1);
+              if (ok && j + 1 < nk) ok = wait_full(idx + 2 * j + 2);
+              for (int t = 0; ok && t < 2; ++t) {
+                ok = mbar_wait(&p_ready[t], pn[t]++ & 1u, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                issue_output<DP>(tmem + 256 + t * TILE, tmem + t * TILE,
+                                 ra + slot_of(idx + 2 * j + 1) * CF::kTileBytes, idesc_o, j > 0);
+                if (j + 1 < nk) issue_s(t, j + 1);
+                commit_s(t);  // the next S, or the finished O
+              }
+              if (!ok) break;
+              mma_commit(&empty[slot_of(idx + 2 * j + 1)]);
+              if (j + 1 < nk) mma_commit(&empty[slot_of(idx + 2 * j + 2)]);
+            }
+          } else {
+            for (int t = 0; ok && t < 2 && t < nk; ++t) {
+              ok = wait_full(idx + 2 * t);
+              if (!ok) break;
+              tc_fence_after();
+              issue_s(t, t);
+              commit_s(t);
+              mma_commit(&empty[slot_of(idx + 2 * t)]);
+            }
+            for (int j = 0; ok && j < nk; ++j) {
+              const int t = j & 1;
+              ok = wait_full(idx + 2 * j + 1) && mbar_wait(&p_ready[t], pn[t]++ & 1u, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+              issue_output<DP>(tmem + 256 + t * TILE, tmem + t * TILE,
+                               ra + slot_of(idx + 2 * j + 1) * CF::kTileBytes, idesc_o, j > 1);
+              mma_commit(&empty[slot_of(idx + 2 * j + 1)]);
+              if (j + 2 < nk) {
+                ok = wait_full(idx + 2 * j + 4);
+                if (!ok) break;
+                tc_fence_after();
+                issue_s(t, j + 2);
+                commit_s(t);
+                mma_commit(&empty[slot_of(idx + 2 * j + 4)]);
+              } else {
+                commit_s(t);  // the finished O
+              }
+            }
+          }
+          idx += 2 * (long long)nk;
+        }
+        // TMEM and shared memory stay until every MMA has finished
+        for (int t = 0; t < 2; ++t)
+          if (sn[t] > 0) mbar_wait(&s_full[t], (sn[t] - 1) & 1u, abort_flag);
+      }
+    } else {
+      // ---- loaders
+      const int lt = threadIdx.x - (kMmaWarp + 1) * 32;
+      const uint32_t ra = smem_u32(ring);
+      const T *kbase = static_cast<const T*>(a.k), *vbase = static_cast<const T*>(a.v);
+      const int ch = lt % CF::kChunks;
+      const bool in = ch * 8 < a.D;
+      long long idx = 0;
+      bool ok = true;
+      for (uint32_t seg = 0; ok && sg.next(a); ++seg) {
+        const int b = sg.b, g = sg.g, len = sg.len, pre = len - a.T;
+        const float* off = kBias ? a.off + b * a.ob + g * a.oh : nullptr;
+        if (seg > 0) ok = mbar_wait(seg_done, (seg - 1) & 1u, abort_flag);  // the queries' tile and O are free
+        ok = !bar_any<kLoaderBarrier, kLoaders>(!ok);
+        if (!ok) break;
+        for (int i = lt; i < CF::kQTiles * TILE * CF::kChunks; i += kLoaders) {
+          const int row = i / CF::kChunks, c = i % CF::kChunks, r = sg.rt * CF::kQTiles * TILE + row;
+          uint4 w = make_uint4(0u, 0u, 0u, 0u);
+          if (r < a.R && c * 8 < a.D)
+            w = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.qs[0] +
+                                                (long long)(g * a.G + r / a.T) * a.qs[1] +
+                                                (long long)(r % a.T) * a.qs[2] + c * 8);
+          const int rl = row % TILE;
+          *reinterpret_cast<uint4*>(q_tile + (row / TILE) * CF::kTileBytes + (c >> 3) * (TILE * 128) + rl * 128 +
+                                    (((c & 7) ^ (rl & 7)) << 4)) = w;
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(q_full);
+
+        auto page_of = [&](int c) -> int {
+          if (c >= len) return -1;
+          const int pi = c / a.pg.page_size;
+          return a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
+        };
+        auto offset_of = [&](int c, int page) {
+          longlong2 o = make_longlong2(-1, -1);
+          if (c >= len || (kBias && off[c] == -INFINITY)) return o;
+          if (page < 0 || page >= a.pg.num_pages) {
+            atomicOr(a.page_error, 1u);
+            return o;
+          }
+          const int at = c % a.pg.page_size;
+          o.x = (long long)page * a.ks[0] + (long long)at * a.ks[1] + g * a.ks[2];
+          o.y = (long long)page * a.vs[0] + (long long)at * a.vs[1] + g * a.vs[2];
+          return o;
+        };
+        // hand over ring entry i (its copies have landed for this thread)
+        auto hand_over = [&](long long i) {
+          const int j = sg.k0 + (int)((i - idx) >> 1);
+          if (((i - idx) & 1) && (j + 1) * TILE > pre) {
+            // v of drafted tokens: rows keep different ones; this thread's
+            // own pieces are checked, non-finite elements taken out and added
+            // to the rows that keep them at the end
+            uint8_t* tile = ring + (int)(i % CF::kSlots) * CF::kTileBytes;
+            bool bad = false;
+            for (int r = lt / CF::kChunks; r < TILE; r += kLoaders / CF::kChunks)
+              if (j * TILE + r >= pre)
+                bad |= drop_nonfinite<kBf16>(reinterpret_cast<uint4*>(tile + (ch >> 3) * (TILE * 128) + r * 128 +
+                                                                      (((ch & 7) ^ (r & 7)) << 4)));
+            if (bad) *bad_flag = 1;
+          }
+          fence_proxy_async_smem();
+          mbar_arrive(&full[i % CF::kSlots]);
+        };
+        int page0 = page_of(sg.k0 * TILE + lt), page1 = lt < TILE - kLoaders ? page_of(sg.k0 * TILE + kLoaders + lt) : -1;
+        const int nk = sg.k1 - sg.k0;
+        for (int j = 0; j < nk; ++j) {
+          const int c0 = (sg.k0 + j) * TILE;
+          longlong2* of = offs + (j & 1) * TILE;
+          of[lt] = offset_of(c0 + lt, page0);
+          if (lt < TILE - kLoaders) of[kLoaders + lt] = offset_of(c0 + kLoaders + lt, page1);
+          if (j + 1 < nk) {
+            page0 = page_of(c0 + TILE + lt);
+            if (lt < TILE - kLoaders) page1 = page_of(c0 + TILE + kLoaders + lt);
+          }
+          ok = !bar_any<kLoaderBarrier, kLoaders>(!ok);
+          if (!ok) break;
+#pragma unroll 1
+          for (int kv = 0; kv < 2; ++kv) {
+            const long long i = idx + 2 * j + kv;
+            const int slot = (int)(i % CF::kSlots);
+            if (i >= CF::kSlots)
+              ok = mbar_wait(&empty[slot], (uint32_t)(i / CF::kSlots - 1) & 1u, abort_flag) && ok;
+            if (ok) {
+              const uint32_t dst = ra + slot * CF::kTileBytes + (ch >> 3) * (TILE * 128);
+              const T* base = kv ? vbase : kbase;
+#pragma unroll 4
+              for (int r = lt / CF::kChunks; r < TILE; r += kLoaders / CF::kChunks) {
+                const long long o = kv ? of[r].y : of[r].x;
+                const bool live = in && o >= 0;
+                cp16(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4), live ? base + o + ch * 8 : base, live);
+              }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (2 * j + kv >= CF::kLag) {
+              cp_wait<CF::kLag>();
+              hand_over(i - CF::kLag);
+            }
+          }
+        }
+        ok = !bar_any<kLoaderBarrier, kLoaders>(!ok);
+        if (!ok) break;
+        static_assert(CF::kLag == 2, "the tail below hands over two entries");
+        cp_wait<1>();
+        hand_over(idx + 2 * nk - 2);
+        cp_wait<0>();
+        hand_over(idx + 2 * nk - 1);
+        idx += 2 * (long long)nk;
+      }
+      cp_wait<0>();
+    }
+  } else {
+    // ---- softmax
+    reg_inc<kRegsSoftmax>();
+    const int t = warp >> 2, sub = warp & 3;
+    const int rl = sub * 32 + lane;
+    const uint32_t ts = tmem + ((uint32_t)(sub * 32) << 16) + t * TILE, to = ts + 256;
+    float* wbias = bias_s + warp * TILE;
+    const float C = kBias ? kLog2eF : a.scale * kLog2eF;
+    uint32_t sn = 0;  // s_full phases used
+    bool ok = true;
+    while (ok && sg.next(a)) {
+      const int b = sg.b, g = sg.g, len = sg.len, pre = len - a.T, nk = sg.k1 - sg.k0;
+      const int r = (sg.rt * CF::kQTiles + (kPair ? t : 0)) * TILE + rl;  // row of the unit
+      const int tok = r % a.T, h = g * a.G + r / a.T;
+      const float* off = kBias ? a.off + b * a.ob + g * a.oh : nullptr;
+      // drafted tokens this row keeps
+      unsigned long long tree = 0;
+      if (sg.k1 * TILE > pre && r < a.R) {
+        if (a.tree != nullptr) {
+          const uint8_t* tm = a.tree + b * a.tb + tok * a.tr;
+          for (int u = 0; u < a.T; ++u) tree |= (unsigned long long)(tm[u] != 0) << u;
+        } else {
+          tree = ~0ull >> (63 - tok);
+        }
+      }
+      float m = -INFINITY, l = 0.f;
+      int done = 0;  // tiles of this stream
+      for (int j = kPair ? 0 : t; ok && j < nk; j += kPair ? 1 : 2, ++done) {
+        const int c0 = (sg.k0 + j) * TILE;
+        if constexpr (kBias) {
+          __syncwarp();
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int c = c0 + 32 * w + lane;
+            wbias[32 * w + lane] = c < len ? off[c] : -INFINITY;
+          }
+          __syncwarp();
+        }
+        ok = mbar_wait(&s_full[t], sn++ & 1u, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        float v[TILE];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) tmem_ld32(ts + 32 * w, *reinterpret_cast<float(*)[32]>(&v[32 * w]));
+        tmem_ld_wait();
+        if constexpr (kBias) {
+#pragma unroll
+          for (int c = 0; c < TILE; c += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(wbias + c);
+            // (a key of offset -inf is a zero row: its score is finite, and drops out here)
+            v[c] = fmaf(v[c], a.scale, x.x);
+            v[c + 1] = fmaf(v[c + 1], a.scale, x.y);
+            v[c + 2] = fmaf(v[c + 2], a.scale, x.z);
+            v[c + 3] = fmaf(v[c + 3], a.scale, x.w);
+          }
+        }
+        if (c0 + TILE > pre) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int sh = c0 + 32 * w - pre;  // drafted token of the word's first key
+            uint32_t bits;
+            if (sh <= -32)
+              bits = 0xffffffffu;
+            else if (sh < 0)
+              bits = ((uint32_t)tree << -sh) | ((1u << -sh) - 1u);
+            else
+              bits = sh < 64 ? (uint32_t)(tree >> sh) : 0u;
+#pragma unroll
+            for (int c = 0; c < 32; ++c) v[32 * w + c] = ((bits >> c) & 1u) ? v[32 * w + c] : -INFINITY;
+          }
+        }
+        const float mt = kBias ? row_max_nan(v) : row_max_nan(v) * C;
+        const bool grow = !(mt <= m + (kBias ? kAttGrow * kLn2F : kAttGrow));
+        if (__any_sync(0xffffffffu, grow)) {
+          const float mn = grow ? mt : m;
+          const float f = m == mn ? 1.f : ex2(kBias ? (m - mn) * kLog2eF : m - mn);
+          l *= f;
+          m = mn;
+          if (done > 0) scale_output<DP>(to, f);
+        }
+        l += put_weights<kBf16, kBias>(v, C, m == -INFINITY ? 0.f : -m, ts);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_ready[t]);
+      }
+      if (ok && done > 0) {
+        ok = mbar_wait(&s_full[t], sn++ & 1u, abort_flag);  // O is complete
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+      }
+      if (bar_any<kSoftmaxBarrier, 2 * TILE>(!ok)) break;
+      // ---- the segment's result
+      const bool whole = sg.k0 == 0 && sg.k1 == sg.nt;
+      const long long pr = ((long long)blockIdx.x * 2 + (sg.begin >= sg.ufirst ? 0 : 1)) * a.BM +
+                           (kPair ? t * TILE + rl : rl);
+      float f0 = 1.f, f1 = 0.f;
+      if constexpr (!kPair) {
+        // both streams hold the same rows: stream t joins the columns [t DP / 2, (t + 1) DP / 2)
+        ml_s[t * TILE + rl] = make_float2(m, l);
+        tc_fence_before();
+        bar_sync<kSoftmaxBarrier, 2 * TILE>();
+        tc_fence_after();
+        const float2 x0 = ml_s[rl], x1 = ml_s[TILE + rl];
+        m = fmaxf(x0.x, x1.x);
+        const float base = m == -INFINITY ? 0.f : m;
+        const float C1 = kBias ? kLog2eF : 1.f;
+        f0 = ex2((x0.x - base) * C1);
+        f1 = ex2((x1.x - base) * C1);
+        l = x0.y * f0 + x1.y * f1;
+      }
+      const bool bad = *bad_flag != 0;
+      const float m_nat = kBias ? m : m * kLn2F;
+      const bool none = l == 0.f;
+      const float inv = none ? 0.f : 1.f / l;
+      const uint32_t o_at = tmem + ((uint32_t)(sub * 32) << 16) + 256;
+      constexpr int kCols = kPair ? DP : DP / 2;
+      uint16_t* out = static_cast<uint16_t*>(a.out) + b * a.os[0] + h * a.os[1] + tok * a.os[2];
+#pragma unroll
+      for (int w = 0; w < kCols / 32; ++w) {
+        const int d0 = (kPair ? 0 : t * kCols) + 32 * w;
+        float o[32];
+        if constexpr (kPair) {
+          tmem_ld32(to + d0, o);
+          tmem_ld_wait();
+        } else {
+          float o1[32];
+          tmem_ld32(o_at + d0, o);
+          if (nk > 1) tmem_ld32(o_at + TILE + d0, o1);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = nk > 1 ? o[e] * f0 + o1[e] * f1 : o[e] * f0;
+        }
+        if (r < a.R) {
+          if (bad) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              float4 x = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+              if (d0 + e < a.D)
+                add_draft_nonfinite<T>(a, b, g, tok, max(max(pre, 0), sg.k0 * TILE), min(len, sg.k1 * TILE), pre, d0 + e,
+                                       x);
+              o[e] = x.x;
+              o[e + 1] = x.y;
+              o[e + 2] = x.z;
+              o[e + 3] = x.w;
+            }
+          }
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              if (d0 + e >= a.D) continue;  // D % 8 == 0
+              uint4 x;
+              x.x = none ? 0u : pack16<kBf16>(o[e] * inv, o[e + 1] * inv);
+              x.y = none ? 0u : pack16<kBf16>(o[e + 2] * inv, o[e + 3] * inv);
+              x.z = none ? 0u : pack16<kBf16>(o[e + 4] * inv, o[e + 5] * inv);
+              x.w = none ? 0u : pack16<kBf16>(o[e + 6] * inv, o[e + 7] * inv);
+              *reinterpret_cast<uint4*>(out + d0 + e) = x;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<float4*>(a.part_o + pr * a.DP + d0 + e) =
+                  make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+        __syncwarp();  // the next load is the whole warp's
+      }
+      if (r < a.R && (kPair || t == 0)) {
+        if (whole)
+          a.lse[b * a.ls[0] + h * a.ls[1] + tok * a.ls[2]] = none ? -INFINITY : m_nat + logf(l);
+        else
+          a.part_ml[pr] = make_float2(m_nat, l);
+      }
+      tc_fence_before();
+      bar_sync<kSoftmaxBarrier, 2 * TILE>();  // everyone has read the flag, ml_s and O
+      if (threadIdx.x == 0) *bad_flag = 0;
+      mbar_arrive(seg_done);
+    }
+    tc_fence_before();
+  }
+
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int DP, bool kBf16, bool kPair, bool kBias>
+int launch(const CachedArgs& a, cudaStream_t s) {
+  auto kern = cached_tc_kernel<DP, kBf16, kPair, kBias>;
+  constexpr size_t bytes = Cfg<DP, kPair>::kSmem;
+  if (allow_smem(kern, bytes) != KVBM_OK) return KVBM_ERR_CUDA;
+  kern<<<(unsigned)a.C, kThreads, bytes, s>>>(a);
+  return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
+}
+
+template <int DP, bool kBf16>
+int launch_d(const CachedArgs& a, cudaStream_t s) {
+  const bool bias = a.off != nullptr;
+  if (a.BM == 2 * TILE) return bias ? launch<DP, kBf16, true, true>(a, s) : launch<DP, kBf16, true, false>(a, s);
+  return bias ? launch<DP, kBf16, false, true>(a, s) : launch<DP, kBf16, false, false>(a, s);
+}
+
+}  // namespace
+
+int launch_cached_tc(const CachedArgs& a, int dtype, cudaStream_t s) {
+  const bool bf16 = dtype == KVBM_BF16;
+  if (a.DP == 64) return bf16 ? launch_d<64, true>(a, s) : launch_d<64, false>(a, s);
+  return bf16 ? launch_d<128, true>(a, s) : launch_d<128, false>(a, s);
+}
+
+int read_and_clear_cached_error(cudaStream_t s, int* err) {
+  unsigned int v = 0;
+  if (cudaMemcpyFromSymbolAsync(&v, g_kvbm_device_error, sizeof(v), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
+      cudaStreamSynchronize(s) != cudaSuccess)
+    return KVBM_ERR_CUDA;
+  *err = v != 0;
+  if (v != 0) {
+    const unsigned int zero = 0;
+    if (cudaMemcpyToSymbolAsync(g_kvbm_device_error, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s) !=
+            cudaSuccess ||
+        cudaStreamSynchronize(s) != cudaSuccess)
+      return KVBM_ERR_CUDA;
+  }
+  return KVBM_OK;
+}
+
+}  // namespace kvbm

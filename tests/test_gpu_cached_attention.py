@@ -117,12 +117,12 @@ def test_tree(cuda_device, dtype, T, Hq, Hkv, D):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_tree_rows_of_their_own(cuda_device, dtype):
+@pytest.mark.parametrize("T,Hq", [(9, 4), (20, 8), (40, 8), (30, 4)])
+def test_tree_rows_of_their_own(cuda_device, dtype, T, Hq):
     """A mask row that keeps no drafted token (and with lens = T nothing at all), a cache shorter than the tree, and
     NaN or infinities in the k and v of one branch, which reach the tokens that attend to it and no other."""
-    T = 9
-    c = Case([T, 4, 70, 131], 8, 4, 2, 64, T, dtype, cuda_device, seed=5)
-    tree = _tree(4, T, 1, cuda_device)
+    c = Case([T, T - 5, 70, 131, 300], 8, Hq, 2, 64, T, dtype, cuda_device, seed=5)
+    tree = _tree(5, T, 1, cuda_device)
     tree[:, 3] = False
     out, lse = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, tree_mask=tree)
     _check(c, out, lse, tree)
@@ -144,10 +144,10 @@ def test_tree_rows_of_their_own(cuda_device, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("T", [1, 6])
+@pytest.mark.parametrize("T", [1, 6, 16, 40])
 @pytest.mark.parametrize("heads", [1, 2])
 def test_log_offsets(cuda_device, dtype, T, heads):
-    c = Case([10, 200, 64, 131], 16, 8, 2, 64, T, dtype, cuda_device, seed=8)
+    c = Case([T + 9, 200, 64, 131], 16, 8, 2, 64, T, dtype, cuda_device, seed=8)
     g = torch.Generator().manual_seed(1)
     off = (3 * torch.rand(4, heads, c.L, generator=g)).to(cuda_device)
     off[torch.rand(off.shape, generator=g).to(cuda_device) < 0.4] = -math.inf
@@ -213,7 +213,7 @@ def test_weights(cuda_device, dtype, Hq, Hkv, D):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("T,Hq", [(1, 4), (1, 32), (16, 8)])
+@pytest.mark.parametrize("T,Hq", [(1, 4), (1, 32), (16, 8), (13, 16), (40, 16)])
 def test_many_sequences(cuda_device, dtype, T, Hq):
     """More units than CTAs, and lengths far apart: every way a unit can fall on the split."""
     g = torch.Generator().manual_seed(7)
@@ -294,11 +294,11 @@ def test_bad_pages(cuda_device, dtype):
     assert bool((e.k[0, 32:48] == 0).all()) and bool((e.k[0, :32] != 0).any())
 
 
-@pytest.mark.parametrize("T", [1, 8])
+@pytest.mark.parametrize("T", [1, 8, 20, 50])
 def test_two_calls_and_graphs(cuda_device, T):
     """Calls on two streams at once, and a captured call replayed on new lengths."""
     c = Case([900, 333, 64, 700], 16, 8, 2, 128, T, torch.bfloat16, cuda_device, seed=3)
-    d = Case([100, 950, 7 + T, 80], 16, 8, 2, 128, T, torch.bfloat16, cuda_device, seed=4)
+    d = Case([100, 950, 7 + T, 180], 16, 8, 2, 128, T, torch.bfloat16, cuda_device, seed=4)
     want = [kb.attention_cached(x.q, x.k, x.v, x.table, x.seq_lens) for x in (c, d)]
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]
     torch.cuda.synchronize()
@@ -316,7 +316,7 @@ def test_two_calls_and_graphs(cuda_device, T):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, out=out, lse_out=lse, workspace=ws)
-    for lens in ([900, 333, 64, 700], [T, 0, 301, 1], [899, 900, 900, 900]):
+    for lens in ([900, 333, 64, 700], [T, 0, 301, 64], [899, 900, 900, 900]):
         c.seq_lens.copy_(torch.tensor(lens))
         ws.fill_(0xFF)
         graph.replay()
