@@ -38,8 +38,6 @@
 
 namespace kvbm {
 
-bool make_attention_map(CUtensorMap* map, const void* base, bool bf16, int B, int H, int N, int D, const int64_t* st);
-
 namespace {
 using namespace sm100;
 
@@ -495,9 +493,9 @@ int launch(const PromptArgs& a, cudaStream_t s) {
   const int B = packed ? 1 : a.B, N = packed ? (int)a.total : a.N;
   const int64_t qs[4] = {a.qs[0], a.qs[1], a.qs[2], 1}, ks[4] = {a.ks[0], a.ks[1], a.ks[2], 1};
   const int64_t vs[4] = {a.vs[0], a.vs[1], a.vs[2], 1};
-  if (!make_attention_map(&tq, a.q, kBf16, B, a.Hq, N, a.D, qs) ||
-      !make_attention_map(&tk, a.k, kBf16, B, a.Hkv, N, a.D, ks) ||
-      !make_attention_map(&tv, a.v, kBf16, B, a.Hkv, N, a.D, vs))
+  if (!make_attention_map(&tq, a.q, kBf16, B, a.Hq, N, a.D, qs, TILE) ||
+      !make_attention_map(&tk, a.k, kBf16, B, a.Hkv, N, a.D, ks, TILE) ||
+      !make_attention_map(&tv, a.v, kBf16, B, a.Hkv, N, a.D, vs, TILE))
     return KVBM_ERR_CUDA;
   auto kern = prompt_tc_kernel<DP, kBf16>;
   constexpr size_t smem = Cfg<DP>::kSmem;

@@ -6,6 +6,12 @@
 #include "kvbm_sm100.cuh"
 
 namespace kvbm {
+
+// A 4-D map over a 16-bit [B, H, N, D] operand, boxes of 64 elements x `rows`
+// rows with 128-byte swizzle (kvbm_tc.cu).
+bool make_attention_map(CUtensorMap* map, const void* base, bool bf16, int B, int H, int N, int D, const int64_t* st,
+                        int rows);
+
 namespace sm100 {
 
 constexpr int kAttTile = 128;

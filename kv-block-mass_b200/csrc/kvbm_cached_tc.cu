@@ -3,10 +3,14 @@
 // the keys (kvbm_attention.cu describes the split and the joining).
 //
 // One CTA an SM.  warps 0-3 and 4-7: softmax of two streams, as in prompt
-// attention; warp 8: MMA issuer; warps 9-11: loaders, which read the rows of a
-// key tile wherever the pages lie with 16-byte cp.async (any page size, rows
-// of 128 keys, swizzled as the MMA wants them), looking page ids up one tile
-// ahead.
+// attention; warp 8: MMA issuer; warps 9-11: loaders, in one of two ways:
+//   kTma:  pages of a multiple of 8 slots that tile 128 keys evenly (or are a
+//          multiple of 128): warp 9 loads each page with TMA, and warps 10-11
+//          zero the v rows nobody keeps in the tiles that hold any (the last
+//          ones, and with log offsets all);
+//   else:  any page size: all three warps read the rows with 16-byte cp.async
+//          into the layout TMA would write, page ids looked up one tile ahead.
+//          (32768 keys x 4 sequences, 64 tokens: 358 us this way.)
 //   kPair (R > 128): the streams are two tiles of 128 rows that share every
 //                    key tile;
 //   else:            one tile of rows, the streams take the even and the odd
@@ -22,6 +26,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "kvbm_attention.cuh"
@@ -35,7 +40,7 @@ constexpr int TILE = kAttTile;
 constexpr int kThreads = 384;
 constexpr int kMmaWarp = 8;
 constexpr int kLoaders = 96;  // warps 9-11
-constexpr int kLoaderBarrier = 2, kSoftmaxBarrier = 3;
+constexpr int kLoaderBarrier = 2, kSoftmaxBarrier = 3, kScrubBarrier = 4;
 // Registers a thread after the split: 2 softmax warpgroups + 1 of the rest; the launch holds 384 x 168.
 constexpr int kRegsSoftmax = 208, kRegsRest = 88;
 static_assert(2 * kRegsSoftmax + kRegsRest <= 3 * 168, "the split draws on the launch's registers");
@@ -51,7 +56,7 @@ struct Cfg {
   // which an MMA issued before the wait for entry i frees); more hide latency.
   static constexpr int kSlots = DP == 128 ? (kPair ? 4 : 5) : 6;
   static constexpr int kLag = 2;  // copies still in flight when a tile is handed over
-  static constexpr int kBars = 1 + 2 * kSlots + 4 + 1;
+  static constexpr int kBars = 1 + 3 * kSlots + 4 + 1;
   static constexpr size_t kRing = (size_t)kTileBytes * (kQTiles + kSlots);
   static constexpr size_t kSmem = 1024 + kRing + 2 * TILE * 16 + 8 * TILE * 4 + 2 * TILE * 8 + 8 * kBars + 64;
   static_assert(kSmem <= 227 * 1024, "one CTA's shared memory");
@@ -114,8 +119,10 @@ struct Segments {
   }
 };
 
-template <int DP, bool kBf16, bool kPair, bool kBias>
-__global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_constant__ CachedArgs a) {
+template <int DP, bool kBf16, bool kPair, bool kBias, bool kTma>
+__global__ void __launch_bounds__(kThreads, 1)
+    cached_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                     const __grid_constant__ CachedArgs a) {
   using CF = Cfg<DP, kPair>;
   using T = std::conditional_t<kBf16, __nv_bfloat16, __half>;
   extern __shared__ uint8_t smem_raw[];
@@ -126,7 +133,8 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
   float* bias_s = reinterpret_cast<float*>(offs + 2 * TILE);              // [8 warps][TILE]
   float2* ml_s = reinterpret_cast<float2*>(bias_s + 8 * TILE);            // [2][TILE]
   uint64_t* q_full = reinterpret_cast<uint64_t*>(ml_s + 2 * TILE);
-  uint64_t *full = q_full + 1, *empty = full + CF::kSlots, *s_full = empty + CF::kSlots, *p_ready = s_full + 2;
+  uint64_t *full = q_full + 1, *empty = full + CF::kSlots, *raw = empty + CF::kSlots, *s_full = raw + CF::kSlots;
+  uint64_t* p_ready = s_full + 2;
   uint64_t* seg_done = p_ready + 2;
   long long* sched = reinterpret_cast<long long*>(seg_done + 1);  // total, first
   int* sched_b = reinterpret_cast<int*>(sched + 2);
@@ -148,8 +156,9 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
       *bad_flag = 0;
       mbar_init(q_full, kLoaders);
       for (int i = 0; i < CF::kSlots; ++i) {
-        mbar_init(&full[i], kLoaders);
+        mbar_init(&full[i], kTma ? 1 : kLoaders);
         mbar_init(&empty[i], 1);
+        mbar_init(&raw[i], 1);
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&s_full[i], 1);
@@ -270,7 +279,12 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
       const int ch = lt % CF::kChunks;
       const bool in = ch * 8 < a.D;
       long long idx = 0;
+      uint32_t raw_phase = 0;  // per slot (kTma)
       bool ok = true;
+      if (kTma && lt == 0) {
+        prefetch_tmap(&tk);
+        prefetch_tmap(&tv);
+      }
       for (uint32_t seg = 0; ok && sg.next(a); ++seg) {
         const int b = sg.b, g = sg.g, len = sg.len, pre = len - a.T;
         const float* off = kBias ? a.off + b * a.ob + g * a.oh : nullptr;
@@ -291,84 +305,173 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
         fence_proxy_async_smem();
         mbar_arrive(q_full);
 
-        auto page_of = [&](int c) -> int {
-          if (c >= len) return -1;
-          const int pi = c / a.pg.page_size;
-          return a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
-        };
-        auto offset_of = [&](int c, int page) {
-          longlong2 o = make_longlong2(-1, -1);
-          if (c >= len || (kBias && off[c] == -INFINITY)) return o;
-          if (page < 0 || page >= a.pg.num_pages) {
-            atomicOr(a.page_error, 1u);
-            return o;
-          }
-          const int at = c % a.pg.page_size;
-          o.x = (long long)page * a.ks[0] + (long long)at * a.ks[1] + g * a.ks[2];
-          o.y = (long long)page * a.vs[0] + (long long)at * a.vs[1] + g * a.vs[2];
-          return o;
-        };
-        // hand over ring entry i (its copies have landed for this thread)
-        auto hand_over = [&](long long i) {
-          const int j = sg.k0 + (int)((i - idx) >> 1);
-          if (((i - idx) & 1) && (j + 1) * TILE > pre) {
-            // v of drafted tokens: rows keep different ones; this thread's
-            // own pieces are checked, non-finite elements taken out and added
-            // to the rows that keep them at the end
-            uint8_t* tile = ring + (int)(i % CF::kSlots) * CF::kTileBytes;
-            bool bad = false;
-            for (int r = lt / CF::kChunks; r < TILE; r += kLoaders / CF::kChunks)
-              if (j * TILE + r >= pre)
-                bad |= drop_nonfinite<kBf16>(reinterpret_cast<uint4*>(tile + (ch >> 3) * (TILE * 128) + r * 128 +
-                                                                      (((ch & 7) ^ (r & 7)) << 4)));
-            if (bad) *bad_flag = 1;
-          }
-          fence_proxy_async_smem();
-          mbar_arrive(&full[i % CF::kSlots]);
-        };
-        int page0 = page_of(sg.k0 * TILE + lt), page1 = lt < TILE - kLoaders ? page_of(sg.k0 * TILE + kLoaders + lt) : -1;
         const int nk = sg.k1 - sg.k0;
-        for (int j = 0; j < nk; ++j) {
-          const int c0 = (sg.k0 + j) * TILE;
-          longlong2* of = offs + (j & 1) * TILE;
-          of[lt] = offset_of(c0 + lt, page0);
-          if (lt < TILE - kLoaders) of[kLoaders + lt] = offset_of(c0 + kLoaders + lt, page1);
-          if (j + 1 < nk) {
-            page0 = page_of(c0 + TILE + lt);
-            if (lt < TILE - kLoaders) page1 = page_of(c0 + TILE + kLoaders + lt);
+        if constexpr (kTma) {
+          const int P = a.pg.page_size, rows = P < TILE ? P : TILE;
+          // v tiles from js on hold rows that not every query keeps, or nobody does
+          const int js = kBias ? 0 : max(0, pre / TILE - sg.k0);
+          if (warp == kMmaWarp + 1) {
+            // lane i: page i / kBlk of the tile, 64-column block i % kBlk
+            constexpr int kBlk = DP / 64;
+            const int pieces = TILE / rows;
+            auto page_at = [&](int j) -> int {  // -2: past the sequence, -1: not a page
+              const int c = (sg.k0 + j) * TILE + (lane / kBlk) * rows;
+              if (lane / kBlk >= pieces || j >= nk || c >= len) return -2;
+              const int pi = c / P;
+              const int page = a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
+              if (page >= 0 && page < a.pg.num_pages) return page;
+              atomicOr(a.page_error, 1u);
+              return -1;
+            };
+            int next = page_at(0);
+            for (int j = 0; ok && j < nk; ++j) {
+              const int page = next;
+              next = page_at(j + 1);
+              const unsigned there = __ballot_sync(0xffffffffu, page >= 0 && lane % kBlk == 0);
+              const bool gone = __any_sync(0xffffffffu, page == -1);
+              const uint32_t bytes = (uint32_t)__popc(there) * rows * DP * 2;
+              const int slot_c = ((sg.k0 + j) * TILE + (lane / kBlk) * rows) % P;
+#pragma unroll 1
+              for (int kv = 0; kv < 2; ++kv) {
+                const long long i = idx + 2 * j + kv;
+                const int slot = (int)(i % CF::kSlots);
+                if (i >= CF::kSlots) ok = mbar_wait(&empty[slot], (uint32_t)(i / CF::kSlots - 1) & 1u, abort_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                uint8_t* tile = ring + slot * CF::kTileBytes;
+                if (gone) {  // keys of a bad table entry count as zero vectors
+                  for (int pc = 0; pc < pieces; ++pc) {
+                    if (__shfl_sync(0xffffffffu, page, pc * kBlk) != -1) continue;
+                    for (int e = lane; e < rows * 8 * kBlk; e += 32)
+                      *reinterpret_cast<uint4*>(tile + (e / (rows * 8)) * (TILE * 128) + pc * rows * 128 +
+                                                (e % (rows * 8)) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                  }
+                  fence_proxy_async_smem();
+                  __syncwarp();
+                }
+                uint64_t* bar = kv && j >= js ? &raw[slot] : &full[slot];
+                if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+                __syncwarp();
+                if (page >= 0)
+                  tma_load_4d(tile + (lane % kBlk) * (TILE * 128) + (lane / kBlk) * rows * 128, kv ? &tv : &tk, bar,
+                              (lane % kBlk) * 64, slot_c, g, page);
+              }
+            }
+          } else {
+            const int st = lt - 32;
+            for (int j = js; j < nk; ++j) {
+              const long long i = idx + 2 * j + 1;
+              const int slot = (int)(i % CF::kSlots);
+              ok = mbar_wait(&raw[slot], (raw_phase >> slot) & 1u, abort_flag) && ok;
+              raw_phase ^= 1u << slot;
+              ok = !bar_any<kScrubBarrier, kLoaders - 32>(!ok);
+              if (!ok) break;
+              {
+                uint8_t* tile = ring + slot * CF::kTileBytes;
+                const int c0 = (sg.k0 + j) * TILE;
+                for (int r = st; r < TILE; r += kLoaders - 32) {
+                  const int c = c0 + r;
+                  if (c < len && !(kBias && off[c] == -INFINITY)) continue;
+#pragma unroll
+                  for (int e = 0; e < CF::kChunks; ++e)
+                    *reinterpret_cast<uint4*>(tile + (e >> 3) * (TILE * 128) + r * 128 + (e & 7) * 16) =
+                        make_uint4(0u, 0u, 0u, 0u);
+                }
+                if (c0 + TILE > pre) {
+                  // drafted tokens: rows keep different ones; non-finite elements are taken out here and
+                  // added to the rows that keep them at the end
+                  bar_sync<kScrubBarrier, kLoaders - 32>();
+                  bool bad = false;
+                  for (int e = st; e < TILE * CF::kChunks; e += kLoaders - 32)
+                    if (c0 + ((e >> 3) & (TILE - 1)) >= pre)
+                      bad |= drop_nonfinite<kBf16>(reinterpret_cast<uint4*>(tile + e * 16));
+                  if (bad) *bad_flag = 1;
+                }
+                fence_proxy_async_smem();
+              }
+              bar_sync<kScrubBarrier, kLoaders - 32>();
+              if (st == 0) mbar_arrive(&full[slot]);
+            }
+          }
+        } else {
+          auto page_of = [&](int c) -> int {
+            if (c >= len) return -1;
+            const int pi = c / a.pg.page_size;
+            return a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
+          };
+          auto offset_of = [&](int c, int page) {
+            longlong2 o = make_longlong2(-1, -1);
+            if (c >= len || (kBias && off[c] == -INFINITY)) return o;
+            if (page < 0 || page >= a.pg.num_pages) {
+              atomicOr(a.page_error, 1u);
+              return o;
+            }
+            const int at = c % a.pg.page_size;
+            o.x = (long long)page * a.ks[0] + (long long)at * a.ks[1] + g * a.ks[2];
+            o.y = (long long)page * a.vs[0] + (long long)at * a.vs[1] + g * a.vs[2];
+            return o;
+          };
+          // hand over ring entry i (its copies have landed for this thread)
+          auto hand_over = [&](long long i) {
+            const int j = sg.k0 + (int)((i - idx) >> 1);
+            if (((i - idx) & 1) && (j + 1) * TILE > pre) {
+              // v of drafted tokens: rows keep different ones; this thread's
+              // own pieces are checked, non-finite elements taken out and added
+              // to the rows that keep them at the end
+              uint8_t* tile = ring + (int)(i % CF::kSlots) * CF::kTileBytes;
+              bool bad = false;
+              for (int r = lt / CF::kChunks; r < TILE; r += kLoaders / CF::kChunks)
+                if (j * TILE + r >= pre)
+                  bad |= drop_nonfinite<kBf16>(reinterpret_cast<uint4*>(tile + (ch >> 3) * (TILE * 128) + r * 128 +
+                                                                        (((ch & 7) ^ (r & 7)) << 4)));
+              if (bad) *bad_flag = 1;
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&full[i % CF::kSlots]);
+          };
+          int page0 = page_of(sg.k0 * TILE + lt), page1 = lt < TILE - kLoaders ? page_of(sg.k0 * TILE + kLoaders + lt) : -1;
+          for (int j = 0; j < nk; ++j) {
+            const int c0 = (sg.k0 + j) * TILE;
+            longlong2* of = offs + (j & 1) * TILE;
+            of[lt] = offset_of(c0 + lt, page0);
+            if (lt < TILE - kLoaders) of[kLoaders + lt] = offset_of(c0 + kLoaders + lt, page1);
+            if (j + 1 < nk) {
+              page0 = page_of(c0 + TILE + lt);
+              if (lt < TILE - kLoaders) page1 = page_of(c0 + TILE + kLoaders + lt);
+            }
+            ok = !bar_any<kLoaderBarrier, kLoaders>(!ok);
+            if (!ok) break;
+#pragma unroll 1
+            for (int kv = 0; kv < 2; ++kv) {
+              const long long i = idx + 2 * j + kv;
+              const int slot = (int)(i % CF::kSlots);
+              if (i >= CF::kSlots)
+                ok = mbar_wait(&empty[slot], (uint32_t)(i / CF::kSlots - 1) & 1u, abort_flag) && ok;
+              if (ok) {
+                const uint32_t dst = ra + slot * CF::kTileBytes + (ch >> 3) * (TILE * 128);
+                const T* base = kv ? vbase : kbase;
+#pragma unroll 4
+                for (int r = lt / CF::kChunks; r < TILE; r += kLoaders / CF::kChunks) {
+                  const long long o = kv ? of[r].y : of[r].x;
+                  const bool live = in && o >= 0;
+                  cp16(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4), live ? base + o + ch * 8 : base, live);
+                }
+              }
+              asm volatile("cp.async.commit_group;" ::: "memory");
+              if (2 * j + kv >= CF::kLag) {
+                cp_wait<CF::kLag>();
+                hand_over(i - CF::kLag);
+              }
+            }
           }
           ok = !bar_any<kLoaderBarrier, kLoaders>(!ok);
           if (!ok) break;
-#pragma unroll 1
-          for (int kv = 0; kv < 2; ++kv) {
-            const long long i = idx + 2 * j + kv;
-            const int slot = (int)(i % CF::kSlots);
-            if (i >= CF::kSlots)
-              ok = mbar_wait(&empty[slot], (uint32_t)(i / CF::kSlots - 1) & 1u, abort_flag) && ok;
-            if (ok) {
-              const uint32_t dst = ra + slot * CF::kTileBytes + (ch >> 3) * (TILE * 128);
-              const T* base = kv ? vbase : kbase;
-#pragma unroll 4
-              for (int r = lt / CF::kChunks; r < TILE; r += kLoaders / CF::kChunks) {
-                const long long o = kv ? of[r].y : of[r].x;
-                const bool live = in && o >= 0;
-                cp16(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4), live ? base + o + ch * 8 : base, live);
-              }
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            if (2 * j + kv >= CF::kLag) {
-              cp_wait<CF::kLag>();
-              hand_over(i - CF::kLag);
-            }
-          }
+          static_assert(CF::kLag == 2, "the tail below hands over two entries");
+          cp_wait<1>();
+          hand_over(idx + 2 * nk - 2);
+          cp_wait<0>();
+          hand_over(idx + 2 * nk - 1);
         }
-        ok = !bar_any<kLoaderBarrier, kLoaders>(!ok);
-        if (!ok) break;
-        static_assert(CF::kLag == 2, "the tail below hands over two entries");
-        cp_wait<1>();
-        hand_over(idx + 2 * nk - 2);
-        cp_wait<0>();
-        hand_over(idx + 2 * nk - 1);
         idx += 2 * (long long)nk;
       }
       cp_wait<0>();
@@ -423,11 +526,11 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
 #pragma unroll
           for (int c = 0; c < TILE; c += 4) {
             const float4 x = *reinterpret_cast<const float4*>(wbias + c);
-            // (a key of offset -inf is a zero row: its score is finite, and drops out here)
-            v[c] = fmaf(v[c], a.scale, x.x);
-            v[c + 1] = fmaf(v[c + 1], a.scale, x.y);
-            v[c + 2] = fmaf(v[c + 2], a.scale, x.z);
-            v[c + 3] = fmaf(v[c + 3], a.scale, x.w);
+            // (a dropped key's score may be anything)
+            v[c] = x.x == -INFINITY ? -INFINITY : fmaf(v[c], a.scale, x.x);
+            v[c + 1] = x.y == -INFINITY ? -INFINITY : fmaf(v[c + 1], a.scale, x.y);
+            v[c + 2] = x.z == -INFINITY ? -INFINITY : fmaf(v[c + 2], a.scale, x.z);
+            v[c + 3] = x.w == -INFINITY ? -INFINITY : fmaf(v[c + 3], a.scale, x.w);
           }
         }
         if (c0 + TILE > pre) {
@@ -561,20 +664,43 @@ __global__ void __launch_bounds__(kThreads, 1) cached_tc_kernel(const __grid_con
   }
 }
 
-template <int DP, bool kBf16, bool kPair, bool kBias>
+template <int DP, bool kBf16, bool kPair, bool kBias, bool kTma>
 int launch(const CachedArgs& a, cudaStream_t s) {
-  auto kern = cached_tc_kernel<DP, kBf16, kPair, kBias>;
+  auto kern = cached_tc_kernel<DP, kBf16, kPair, kBias, kTma>;
   constexpr size_t bytes = Cfg<DP, kPair>::kSmem;
   if (allow_smem(kern, bytes) != KVBM_OK) return KVBM_ERR_CUDA;
-  kern<<<(unsigned)a.C, kThreads, bytes, s>>>(a);
+  CUtensorMap tk = {}, tv = {};
+  if constexpr (kTma) {
+    const int rows = std::min(a.pg.page_size, TILE);
+    const int64_t ks[4] = {a.ks[0], a.ks[2], a.ks[1], 1}, vs[4] = {a.vs[0], a.vs[2], a.vs[1], 1};
+    if (!make_attention_map(&tk, a.k, kBf16, a.pg.num_pages, a.Hkv, a.pg.page_size, a.D, ks, rows) ||
+        !make_attention_map(&tv, a.v, kBf16, a.pg.num_pages, a.Hkv, a.pg.page_size, a.D, vs, rows))
+      return KVBM_ERR_CUDA;
+  }
+  kern<<<(unsigned)a.C, kThreads, bytes, s>>>(tk, tv, a);
   return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
+}
+
+// Pages that TMA can load as pieces of a 128-key tile: whole 8-row swizzle
+// atoms, even division, no expanded dimension.
+bool pages_by_tma(const CachedArgs& a) {
+  const int P = a.pg.page_size;
+  if (P % 8 != 0 || !(TILE % P == 0 || P % TILE == 0)) return false;
+  for (const long long* st : {a.ks, a.vs})
+    if ((st[0] == 0 && a.pg.num_pages > 1) || (st[1] == 0 && P > 1) || (st[2] == 0 && a.Hkv > 1)) return false;
+  return true;
+}
+
+template <int DP, bool kBf16, bool kPair>
+int launch_p(const CachedArgs& a, cudaStream_t s) {
+  if (pages_by_tma(a))
+    return a.off != nullptr ? launch<DP, kBf16, kPair, true, true>(a, s) : launch<DP, kBf16, kPair, false, true>(a, s);
+  return a.off != nullptr ? launch<DP, kBf16, kPair, true, false>(a, s) : launch<DP, kBf16, kPair, false, false>(a, s);
 }
 
 template <int DP, bool kBf16>
 int launch_d(const CachedArgs& a, cudaStream_t s) {
-  const bool bias = a.off != nullptr;
-  if (a.BM == 2 * TILE) return bias ? launch<DP, kBf16, true, true>(a, s) : launch<DP, kBf16, true, false>(a, s);
-  return bias ? launch<DP, kBf16, false, true>(a, s) : launch<DP, kBf16, false, false>(a, s);
+  return a.BM == 2 * TILE ? launch_p<DP, kBf16, true>(a, s) : launch_p<DP, kBf16, false>(a, s);
 }
 
 }  // namespace

@@ -1366,8 +1366,9 @@ EncodeTiledFn encode_fn() {
 // 4-D map over a [B, H, N, D] operand with unit-stride D: box (128 bytes of
 // D) x 128 rows x 1 x 1, 128-byte swizzle, zero fill outside [N) so ragged
 // tiles read zeros.
+// `rows`: rows of a box.
 bool make_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, int esize, int B, int H, int N,
-              int D, const int64_t* st) {
+              int D, const int64_t* st, int rows = TILE) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return false;
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)N, (cuuint64_t)H, (cuuint64_t)B};
@@ -1377,7 +1378,7 @@ bool make_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, int 
   if (H == 1) hs = row * (uint64_t)N;
   if (B == 1) bs = hs * (uint64_t)H;
   const cuuint64_t strides[3] = {row, hs, bs};
-  const cuuint32_t box[4] = {(cuuint32_t)(128 / esize), (cuuint32_t)TILE, 1, 1};
+  const cuuint32_t box[4] = {(cuuint32_t)(128 / esize), (cuuint32_t)rows, 1, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult r = fn(map, type, 4, const_cast<void*>(base), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -1723,9 +1724,10 @@ int launch_km(const kvbm_problem* p, const WsLayout& L, void* ws, cudaStream_t s
 bool tc_path_enabled() { return encode_fn() != nullptr; }
 
 // The same map for the attention kernels (16-bit operands).
-bool make_attention_map(CUtensorMap* map, const void* base, bool bf16, int B, int H, int N, int D, const int64_t* st) {
+bool make_attention_map(CUtensorMap* map, const void* base, bool bf16, int B, int H, int N, int D, const int64_t* st,
+                        int rows) {
   return make_map(map, base, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, B, H, N, D,
-                  st);
+                  st, rows);
 }
 
 namespace {

@@ -116,6 +116,38 @@ def test_tree(cuda_device, dtype, T, Hq, Hkv, D):
     _check(c, out, lse, tree[0], scale=0.07)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("page", [1, 5, 8, 24, 32, 64, 128, 256, 384])
+@pytest.mark.parametrize("T,Hq,D", [(21, 4, 128), (40, 8, 64), (64, 8, 96)])
+def test_tree_pages(cuda_device, dtype, page, T, Hq, D):
+    """Page sizes that tile 128 keys and ones that do not, bad pages among them, with and without offsets."""
+    c = Case([T, 128, 129, 640, 777, 0], page, Hq, 2, D, T, dtype, cuda_device, seed=page).poison_tail()
+    tree = _tree(6, T, page, cuda_device)
+    out, lse = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, tree_mask=tree)
+    _check(c, out, lse, tree)
+    g = torch.Generator().manual_seed(page)
+    off = (3 * torch.rand(6, 1, c.L, generator=g)).to(cuda_device)
+    off[torch.rand(off.shape, generator=g).to(cuda_device) < 0.3] = -math.inf
+    for b in range(6):
+        for s in (off[b, 0, :c.lens[b]] == -math.inf).nonzero()[:, 0].tolist()[:40]:
+            pg = int(c.table[b, s // page])
+            c.k[pg, s % page] = math.nan
+            c.v[pg, s % page] = math.inf
+    out, lse = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, tree_mask=tree, log_offsets=off)
+    _check(c, out, lse, tree, off=off)
+    kb.check_device_errors()
+    c = Case([640, 777], page, Hq, 2, D, T, dtype, cuda_device, seed=page + 1).poison_tail()
+    pg = int(c.table[1, 100 // page])
+    c.table[1, 100 // page] = 1 << 30
+    out, lse = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens)
+    with pytest.raises(RuntimeError):
+        kb.check_device_errors()
+    c.table[1, 100 // page] = pg
+    c.k[pg] = 0
+    c.v[pg] = 0
+    _check(c, out, lse)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,Hq", [(9, 4), (20, 8), (40, 8), (30, 4)])
 def test_tree_rows_of_their_own(cuda_device, dtype, T, Hq):
