@@ -4,14 +4,14 @@
 //
 // One CTA owns two tiles of 128 query rows (A and B) of one head and streams
 // the key tiles of 128 keys once:
-//   warps 0-3, 4-7  softmax of tile A, of tile B: one thread a row, its 128
-//                   scores read from TMEM into registers; the weights go back
+//   warps 0-7, 8-15 softmax of tile A, of tile B: two threads a row
+//                   (kvbm_attention_tile.cuh); scores from TMEM, weights back
 //                   to TMEM (16 bit, over the scores' columns)
-//   warp 8          MMA issuer: S = Q K^T (operands in shared memory), then
+//   warp 16         MMA issuer: S = Q K^T (operands in shared memory), then
 //                   O += P V with P read from TMEM and V MN-major in shared
 //                   memory as TMA left it
-//   warp 9          TMA producer: K and V rings of two tiles each
-//   warps 10-11     scrub: zero the V rows nobody keeps (masked keys, rows
+//   warp 17         TMA producer: K and V rings of two tiles each
+//   warps 18-19     scrub: zero the V rows nobody keeps (masked keys, rows
 //                   past the sequence) and non-finite elements of the
 //                   diagonal tiles, since 0 * NaN is not 0
 // Why two row tiles: while one tile's softmax runs, the tensor pipe does the
@@ -43,14 +43,14 @@ using namespace sm100;
 
 constexpr int TILE = 128;
 constexpr int ROWS = 2 * TILE;  // query rows of a CTA
-constexpr int kThreads = 384;
-constexpr int kMmaWarp = 8, kTmaWarp = 9;
+constexpr int kThreads = 640;
+constexpr int kMmaWarp = 16, kTmaWarp = 17;
 constexpr int kScrubThreads = 64;
 constexpr int kStages = 2;  // K ring, V ring
-// Registers a thread after the split: 2 softmax warpgroups + 1 of the rest;
-// the launch holds 384 x 168.
-constexpr int kRegsSoftmax = 208, kRegsRest = 88;
-static_assert(2 * kRegsSoftmax + kRegsRest <= 3 * 168, "the split draws on the launch's registers");
+// Registers a thread after the split: 4 softmax warpgroups + 1 of the rest;
+// the launch holds 640 x 96.
+constexpr int kRegsSoftmax = 104, kRegsRest = 64;
+static_assert(4 * kRegsSoftmax + kRegsRest <= 5 * 96, "the split draws on the launch's registers");
 
 template <int DP>
 struct Cfg {
@@ -58,7 +58,7 @@ struct Cfg {
   static constexpr int kBlockBytes = TILE * 128;        // one block of a tile
   static constexpr int kTileBytes = kBlocks * kBlockBytes;
   static constexpr int kBars = 2 + 6 * kStages + 4;
-  static constexpr size_t kSmem = 1024 + (size_t)kTileBytes * (2 + 2 * kStages) + 8 * kBars + 64;
+  static constexpr size_t kSmem = 1024 + (size_t)kTileBytes * (2 + 2 * kStages) + 8 * kBars + 64 + 2 * 4 * TILE * 4;
 };
 
 // The work of a CTA: 256-row tile qt of sequence b, head h; or, past the last
@@ -188,6 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* bad_flag = abort_flag + 1;
   int* item_s = reinterpret_cast<int*>(tmem_slot + 3);  // b, h, qt
   long long* spare_s = reinterpret_cast<long long*>(p_ready + 2) + 4;
+  float* max_s = reinterpret_cast<float*>(spare_s + 4);  // [2 turns][2 tiles][2 halves][TILE]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < 2; ++i) {
         mbar_init(&q_full[i], 1);
         mbar_init(&s_full[i], 1);
-        mbar_init(&p_ready[i], TILE);
+        mbar_init(&p_ready[i], 2 * TILE);
       }
       for (int s = 0; s < kStages; ++s) {
         mbar_init(&k_full[s], 1);
@@ -355,62 +356,75 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     reg_inc<kRegsSoftmax>();
-    const int t = warp >> 2, sub = warp & 3;
+    const int t = warp >> 3, half = (warp >> 2) & 1, sub = warp & 3;
     const int rl = sub * 32 + lane;
     const int row = r0 + t * TILE + rl;
-    const uint32_t ts = tmem + ((uint32_t)(sub * 32) << 16) + t * TILE, to = ts + 256;
+    // this thread's scores, its weights' columns, its output columns
+    constexpr int kOut = DP / 2;
+    const uint32_t lanes = tmem + ((uint32_t)(sub * 32) << 16) + t * TILE;
+    const uint32_t ts = lanes + half * kAttCols, tp = lanes + half * (kAttCols / 2), to = lanes + 256 + half * kOut;
     const int cnt = t == 0 ? nA : nB;
     const int rt0 = r0 + t * TILE;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < cnt; ++j) {
-      const int c0 = j * TILE;
-      bool kk[4];
+      const int c0 = j * TILE + half * kAttCols;
+      bool kk[2];
       if (km != nullptr) {  // before the wait: the loads overlap it
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < 2; ++w) {
           const int c = c0 + w * 32 + lane;
           kk[w] = c < n && km[c] != 0;
         }
       }
       ok = mbar_wait(&s_full[t], j & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
       tc_fence_after();
-      float v[TILE];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) tmem_ld32(ts + 32 * w, *reinterpret_cast<float(*)[32]>(&v[32 * w]));
+      float v[kAttCols];
+      tmem_ld32(ts, *reinterpret_cast<float(*)[32]>(&v[0]));
+      tmem_ld32(ts + 32, *reinterpret_cast<float(*)[32]>(&v[32]));
       tmem_ld_wait();
-      const bool edge = c0 + TILE > n || (a.causal && c0 + TILE - 1 > rt0);
       if (km != nullptr) {
-        uint32_t bits[4];
+        uint32_t bits[2];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) bits[w] = __ballot_sync(0xffffffffu, kk[w]);
+        for (int w = 0; w < 2; ++w) bits[w] = __ballot_sync(0xffffffffu, kk[w]);
 #pragma unroll
-        for (int c = 0; c < TILE; ++c) v[c] = ((bits[c >> 5] >> (c & 31)) & 1u) ? v[c] : -INFINITY;
+        for (int c = 0; c < kAttCols; ++c) v[c] = ((bits[c >> 5] >> (c & 31)) & 1u) ? v[c] : -INFINITY;
       }
-      if (edge) {
-        const int lim = min(a.causal ? row - c0 : TILE - 1, n - 1 - c0);
+      if (c0 + kAttCols > n || (a.causal && c0 + kAttCols - 1 > rt0)) {
+        const int lim = min(a.causal ? row - c0 : kAttCols - 1, n - 1 - c0);
 #pragma unroll
-        for (int c = 0; c < TILE; ++c) v[c] = c <= lim ? v[c] : -INFINITY;
+        for (int c = 0; c < kAttCols; ++c) v[c] = c <= lim ? v[c] : -INFINITY;
       }
-      const float mt = row_max_nan(v) * C;
+      float mt = row_max_nan(v);
+      // the row's other half (past the barrier, its scores are in registers too: the weights may overwrite them)
+      float* mx = max_s + ((j & 1) * 2 + t) * 2 * TILE;
+      mx[half * TILE + rl] = mt;
+      if (bar_any<2 * TILE>(1 + t, !ok)) {
+        ok = false;
+        break;
+      }
+      mt = fmax_nan(mt, mx[(half ^ 1) * TILE + rl]) * C;
       const bool grow = !(mt <= m + kAttGrow);  // (true from -inf to anything finite, and for NaN)
       if (__any_sync(0xffffffffu, grow)) {
         const float mn = grow ? mt : m;
         const float f = m == mn ? 1.f : ex2(m - mn);
         l *= f;
         m = mn;
-        if (j > 0) scale_output<DP>(to, f);
+        if (j > 0) scale_output<kOut>(to, f);
       }
-      l += put_weights<kBf16, false>(v, C, m == -INFINITY ? 0.f : -m, ts);
+      l += put_weights<kBf16, false>(v, C, m == -INFINITY ? 0.f : -m, tp);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&p_ready[t]);
     }
-    if (ok && cnt > 0) {
-      ok = mbar_wait(&s_full[t], cnt & 1, abort_flag);  // O is complete
-      ok = __all_sync(0xffffffffu, ok);
+    if (cnt > 0) {
+      ok = ok && mbar_wait(&s_full[t], cnt & 1, abort_flag);  // O is complete
+      float* ls = max_s + t * 2 * TILE;  // (the turns' slots are free: everyone has read its last maximum)
+      bar_any<2 * TILE>(1 + t, !ok);
+      ls[half * TILE + rl] = l;
+      ok = !bar_any<2 * TILE>(1 + t, !ok);
+      l += ls[(half ^ 1) * TILE + rl];
     }
     if (ok && cnt > 0) {
       tc_fence_after();
@@ -425,7 +439,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint16_t* vg = static_cast<const uint16_t*>(a.v) + sv.k_b * a.vs[0] + g * a.vs[1] +
                            (long long)sv.k_row * a.vs[2];
 #pragma unroll
-      for (int w = 0; w < DP / 32; ++w) {
+      for (int w = 0; w < kOut / 32; ++w) {
+        const int d0 = half * kOut + 32 * w;
         float o[32];
         tmem_ld32(to + 32 * w, o);
         tmem_ld_wait();
@@ -437,8 +452,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (km != nullptr && km[c] == 0) continue;
 #pragma unroll
               for (int e = 0; e < 32; ++e) {
-                if (32 * w + e >= a.D) continue;
-                const uint16_t x = vg[(long long)c * a.vs[2] + 32 * w + e];
+                if (d0 + e >= a.D) continue;
+                const uint16_t x = vg[(long long)c * a.vs[2] + d0 + e];
                 if (!finite16<kBf16>(x)) {
                   float xf;
                   if constexpr (kBf16)
@@ -452,18 +467,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
-            if (32 * w + e >= a.D) continue;  // D % 8 == 0
+            if (d0 + e >= a.D) continue;  // D % 8 == 0
             uint4 r;
             r.x = none ? 0u : pack16<kBf16>(o[e] * inv, o[e + 1] * inv);
             r.y = none ? 0u : pack16<kBf16>(o[e + 2] * inv, o[e + 3] * inv);
             r.z = none ? 0u : pack16<kBf16>(o[e + 4] * inv, o[e + 5] * inv);
             r.w = none ? 0u : pack16<kBf16>(o[e + 6] * inv, o[e + 7] * inv);
-            *reinterpret_cast<uint4*>(out + 32 * w + e) = r;
+            *reinterpret_cast<uint4*>(out + d0 + e) = r;
           }
         }
         __syncwarp();  // the next load is the whole warp's
       }
-      if (row < n)
+      if (row < n && half == 0)
         a.lse[sv.q_b * a.ls[0] + h * a.ls[1] + ((long long)sv.q_row + row) * a.ls[2]] =
             none ? -INFINITY : (m + lg2(l)) * kLn2F;
     }

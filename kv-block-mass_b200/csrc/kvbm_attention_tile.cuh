@@ -1,6 +1,13 @@
-// The softmax of one row of a 128-key tile, shared by the tcgen05 attention
-// kernels: the row's 128 scores are in registers, its weights go to TMEM as
-// the A operand of P V, its output accumulator is in TMEM.
+// The softmax of a 128 x 128 score tile, shared by the tcgen05 attention
+// kernels.  Two threads own a row, 64 scores each in registers; its weights go
+// to TMEM as the A operand of P V, over the scores; its output accumulator is
+// in TMEM, half of the columns to each of the two threads.
+//
+// Why two threads a row: with two tiles in flight the tensor pipe waits for
+// one tile's softmax while it does the other's P V and next S (1024 cycles at
+// D = 128).  One thread a row took about 2600 cycles a tile (128 scores one
+// after another, registers spilled); two need half, and the only price is one
+// exchange of the row maximum through shared memory.
 #pragma once
 
 #include "kvbm_sm100.cuh"
@@ -15,6 +22,7 @@ bool make_attention_map(CUtensorMap* map, const void* base, bool bf16, int B, in
 namespace sm100 {
 
 constexpr int kAttTile = 128;
+constexpr int kAttCols = 64;  // scores of a row in one thread
 // Growth of a row's maximum (base 2) that makes it the new reference: weights
 // stay below 2^8, which both 16-bit types hold at full precision.
 constexpr float kAttGrow = 8.f;
@@ -28,22 +36,22 @@ constexpr int kAttEmu = KVBM_ATT_EMU;
 __host__ __device__ constexpr bool att_emulated(int g) { return ((g + 1) * kAttEmu) / 8 != (g * kAttEmu) / 8; }
 
 // A NaN among the values makes the maximum NaN (and with it the row).
-__device__ __forceinline__ float row_max_nan(const float (&v)[kAttTile]) {
+__device__ __forceinline__ float row_max_nan(const float (&v)[kAttCols]) {
   float mx[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) mx[e] = fmax_nan(v[e], v[e + 4]);
 #pragma unroll
-  for (int c = 8; c < kAttTile; c += 8)
+  for (int c = 8; c < kAttCols; c += 8)
 #pragma unroll
     for (int e = 0; e < 4; ++e) mx[e] = fmax3_nan(mx[e], v[c + e], v[c + e + 4]);
   return fmax3_nan(fmax_nan(mx[0], mx[1]), mx[2], mx[3]);
 }
 
-// Multiplies the row's DP accumulator columns at `to` by f (whole warp).
-template <int DP>
+// Multiplies kCols accumulator columns of the thread's lane at `to` by f (whole warp).
+template <int kCols>
 __device__ __forceinline__ void scale_output(uint32_t to, float f) {
 #pragma unroll
-  for (int w = 0; w < DP / 32; ++w) {
+  for (int w = 0; w < kCols / 32; ++w) {
     float o[32];
     tmem_ld32(to + 32 * w, o);
     tmem_ld_wait();
@@ -53,13 +61,13 @@ __device__ __forceinline__ void scale_output(uint32_t to, float f) {
   }
 }
 
-// Weights of the row, rounded to 16 bits, to the 64 columns at `ts`; returns
-// their float32 sum (of the unrounded values).
+// Weights of the thread's 64 scores, rounded to 16 bits, to the 32 columns at
+// `ts`; returns their float32 sum (of the unrounded values).
 //   kShift false: 2^(v C + shift), shift = -(reference in base 2)
 //   kShift true:  2^((v + shift) C), shift = -(reference), so that a score of
 //                 float32's lowest value less itself is 0
 template <bool kBf16, bool kShift>
-__device__ __forceinline__ float put_weights(const float (&v)[kAttTile], float C, float shift, uint32_t ts) {
+__device__ __forceinline__ float put_weights(const float (&v)[kAttCols], float C, float shift, uint32_t ts) {
   const float2 C2 = make_float2(C, C), N2 = make_float2(shift, shift);
   float2 s0 = make_float2(0.f, 0.f), s1 = s0;
   auto arg = [&](float a, float b) {
@@ -71,7 +79,7 @@ __device__ __forceinline__ float put_weights(const float (&v)[kAttTile], float C
     }
   };
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < kAttCols / 32; ++w) {
     uint32_t p16[16];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -102,6 +110,23 @@ __device__ __forceinline__ bool finite16(uint32_t half) {
   return (half & e) != e;
 }
 
+// Barrier kId of kCount threads, with one answer for all of them: whether any
+// came with `stop`.  (Roles whose wait gave up leave together: nobody stays
+// behind at a barrier.)
+template <int kCount>
+__device__ __forceinline__ bool bar_any(int id, bool stop) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)stop), "r"(id), "n"(kCount)
+      : "memory");
+  return r != 0;
+}
+
 // Zeroes the non-finite 16-bit elements of a 16-byte piece; true if any was.
 template <bool kBf16>
 __device__ __forceinline__ bool drop_nonfinite(uint4* p) {
@@ -123,23 +148,42 @@ __device__ __forceinline__ bool drop_nonfinite(uint4* p) {
   return bad;
 }
 
-// S (+)= Q K^T of a 128 x 128 tile, both K-major with 128-byte swizzle.
+// Descriptors of a tile's K steps differ from the tile's first one by a
+// constant in the low word (addresses stay below 2^18, so no carry leaves the
+// address field).  The tile's own low word is made opaque, or the compiler
+// keeps every step's descriptor of every ring slot alive across the loop and
+// spills them: 70 local loads a tile in the issuing thread (16k prompt: 2.19 ms
+// with them).
+__device__ __forceinline__ uint32_t opaque(uint32_t x) {
+  uint32_t y;
+  asm volatile("mov.u32 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint64_t step_desc(uint64_t base, uint32_t low, uint32_t bytes) {
+  return (base & 0xFFFFFFFF00000000ull) | (uint64_t)(low + (bytes >> 4));
+}
+
+// S = Q K^T of a 128 x 128 tile, both K-major with 128-byte swizzle.
 template <int DP>
 __device__ __forceinline__ void issue_scores(uint32_t d_tmem, uint32_t q, uint32_t k, uint32_t idesc) {
+  const uint64_t base = sw128_desc(0);
+  const uint32_t ql = opaque((uint32_t)sw128_desc(q)), kl = opaque((uint32_t)sw128_desc(k));
 #pragma unroll
   for (int i = 0; i < DP / 64; ++i)
 #pragma unroll
     for (int k4 = 0; k4 < 4; ++k4)
-      mma_f16(d_tmem, sw128_desc(q + i * kAttTile * 128 + k4 * 32), sw128_desc(k + i * kAttTile * 128 + k4 * 32),
+      mma_f16(d_tmem, step_desc(base, ql, i * kAttTile * 128 + k4 * 32), step_desc(base, kl, i * kAttTile * 128 + k4 * 32),
               idesc, (i | k4) != 0);
 }
 
 // O (+)= P V: P (128 x 128, 16 bit) in TMEM, V [128 keys][DP] MN-major.
 template <int DP>
 __device__ __forceinline__ void issue_output(uint32_t d_tmem, uint32_t p_tmem, uint32_t v, uint32_t idesc, bool add) {
+  const uint64_t base = sw128_mn_desc(0, kAttTile * 128);
+  const uint32_t vl = opaque((uint32_t)sw128_mn_desc(v, kAttTile * 128));
 #pragma unroll
   for (int k = 0; k < 8; ++k)  // 16 keys a step
-    mma_f16_ts(d_tmem, p_tmem + k * 8, sw128_mn_desc(v + k * 2048, kAttTile * 128), idesc, (add || k > 0) ? 1u : 0u);
+    mma_f16_ts(d_tmem, p_tmem + k * 8, step_desc(base, vl, k * 2048), idesc, (add || k > 0) ? 1u : 0u);
 }
 
 }  // namespace sm100

@@ -2,10 +2,10 @@
 // paged cache on the tensor cores (tcgen05), bf16 / fp16, D <= 128, split over
 // the keys (kvbm_attention.cu describes the split and the joining).
 //
-// One CTA an SM.  warps 0-3 and 4-7: softmax of two streams, as in prompt
-// attention; warp 8: MMA issuer; warps 9-11: loaders, in one of two ways:
+// One CTA an SM.  warps 0-7 and 8-15: softmax of two streams, two threads a
+// row (kvbm_attention_tile.cuh); warp 16: MMA issuer; warps 17-19: loaders, in one of two ways:
 //   kTma:  pages of a multiple of 8 slots that tile 128 keys evenly (or are a
-//          multiple of 128): warp 9 loads each page with TMA, and warps 10-11
+//          multiple of 128): warp 17 loads each page with TMA, and warps 18-19
 //          zero the v rows nobody keeps in the tiles that hold any (the last
 //          ones, and with log offsets all);
 //   else:  any page size: all three warps read the rows with 16-byte cp.async
@@ -37,13 +37,15 @@ namespace {
 using namespace sm100;
 
 constexpr int TILE = kAttTile;
-constexpr int kThreads = 384;
-constexpr int kMmaWarp = 8;
-constexpr int kLoaders = 96;  // warps 9-11
-constexpr int kLoaderBarrier = 2, kSoftmaxBarrier = 3, kScrubBarrier = 4;
-// Registers a thread after the split: 2 softmax warpgroups + 1 of the rest; the launch holds 384 x 168.
-constexpr int kRegsSoftmax = 208, kRegsRest = 88;
-static_assert(2 * kRegsSoftmax + kRegsRest <= 3 * 168, "the split draws on the launch's registers");
+constexpr int kThreads = 640;
+constexpr int kMmaWarp = 16;
+constexpr int kLoaders = 96;  // warps 17-19
+constexpr int kSoftmax = 4 * TILE;  // softmax threads
+// barriers: 1, 2 the streams' row maxima, then
+constexpr int kLoaderBarrier = 3, kSoftmaxBarrier = 4, kScrubBarrier = 5;
+// Registers a thread after the split: 4 softmax warpgroups + 1 of the rest; the launch holds 640 x 96.
+constexpr int kRegsSoftmax = 104, kRegsRest = 64;
+static_assert(4 * kRegsSoftmax + kRegsRest <= 5 * 96, "the split draws on the launch's registers");
 
 template <int DP, bool kPair>
 struct Cfg {
@@ -58,7 +60,7 @@ struct Cfg {
   static constexpr int kLag = 2;  // copies still in flight when a tile is handed over
   static constexpr int kBars = 1 + 3 * kSlots + 4 + 1;
   static constexpr size_t kRing = (size_t)kTileBytes * (kQTiles + kSlots);
-  static constexpr size_t kSmem = 1024 + kRing + 2 * TILE * 16 + 8 * TILE * 4 + 2 * TILE * 8 + 8 * kBars + 64;
+  static constexpr size_t kSmem = 1024 + kRing + 2 * TILE * 16 + 16 * kAttCols * 4 + 8 * TILE * 4 + 8 * kBars + 64;
   static_assert(kSmem <= 227 * 1024, "one CTA's shared memory");
 };
 
@@ -73,22 +75,6 @@ __device__ __forceinline__ void cp_wait() {
 template <int kId, int kCount>
 __device__ __forceinline__ void bar_sync() {
   asm volatile("bar.sync %0, %1;" ::"n"(kId), "n"(kCount) : "memory");
-}
-
-// The same barrier, with one answer for every thread: whether any came with `stop`.
-// (A role whose wait gave up leaves together: nobody stays behind at a barrier.)
-template <int kId, int kCount>
-__device__ __forceinline__ bool bar_any(bool stop) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %1, 0;\n\t"
-      "bar.red.or.pred q, %2, %3, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"((uint32_t)stop), "n"(kId), "n"(kCount)
-      : "memory");
-  return r != 0;
 }
 
 // The segments of a CTA: parts [k0, k1) of units (b, g, rt), in order.
@@ -130,9 +116,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* q_tile = smem;
   uint8_t* ring = q_tile + CF::kQTiles * CF::kTileBytes;
   longlong2* offs = reinterpret_cast<longlong2*>(smem + CF::kRing);       // [2][TILE]
-  float* bias_s = reinterpret_cast<float*>(offs + 2 * TILE);              // [8 warps][TILE]
-  float2* ml_s = reinterpret_cast<float2*>(bias_s + 8 * TILE);            // [2][TILE]
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(ml_s + 2 * TILE);
+  float* bias_s = reinterpret_cast<float*>(offs + 2 * TILE);              // [16 warps][kAttCols]
+  float* max_s = bias_s + 16 * kAttCols;                                  // [2 turns][2 streams][2 halves][TILE]
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(max_s + 8 * TILE);
   uint64_t *full = q_full + 1, *empty = full + CF::kSlots, *raw = empty + CF::kSlots, *s_full = raw + CF::kSlots;
   uint64_t* p_ready = s_full + 2;
   uint64_t* seg_done = p_ready + 2;
@@ -162,9 +148,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&s_full[i], 1);
-        mbar_init(&p_ready[i], TILE);
+        mbar_init(&p_ready[i], 2 * TILE);
       }
-      mbar_init(seg_done, 2 * TILE);
+      mbar_init(seg_done, kSoftmax);
       fence_mbar_init();
     }
   } else if (warp == kMmaWarp) {
@@ -289,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int b = sg.b, g = sg.g, len = sg.len, pre = len - a.T;
         const float* off = kBias ? a.off + b * a.ob + g * a.oh : nullptr;
         if (seg > 0) ok = mbar_wait(seg_done, (seg - 1) & 1u, abort_flag);  // the queries' tile and O are free
-        ok = !bar_any<kLoaderBarrier, kLoaders>(!ok);
+        ok = !bar_any<kLoaders>(kLoaderBarrier, !ok);
         if (!ok) break;
         for (int i = lt; i < CF::kQTiles * TILE * CF::kChunks; i += kLoaders) {
           const int row = i / CF::kChunks, c = i % CF::kChunks, r = sg.rt * CF::kQTiles * TILE + row;
@@ -364,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const int slot = (int)(i % CF::kSlots);
               ok = mbar_wait(&raw[slot], (raw_phase >> slot) & 1u, abort_flag) && ok;
               raw_phase ^= 1u << slot;
-              ok = !bar_any<kScrubBarrier, kLoaders - 32>(!ok);
+              ok = !bar_any<kLoaders - 32>(kScrubBarrier, !ok);
               if (!ok) break;
               {
                 uint8_t* tile = ring + slot * CF::kTileBytes;
@@ -439,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               page0 = page_of(c0 + TILE + lt);
               if (lt < TILE - kLoaders) page1 = page_of(c0 + TILE + kLoaders + lt);
             }
-            ok = !bar_any<kLoaderBarrier, kLoaders>(!ok);
+            ok = !bar_any<kLoaders>(kLoaderBarrier, !ok);
             if (!ok) break;
 #pragma unroll 1
             for (int kv = 0; kv < 2; ++kv) {
@@ -464,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
-          ok = !bar_any<kLoaderBarrier, kLoaders>(!ok);
+          ok = !bar_any<kLoaders>(kLoaderBarrier, !ok);
           if (!ok) break;
           static_assert(CF::kLag == 2, "the tail below hands over two entries");
           cp_wait<1>();
@@ -479,10 +465,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ---- softmax
     reg_inc<kRegsSoftmax>();
-    const int t = warp >> 2, sub = warp & 3;
+    const int t = warp >> 3, half = (warp >> 2) & 1, sub = warp & 3;
     const int rl = sub * 32 + lane;
-    const uint32_t ts = tmem + ((uint32_t)(sub * 32) << 16) + t * TILE, to = ts + 256;
-    float* wbias = bias_s + warp * TILE;
+    constexpr int kOut = DP / 2;  // output columns a thread scales
+    const uint32_t row_at = tmem + ((uint32_t)(sub * 32) << 16), lanes = row_at + t * TILE;
+    const uint32_t ts = lanes + half * kAttCols, tp = lanes + half * (kAttCols / 2), to = lanes + 256 + half * kOut;
+    float* wbias = bias_s + warp * kAttCols;
     const float C = kBias ? kLog2eF : a.scale * kLog2eF;
     uint32_t sn = 0;  // s_full phases used
     bool ok = true;
@@ -496,6 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (sg.k1 * TILE > pre && r < a.R) {
         if (a.tree != nullptr) {
           const uint8_t* tm = a.tree + b * a.tb + tok * a.tr;
+#pragma unroll 8
           for (int u = 0; u < a.T; ++u) tree |= (unsigned long long)(tm[u] != 0) << u;
         } else {
           tree = ~0ull >> (63 - tok);
@@ -503,12 +492,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       float m = -INFINITY, l = 0.f;
       int done = 0;  // tiles of this stream
-      for (int j = kPair ? 0 : t; ok && j < nk; j += kPair ? 1 : 2, ++done) {
-        const int c0 = (sg.k0 + j) * TILE;
+      for (int j = kPair ? 0 : t; j < nk; j += kPair ? 1 : 2, ++done) {
+        const int c0 = (sg.k0 + j) * TILE + half * kAttCols;
         if constexpr (kBias) {
           __syncwarp();
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
+          for (int w = 0; w < 2; ++w) {
             const int c = c0 + 32 * w + lane;
             wbias[32 * w + lane] = c < len ? off[c] : -INFINITY;
           }
@@ -516,15 +505,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ok = mbar_wait(&s_full[t], sn++ & 1u, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
         tc_fence_after();
-        float v[TILE];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) tmem_ld32(ts + 32 * w, *reinterpret_cast<float(*)[32]>(&v[32 * w]));
+        float v[kAttCols];
+        tmem_ld32(ts, *reinterpret_cast<float(*)[32]>(&v[0]));
+        tmem_ld32(ts + 32, *reinterpret_cast<float(*)[32]>(&v[32]));
         tmem_ld_wait();
         if constexpr (kBias) {
 #pragma unroll
-          for (int c = 0; c < TILE; c += 4) {
+          for (int c = 0; c < kAttCols; c += 4) {
             const float4 x = *reinterpret_cast<const float4*>(wbias + c);
             // (a dropped key's score may be anything)
             v[c] = x.x == -INFINITY ? -INFINITY : fmaf(v[c], a.scale, x.x);
@@ -533,9 +521,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             v[c + 3] = x.w == -INFINITY ? -INFINITY : fmaf(v[c + 3], a.scale, x.w);
           }
         }
-        if (c0 + TILE > pre) {
+        if (c0 + kAttCols > pre) {
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
+          for (int w = 0; w < 2; ++w) {
             const int sh = c0 + 32 * w - pre;  // drafted token of the word's first key
             uint32_t bits;
             if (sh <= -32)
@@ -548,71 +536,81 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int c = 0; c < 32; ++c) v[32 * w + c] = ((bits >> c) & 1u) ? v[32 * w + c] : -INFINITY;
           }
         }
-        const float mt = kBias ? row_max_nan(v) : row_max_nan(v) * C;
+        float mt = row_max_nan(v);
+        // the row's other half (past the barrier its scores are in registers too: the weights may overwrite them)
+        float* mx = max_s + ((done & 1) * 2 + t) * 2 * TILE;
+        mx[half * TILE + rl] = mt;
+        if (bar_any<2 * TILE>(1 + t, !ok)) {
+          ok = false;
+          break;
+        }
+        mt = fmax_nan(mt, mx[(half ^ 1) * TILE + rl]);
+        if (!kBias) mt *= C;
         const bool grow = !(mt <= m + (kBias ? kAttGrow * kLn2F : kAttGrow));
         if (__any_sync(0xffffffffu, grow)) {
           const float mn = grow ? mt : m;
           const float f = m == mn ? 1.f : ex2(kBias ? (m - mn) * kLog2eF : m - mn);
           l *= f;
           m = mn;
-          if (done > 0) scale_output<DP>(to, f);
+          if (done > 0) scale_output<kOut>(to, f);
         }
-        l += put_weights<kBf16, kBias>(v, C, m == -INFINITY ? 0.f : -m, ts);
+        l += put_weights<kBf16, kBias>(v, C, m == -INFINITY ? 0.f : -m, tp);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&p_ready[t]);
       }
-      if (ok && done > 0) {
-        ok = mbar_wait(&s_full[t], sn++ & 1u, abort_flag);  // O is complete
-        ok = __all_sync(0xffffffffu, ok);
-        tc_fence_after();
-      }
-      if (bar_any<kSoftmaxBarrier, 2 * TILE>(!ok)) break;
+      if (ok && done > 0) ok = mbar_wait(&s_full[t], sn++ & 1u, abort_flag);  // O is complete
+      // sums of the halves (and of the streams) meet in the turns' slots, which everyone has read
+      if (bar_any<kSoftmax>(kSoftmaxBarrier, !ok)) break;
+      float* ls = max_s;                 // [2 streams][2 halves][TILE]
+      float* ms = max_s + 4 * TILE;      // [2 streams][TILE]
+      ls[(t * 2 + half) * TILE + rl] = l;
+      if (half == 0) ms[t * TILE + rl] = m;
+      bar_any<kSoftmax>(kSoftmaxBarrier, false);
+      tc_fence_after();
+      l = ls[t * 2 * TILE + rl] + ls[(t * 2 + 1) * TILE + rl];
       // ---- the segment's result
       const bool whole = sg.k0 == 0 && sg.k1 == sg.nt;
       const long long pr = ((long long)blockIdx.x * 2 + (sg.begin >= sg.ufirst ? 0 : 1)) * a.BM +
                            (kPair ? t * TILE + rl : rl);
       float f0 = 1.f, f1 = 0.f;
-      if constexpr (!kPair) {
-        // both streams hold the same rows: stream t joins the columns [t DP / 2, (t + 1) DP / 2)
-        ml_s[t * TILE + rl] = make_float2(m, l);
-        tc_fence_before();
-        bar_sync<kSoftmaxBarrier, 2 * TILE>();
-        tc_fence_after();
-        const float2 x0 = ml_s[rl], x1 = ml_s[TILE + rl];
-        m = fmaxf(x0.x, x1.x);
+      if constexpr (!kPair) {  // both streams hold the same rows
+        const float m0 = ms[rl], m1 = ms[TILE + rl];
+        m = fmaxf(m0, m1);
         const float base = m == -INFINITY ? 0.f : m;
         const float C1 = kBias ? kLog2eF : 1.f;
-        f0 = ex2((x0.x - base) * C1);
-        f1 = ex2((x1.x - base) * C1);
-        l = x0.y * f0 + x1.y * f1;
+        f0 = ex2((m0 - base) * C1);
+        f1 = ex2((m1 - base) * C1);
+        l = (ls[rl] + ls[TILE + rl]) * f0 + (ls[2 * TILE + rl] + ls[3 * TILE + rl]) * f1;
       }
       const bool bad = *bad_flag != 0;
       const float m_nat = kBias ? m : m * kLn2F;
       const bool none = l == 0.f;
       const float inv = none ? 0.f : 1.f / l;
-      const uint32_t o_at = tmem + ((uint32_t)(sub * 32) << 16) + 256;
-      constexpr int kCols = kPair ? DP : DP / 2;
+      // columns of the result: of the thread's own row tile half of them, of the joined streams a quarter
+      constexpr int kCols = kPair ? DP / 2 : DP / 4;
+      const int col0 = kPair ? half * kCols : (t * 2 + half) * kCols;
+      constexpr int kStep = kCols < 32 ? 16 : 32;
       uint16_t* out = static_cast<uint16_t*>(a.out) + b * a.os[0] + h * a.os[1] + tok * a.os[2];
 #pragma unroll
-      for (int w = 0; w < kCols / 32; ++w) {
-        const int d0 = (kPair ? 0 : t * kCols) + 32 * w;
-        float o[32];
+      for (int w = 0; w < kCols / kStep; ++w) {
+        const int d0 = col0 + kStep * w;
+        float o[kStep];
         if constexpr (kPair) {
-          tmem_ld32(to + d0, o);
+          tmem_load<kStep>(row_at + 256 + t * TILE + d0, o);
           tmem_ld_wait();
         } else {
-          float o1[32];
-          tmem_ld32(o_at + d0, o);
-          if (nk > 1) tmem_ld32(o_at + TILE + d0, o1);
+          float o1[kStep];
+          tmem_load<kStep>(row_at + 256 + d0, o);
+          tmem_load<kStep>(row_at + 256 + TILE + d0, o1);
           tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = nk > 1 ? o[e] * f0 + o1[e] * f1 : o[e] * f0;
+          for (int e = 0; e < kStep; ++e) o[e] = nk > 1 ? o[e] * f0 + o1[e] * f1 : o[e] * f0;
         }
         if (r < a.R) {
           if (bad) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
+            for (int e = 0; e < kStep; e += 4) {
               float4 x = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
               if (d0 + e < a.D)
                 add_draft_nonfinite<T>(a, b, g, tok, max(max(pre, 0), sg.k0 * TILE), min(len, sg.k1 * TILE), pre, d0 + e,
@@ -625,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (whole) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
+            for (int e = 0; e < kStep; e += 8) {
               if (d0 + e >= a.D) continue;  // D % 8 == 0
               uint4 x;
               x.x = none ? 0u : pack16<kBf16>(o[e] * inv, o[e + 1] * inv);
@@ -636,21 +634,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           } else {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
+            for (int e = 0; e < kStep; e += 4)
               *reinterpret_cast<float4*>(a.part_o + pr * a.DP + d0 + e) =
                   make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
         }
         __syncwarp();  // the next load is the whole warp's
       }
-      if (r < a.R && (kPair || t == 0)) {
+      if (r < a.R && half == 0 && (kPair || t == 0)) {
         if (whole)
           a.lse[b * a.ls[0] + h * a.ls[1] + tok * a.ls[2]] = none ? -INFINITY : m_nat + logf(l);
         else
           a.part_ml[pr] = make_float2(m_nat, l);
       }
       tc_fence_before();
-      bar_sync<kSoftmaxBarrier, 2 * TILE>();  // everyone has read the flag, ml_s and O
+      bar_any<kSoftmax>(kSoftmaxBarrier, false);  // everyone has read the flag, the sums and O
       if (threadIdx.x == 0) *bad_flag = 0;
       mbar_arrive(seg_done);
     }

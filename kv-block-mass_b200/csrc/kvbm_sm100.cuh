@@ -220,6 +220,25 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// The same for 16 or 32 columns.
+template <int kCols>
+__device__ __forceinline__ void tmem_load(uint32_t taddr, float (&v)[kCols]) {
+  if constexpr (kCols == 32) {
+    tmem_ld32(taddr, v);
+  } else {
+    static_assert(kCols == 16, "16 or 32 columns");
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+  }
+}
+
 // 16 lanes x 256 bits, repeated over 8 blocks of 8 columns starting at
 // `taddr`'s column: thread t of the warp gets, for block m, lanes
 // (lane(taddr) + t/4) and (+ 8) and the columns 8m + 2(t%4) + {0, 1}, in
