@@ -1,13 +1,17 @@
 // The softmax of a 128 x 128 score tile, shared by the tcgen05 attention
-// kernels.  Two threads own a row, 64 scores each in registers; its weights go
-// to TMEM as the A operand of P V, over the scores; its output accumulator is
-// in TMEM, half of the columns to each of the two threads.
+// kernels.  Two threads own a row, 64 scores each, 32 in registers at a time;
+// its weights go to TMEM as the A operand of P V, over the same
+// scores;
+// its output accumulator is in TMEM, half of the columns to each of the two.
 //
 // Why two threads a row: with two tiles in flight the tensor pipe waits for
 // one tile's softmax while it does the other's P V and next S (1024 cycles at
 // D = 128).  One thread a row took about 2600 cycles a tile (128 scores one
 // after another, registers spilled); two need half, and the only price is one
-// exchange of the row maximum through shared memory.
+// exchange of the row maximum through shared memory.  The first 32 scores are
+// read from TMEM twice (for the maximum, and again for the weights): with all
+// 64 in registers the loop spilled (16k causal prompt 2.10 ms, with eight
+// registers a thread less 4.2 ms).
 #pragma once
 
 #include "kvbm_sm100.cuh"
@@ -26,22 +30,24 @@ constexpr int kAttCols = 64;  // scores of a row in one thread
 // Growth of a row's maximum (base 2) that makes it the new reference: weights
 // stay below 2^8, which both 16-bit types hold at full precision.
 constexpr float kAttGrow = 8.f;
-// Of 8 groups of four columns, kAttEmu take their exp2 from the FMA pipe
-// (degree 4, 2.7e-6 relative: far below a 16-bit weight's step, and the row
-// sums' float32 results stay within 1e-6).
+// Of 8 groups of four columns, kAttEmu take their exp2 from the FMA pipe.  None:
+// here the tensor pipe and the power it draws bind, not the exponentials, and
+// the polynomial's instructions cost more than the MUFU time they save (16k
+// causal prompt, single / repeated calls: 0 of 8 1.91 / 2.23 ms, 1 of 8 1.95 /
+// 2.26, 2 of 8 2.00 / 2.32).
 #ifndef KVBM_ATT_EMU
-#define KVBM_ATT_EMU 2
+#define KVBM_ATT_EMU 0
 #endif
 constexpr int kAttEmu = KVBM_ATT_EMU;
 __host__ __device__ constexpr bool att_emulated(int g) { return ((g + 1) * kAttEmu) / 8 != (g * kAttEmu) / 8; }
 
 // A NaN among the values makes the maximum NaN (and with it the row).
-__device__ __forceinline__ float row_max_nan(const float (&v)[kAttCols]) {
+__device__ __forceinline__ float max32_nan(const float (&v)[32]) {
   float mx[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) mx[e] = fmax_nan(v[e], v[e + 4]);
 #pragma unroll
-  for (int c = 8; c < kAttCols; c += 8)
+  for (int c = 8; c < 32; c += 8)
 #pragma unroll
     for (int e = 0; e < 4; ++e) mx[e] = fmax3_nan(mx[e], v[c + e], v[c + e + 4]);
   return fmax3_nan(fmax_nan(mx[0], mx[1]), mx[2], mx[3]);
@@ -61,13 +67,13 @@ __device__ __forceinline__ void scale_output(uint32_t to, float f) {
   }
 }
 
-// Weights of the thread's 64 scores, rounded to 16 bits, to the 32 columns at
-// `ts`; returns their float32 sum (of the unrounded values).
+// Weights of 32 scores, rounded to 16 bits, to the 16 columns at `ts`; returns
+// their float32 sum (of the unrounded values).
 //   kShift false: 2^(v C + shift), shift = -(reference in base 2)
 //   kShift true:  2^((v + shift) C), shift = -(reference), so that a score of
 //                 float32's lowest value less itself is 0
 template <bool kBf16, bool kShift>
-__device__ __forceinline__ float put_weights(const float (&v)[kAttCols], float C, float shift, uint32_t ts) {
+__device__ __forceinline__ float put_weights(const float (&v)[32], float C, float shift, uint32_t ts) {
   const float2 C2 = make_float2(C, C), N2 = make_float2(shift, shift);
   float2 s0 = make_float2(0.f, 0.f), s1 = s0;
   auto arg = [&](float a, float b) {
@@ -78,28 +84,25 @@ __device__ __forceinline__ float put_weights(const float (&v)[kAttCols], float C
       return ffma2(make_float2(a, b), C2, N2);
     }
   };
+  uint32_t p16[16];
 #pragma unroll
-  for (int w = 0; w < kAttCols / 32; ++w) {
-    uint32_t p16[16];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = 32 * w + 4 * e;
-      const float2 x0 = arg(v[c], v[c + 1]), x1 = arg(v[c + 2], v[c + 3]);
-      float2 p0, p1;
-      if (att_emulated(e)) {
-        p0 = exp2_fma2<4>(x0);
-        p1 = exp2_fma2<4>(x1);
-      } else {
-        p0 = make_float2(ex2(x0.x), ex2(x0.y));
-        p1 = make_float2(ex2(x1.x), ex2(x1.y));
-      }
-      s0 = fadd2_ftz(s0, p0);
-      s1 = fadd2_ftz(s1, p1);
-      p16[2 * e] = pack16<kBf16>(p0.x, p0.y);
-      p16[2 * e + 1] = pack16<kBf16>(p1.x, p1.y);
+  for (int e = 0; e < 8; ++e) {
+    const int c = 4 * e;
+    const float2 x0 = arg(v[c], v[c + 1]), x1 = arg(v[c + 2], v[c + 3]);
+    float2 p0, p1;
+    if (att_emulated(e)) {
+      p0 = exp2_fma2<4>(x0);
+      p1 = exp2_fma2<4>(x1);
+    } else {
+      p0 = make_float2(ex2(x0.x), ex2(x0.y));
+      p1 = make_float2(ex2(x1.x), ex2(x1.y));
     }
-    tmem_st16(ts + 16 * w, p16);
+    s0 = fadd2_ftz(s0, p0);
+    s1 = fadd2_ftz(s1, p1);
+    p16[2 * e] = pack16<kBf16>(p0.x, p0.y);
+    p16[2 * e + 1] = pack16<kBf16>(p1.x, p1.y);
   }
+  tmem_st16(ts, p16);
   s0 = fadd2(s0, s1);
   return s0.x + s0.y;
 }
@@ -148,6 +151,42 @@ __device__ __forceinline__ bool drop_nonfinite(uint4* p) {
   return bad;
 }
 
+// Whether the 32 bits hold a non-finite 16-bit element: x * 0 + acc is NaN from
+// then on (one instruction a word).
+template <bool kBf16>
+__device__ __forceinline__ uint32_t mark_nonfinite(uint32_t x, uint32_t acc) {
+  uint32_t r;
+  if constexpr (kBf16)
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(acc));
+  else
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(acc));
+  return r;
+}
+
+// Takes the non-finite elements out of 16-byte pieces first, first + step, ...
+// < count of a tile; true if there were any.  (Eight pieces a test: they are rare.)
+template <bool kBf16, typename Skip>
+__device__ __forceinline__ bool scrub_pieces(uint8_t* tile, int first, int step, int count, Skip&& skip) {
+  bool bad = false;
+  for (int i0 = first; i0 < count; i0 += 8 * step) {
+    uint32_t acc = 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = i0 + u * step;
+      if (i >= count) continue;
+      const uint4 w = *reinterpret_cast<const uint4*>(tile + i * 16);
+      acc = mark_nonfinite<kBf16>(w.x, acc);
+      acc = mark_nonfinite<kBf16>(w.y, acc);
+      acc = mark_nonfinite<kBf16>(w.z, acc);
+      acc = mark_nonfinite<kBf16>(w.w, acc);
+    }
+    if ((acc & 0x7FFF7FFFu) == 0u) continue;
+    for (int i = i0; i < min(count, i0 + 8 * step); i += step)
+      if (!skip(i)) bad |= drop_nonfinite<kBf16>(reinterpret_cast<uint4*>(tile + i * 16));
+  }
+  return bad;
+}
+
 // Descriptors of a tile's K steps differ from the tile's first one by a
 // constant in the low word (addresses stay below 2^18, so no carry leaves the
 // address field).  The tile's own low word is made opaque, or the compiler
@@ -176,14 +215,15 @@ __device__ __forceinline__ void issue_scores(uint32_t d_tmem, uint32_t q, uint32
               idesc, (i | k4) != 0);
 }
 
-// O (+)= P V: P (128 x 128, 16 bit) in TMEM, V [128 keys][DP] MN-major.
+// O (+)= P V: P (128 x 128, 16 bit) in TMEM, the weights of each 32 keys over
+// the first 16 columns of their own scores; V [128 keys][DP] MN-major.
 template <int DP>
 __device__ __forceinline__ void issue_output(uint32_t d_tmem, uint32_t p_tmem, uint32_t v, uint32_t idesc, bool add) {
   const uint64_t base = sw128_mn_desc(0, kAttTile * 128);
   const uint32_t vl = opaque((uint32_t)sw128_mn_desc(v, kAttTile * 128));
 #pragma unroll
   for (int k = 0; k < 8; ++k)  // 16 keys a step
-    mma_f16_ts(d_tmem, p_tmem + k * 8, step_desc(base, vl, k * 2048), idesc, (add || k > 0) ? 1u : 0u);
+    mma_f16_ts(d_tmem, p_tmem + (k >> 1) * 32 + (k & 1) * 8, step_desc(base, vl, k * 2048), idesc, (add || k > 0) ? 1u : 0u);
 }
 
 }  // namespace sm100

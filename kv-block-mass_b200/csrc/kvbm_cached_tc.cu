@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&s_full[i], 1);
-        mbar_init(&p_ready[i], 2 * TILE);
+        mbar_init(&p_ready[i], 2 * TILE / 32);
       }
       mbar_init(seg_done, kSoftmax);
       fence_mbar_init();
@@ -367,10 +367,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                   // drafted tokens: rows keep different ones; non-finite elements are taken out here and
                   // added to the rows that keep them at the end
                   bar_sync<kScrubBarrier, kLoaders - 32>();
-                  bool bad = false;
-                  for (int e = st; e < TILE * CF::kChunks; e += kLoaders - 32)
-                    if (c0 + ((e >> 3) & (TILE - 1)) >= pre)
-                      bad |= drop_nonfinite<kBf16>(reinterpret_cast<uint4*>(tile + e * 16));
+                  const bool bad =
+                      scrub_pieces<kBf16>(tile, st, kLoaders - 32, TILE * CF::kChunks,
+                                          [&](int e) { return c0 + ((e >> 3) & (TILE - 1)) < pre; });
                   if (bad) *bad_flag = 1;
                 }
                 fence_proxy_async_smem();
@@ -469,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int rl = sub * 32 + lane;
     constexpr int kOut = DP / 2;  // output columns a thread scales
     const uint32_t row_at = tmem + ((uint32_t)(sub * 32) << 16), lanes = row_at + t * TILE;
-    const uint32_t ts = lanes + half * kAttCols, tp = lanes + half * (kAttCols / 2), to = lanes + 256 + half * kOut;
+    const uint32_t ts = lanes + half * kAttCols, to = lanes + 256 + half * kOut;
     float* wbias = bias_s + warp * kAttCols;
     const float C = kBias ? kLog2eF : a.scale * kLog2eF;
     uint32_t sn = 0;  // s_full phases used
@@ -506,25 +505,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = mbar_wait(&s_full[t], sn++ & 1u, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
-        float v[kAttCols];
-        tmem_ld32(ts, *reinterpret_cast<float(*)[32]>(&v[0]));
-        tmem_ld32(ts + 32, *reinterpret_cast<float(*)[32]>(&v[32]));
-        tmem_ld_wait();
-        if constexpr (kBias) {
+        auto scores = [&](int i, float (&v)[32]) {
+          tmem_ld32(ts + 32 * i, v);
+          tmem_ld_wait();
+          if constexpr (kBias) {
 #pragma unroll
-          for (int c = 0; c < kAttCols; c += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(wbias + c);
-            // (a dropped key's score may be anything)
-            v[c] = x.x == -INFINITY ? -INFINITY : fmaf(v[c], a.scale, x.x);
-            v[c + 1] = x.y == -INFINITY ? -INFINITY : fmaf(v[c + 1], a.scale, x.y);
-            v[c + 2] = x.z == -INFINITY ? -INFINITY : fmaf(v[c + 2], a.scale, x.z);
-            v[c + 3] = x.w == -INFINITY ? -INFINITY : fmaf(v[c + 3], a.scale, x.w);
+            for (int c = 0; c < 32; c += 4) {
+              const float4 x = *reinterpret_cast<const float4*>(wbias + 32 * i + c);
+              // (a dropped key's score may be anything)
+              v[c] = x.x == -INFINITY ? -INFINITY : fmaf(v[c], a.scale, x.x);
+              v[c + 1] = x.y == -INFINITY ? -INFINITY : fmaf(v[c + 1], a.scale, x.y);
+              v[c + 2] = x.z == -INFINITY ? -INFINITY : fmaf(v[c + 2], a.scale, x.z);
+              v[c + 3] = x.w == -INFINITY ? -INFINITY : fmaf(v[c + 3], a.scale, x.w);
+            }
           }
-        }
-        if (c0 + kAttCols > pre) {
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const int sh = c0 + 32 * w - pre;  // drafted token of the word's first key
+          if (c0 + kAttCols > pre) {
+            const int sh = c0 + 32 * i - pre;  // drafted token of the first key
             uint32_t bits;
             if (sh <= -32)
               bits = 0xffffffffu;
@@ -533,11 +529,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             else
               bits = sh < 64 ? (uint32_t)(tree >> sh) : 0u;
 #pragma unroll
-            for (int c = 0; c < 32; ++c) v[32 * w + c] = ((bits >> c) & 1u) ? v[32 * w + c] : -INFINITY;
+            for (int c = 0; c < 32; ++c) v[c] = ((bits >> c) & 1u) ? v[c] : -INFINITY;
           }
-        }
-        float mt = row_max_nan(v);
-        // the row's other half (past the barrier its scores are in registers too: the weights may overwrite them)
+        };
+        float v[32];
+        scores(0, v);
+        float mt = max32_nan(v);
+        scores(1, v);
+        mt = fmax_nan(mt, max32_nan(v));
+        // the row's other half
         float* mx = max_s + ((done & 1) * 2 + t) * 2 * TILE;
         mx[half * TILE + rl] = mt;
         if (bar_any<2 * TILE>(1 + t, !ok)) {
@@ -554,10 +554,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           m = mn;
           if (done > 0) scale_output<kOut>(to, f);
         }
-        l += put_weights<kBf16, kBias>(v, C, m == -INFINITY ? 0.f : -m, tp);
+        const float shift = m == -INFINITY ? 0.f : -m;
+        l += put_weights<kBf16, kBias>(v, C, shift, ts + 32);
+        scores(0, v);
+        l += put_weights<kBf16, kBias>(v, C, shift, ts);
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&p_ready[t]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[t]);  // one arrival a warp
       }
       if (ok && done > 0) ok = mbar_wait(&s_full[t], sn++ & 1u, abort_flag);  // O is complete
       // sums of the halves (and of the streams) meet in the turns' slots, which everyone has read

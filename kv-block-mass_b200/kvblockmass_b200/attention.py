@@ -40,12 +40,19 @@ _I3, _I4 = ctypes.c_int64 * 3, ctypes.c_int64 * 4
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 
+# The current stream's handle by device index, without building a Stream object
+# where this torch has the function (2 us of a call that runs for 15).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _on_device(dev: torch.device, call):
     """``call(stream)`` with ``dev`` current, on its current stream."""
-    if torch.cuda.current_device() == dev.index:
-        return call(torch.cuda.current_stream(dev).cuda_stream)
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        return call(_raw_stream(index))
     with torch.cuda.device(dev):
-        return call(torch.cuda.current_stream(dev).cuda_stream)
+        return call(_raw_stream(index))
 
 
 def _int32_on(t: torch.Tensor, dev, name: str) -> torch.Tensor:
@@ -171,7 +178,7 @@ def attention_b200(q, k, v, attn_mask=None, causal=False, scale=None, *, seq_len
         _check_out("out", out, q.shape, q.dtype, q.device)
         _no_overlap("out", out, {"q": q, "k": k, "v": v})
     if lse_out is None:
-        lse_out = torch.empty(B, Hq, N, dtype=torch.float32, device=q.device) if fill or lens is None else \
+        lse_out = q.new_empty((B, Hq, N), dtype=torch.float32) if fill or lens is None else \
             torch.full((B, Hq, N), float("-inf"), dtype=torch.float32, device=q.device)
     else:
         _check_out("lse_out", lse_out, (B, Hq, N), torch.float32, q.device)
@@ -209,13 +216,12 @@ def attention_varlen(q, k, v, cu_seqlens, max_seqlen=None, causal=False, scale=N
     cu = _int32_on(cu_seqlens, q.device, "cu_seqlens")
     fill = out is None and lse_out is None
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if fill else torch.zeros(q.shape, dtype=q.dtype,
-                                                                                            device=q.device)
+        out = q.new_empty((T, Hq, D)) if fill else q.new_zeros((T, Hq, D))
     else:
         _check_out("out", out, q.shape, q.dtype, q.device)
         _no_overlap("out", out, {"q": q, "k": k, "v": v})
     if lse_out is None:
-        lse_out = torch.empty(Hq, T, dtype=torch.float32, device=q.device) if fill else \
+        lse_out = q.new_empty((Hq, T), dtype=torch.float32) if fill else \
             torch.full((Hq, T), float("-inf"), dtype=torch.float32, device=q.device)
     else:
         _check_out("lse_out", lse_out, (Hq, T), torch.float32, q.device)
@@ -338,12 +344,12 @@ def _cached_args(q, k_cache, v_cache, block_table, seq_lens, tree_mask, log_offs
     if out is not None or lse_out is not None:
         ins = {"q": q, "k_cache": k_cache, "v_cache": v_cache}
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty((B, Hq, T, D))
     else:
         _check_out("out", out, q.shape, q.dtype, q.device)
         _no_overlap("out", out, ins)
     if lse_out is None:
-        lse_out = torch.empty(B, Hq, T, dtype=torch.float32, device=q.device)
+        lse_out = q.new_empty((B, Hq, T), dtype=torch.float32)
     else:
         _check_out("lse_out", lse_out, (B, Hq, T), torch.float32, q.device)
         _no_overlap("lse_out", lse_out, ins)

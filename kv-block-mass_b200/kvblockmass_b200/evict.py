@@ -78,8 +78,8 @@ def evict_cache(k_cache, v_cache, block_table, seq_lens, weights, budget, *, n_s
         if cap < budget:
             raise ValueError(f"capacity={cap} < budget={budget}")
         # a head's slots one after another: the next reader streams them
-        both = torch.empty(2, B, Hkv, cap, D, dtype=k_cache.dtype, device=dev).transpose(2, 3)
-        ko, vo = both.unbind(0)
+        ko = k_cache.new_empty((B, Hkv, cap, D)).transpose(1, 2)
+        vo = k_cache.new_empty((B, Hkv, cap, D)).transpose(1, 2)
     else:
         ko, vo = out
         if not isinstance(ko, torch.Tensor) or ko.dim() != 4:
@@ -103,13 +103,10 @@ def evict_cache(k_cache, v_cache, block_table, seq_lens, weights, budget, *, n_s
     a.seq_lens = lens.data_ptr()
     a.weights, a.weights_bstride, a.weights_hstride, a.weight_heads = w.data_ptr(), wb, wh, Hw
     a.budget, a.n_sinks, a.recency, a.capacity, a.zero_tail = budget, n_sinks, recency, cap, int(out is None)
-    # one block of memory for the three small results: slots and lengths are int32, weights float32
-    n = B * Hw * budget
-    small = torch.empty(2 * n + B, dtype=torch.int32, device=dev)
-    kept, new_lens = small[:n].view(B, Hw, budget), small[2 * n:]
-    wout = small[n:2 * n].view(torch.float32).view(B, Hw, budget)
-    a.kept_out = small.data_ptr()
-    a.weights_out, a.seq_lens_out = a.kept_out + 4 * n, a.kept_out + 8 * n
+    kept = w.new_empty((B, Hw, budget), dtype=torch.int32)
+    wout = w.new_empty((B, Hw, budget))
+    new_lens = w.new_empty((B,), dtype=torch.int32)
+    a.kept_out, a.weights_out, a.seq_lens_out = kept.data_ptr(), wout.data_ptr(), new_lens.data_ptr()
     code = _on_device(dev, lambda stream: _lib.load().kvbm_evict_cache(ctypes.byref(a), stream))
     if code != _lib.KVBM_OK:
         _fail(code, "evict_cache")
