@@ -277,16 +277,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (seg > 0) ok = mbar_wait(seg_done, (seg - 1) & 1u, abort_flag);  // the queries' tile and O are free
         ok = !bar_any<kLoaders>(kLoaderBarrier, !ok);
         if (!ok) break;
-        for (int i = lt; i < CF::kQTiles * TILE * CF::kChunks; i += kLoaders) {
-          const int row = i / CF::kChunks, c = i % CF::kChunks, r = sg.rt * CF::kQTiles * TILE + row;
-          uint4 w = make_uint4(0u, 0u, 0u, 0u);
-          if (r < a.R && c * 8 < a.D)
-            w = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.qs[0] +
-                                                (long long)(g * a.G + r / a.T) * a.qs[1] +
-                                                (long long)(r % a.T) * a.qs[2] + c * 8);
-          const int rl = row % TILE;
-          *reinterpret_cast<uint4*>(q_tile + (row / TILE) * CF::kTileBytes + (c >> 3) * (TILE * 128) + rl * 128 +
-                                    (((c & 7) ^ (rl & 7)) << 4)) = w;
+        // queries: eight pieces a thread in flight (one at a time, this took as long as 20 key tiles)
+        constexpr int kPieces = CF::kQTiles * TILE * CF::kChunks, kAhead = 8;
+        for (int i0 = lt; i0 < kPieces; i0 += kAhead * kLoaders) {
+          uint4 w[kAhead];
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            const int i = i0 + u * kLoaders, row = i / CF::kChunks, c = i % CF::kChunks;
+            const int r = sg.rt * CF::kQTiles * TILE + row;
+            w[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (i < kPieces && r < a.R && c * 8 < a.D)
+              w[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.qs[0] +
+                                                     (long long)(g * a.G + r / a.T) * a.qs[1] +
+                                                     (long long)(r % a.T) * a.qs[2] + c * 8);
+          }
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            const int i = i0 + u * kLoaders, row = i / CF::kChunks, c = i % CF::kChunks, rl = row % TILE;
+            if (i < kPieces)
+              *reinterpret_cast<uint4*>(q_tile + (row / TILE) * CF::kTileBytes + (c >> 3) * (TILE * 128) + rl * 128 +
+                                        (((c & 7) ^ (rl & 7)) << 4)) = w[u];
+          }
         }
         fence_proxy_async_smem();
         mbar_arrive(q_full);
