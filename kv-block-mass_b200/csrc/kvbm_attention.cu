@@ -428,96 +428,102 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(const __grid_cons
 }
 
 // Joins the partials of every split unit, and writes the rows of sequences
-// with no keys (out 0, lse -inf).  One warp per row, grid (B * Hkv * RT, BM / 8);
-// partials in CTA order: the same bits on every run.  Lanes read 32 partials'
-// (m, l) at once and then stream their output rows, eight loads in flight.
-template <typename T>
+// with no keys (out 0, lse -inf).  A warp takes kMergeRows / 8 rows, one after
+// another, grid (B * Hkv * RT, BM / kMergeRows); partials in CTA order: the same
+// bits on every run.  Lanes read 32 partials' (m, l) at once and then stream
+// their output rows, eight loads in flight.  kCols: columns a lane holds (4 for
+// D <= 128, else 8).
+constexpr int kMergeRows = 16;
+template <typename T, int kCols>
 __global__ void __launch_bounds__(256) cached_merge_kernel(const __grid_constant__ CachedArgs a) {
   const int unit = blockIdx.x, b = unit / (a.Hkv * a.RT), u = unit % (a.Hkv * a.RT), g = u / a.RT, rt = u % a.RT;
-  const int rl = blockIdx.y * 8 + threadIdx.x / 32, r = rt * a.BM + rl, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31;
   long long pre, total;
   warp_tile_prefix(a, b, &pre, &total);
   const int nt = (cached_len(a, b) + a.KT - 1) / a.KT;
+  const long long t0 = pre + (long long)u * nt, t1 = t0 + nt;
+  const int i0 = nt > 0 ? (int)split_owner(t0, total, a.C) : 0, i1 = nt > 0 ? (int)split_owner(t1 - 1, total, a.C) : 0;
+  // the slot that holds the unit's share of CTA i (-1: a CTA without tiles)
+  auto slot_of = [&](int i) -> long long {
+    if (i > i1) return -1;
+    const long long s0 = split_begin(i, total, a.C), s1 = split_begin(i + 1, total, a.C);
+    return s0 == s1 ? -1 : (long long)i * 2 + (s0 >= t0 ? 0 : 1);
+  };
+  const long long first = slot_of(i0 + lane);
   // launched while the split kernel runs: what is above overlaps it, and every
   // thread waits here for its results
   cudaGridDependencySynchronize();
-  if (rl >= a.BM || r >= a.R) return;
-  const int h = g * a.G + r / a.T, tok = r % a.T;
-  T* out = static_cast<T*>(a.out) + b * a.os[0] + h * a.os[1] + tok * a.os[2];
-  float* lse = a.lse + b * a.ls[0] + h * a.ls[1] + tok * a.ls[2];
-  if (nt == 0) {
-    for (int d = lane; d < a.D; d += 32) out[d * a.os[3]] = from_f32<T>(0.f);
-    if (lane == 0) *lse = -INFINITY;
-    return;
-  }
-  const long long t0 = pre + (long long)u * nt, t1 = t0 + nt;
-  const int i0 = (int)split_owner(t0, total, a.C), i1 = (int)split_owner(t1 - 1, total, a.C);
-  if (i0 == i1) return;  // finished by its CTA
-  auto load_ml = [&](int i, long long* pr) {
-    *pr = 0;
-    if (i > i1) return make_float2(-INFINITY, 0.f);
-    const long long s0 = split_begin(i, total, a.C), s1 = split_begin(i + 1, total, a.C);
-    if (s0 == s1) return make_float2(-INFINITY, 0.f);  // a CTA without tiles
-    *pr = ((long long)i * 2 + (s0 >= t0 ? 0 : 1)) * a.BM + rl;
-    return a.part_ml[*pr];
-  };
-  long long pr;
-  float2 ml = load_ml(i0 + lane, &pr);
-  float m = ml.x;
-  for (int base = i0 + 32; base <= i1; base += 32) {
-    long long p2;
-    m = fmaxf(m, load_ml(base + lane, &p2).x);
-  }
+  if (nt > 0 && i0 == i1) return;  // finished by its CTA
+  const int lanes = a.DP < 32 * kCols ? a.DP / kCols : 32;
+  for (int rl = blockIdx.y * kMergeRows + threadIdx.x / 32; rl < (int)(blockIdx.y + 1) * kMergeRows; rl += 8) {
+    const int r = rt * a.BM + rl;
+    if (rl >= a.BM || r >= a.R) return;
+    const int h = g * a.G + r / a.T, tok = r % a.T;
+    T* out = static_cast<T*>(a.out) + b * a.os[0] + h * a.os[1] + tok * a.os[2];
+    float* lse = a.lse + b * a.ls[0] + h * a.ls[1] + tok * a.ls[2];
+    if (nt == 0) {
+      for (int d = lane; d < a.D; d += 32) out[d * a.os[3]] = from_f32<T>(0.f);
+      if (lane == 0) *lse = -INFINITY;
+      continue;
+    }
+    auto load_ml = [&](long long slot) {
+      return slot < 0 ? make_float2(-INFINITY, 0.f) : a.part_ml[slot * a.BM + rl];
+    };
+    long long slot = first;
+    float2 ml = load_ml(slot);
+    float m = ml.x;
+    for (int base = i0 + 32; base <= i1; base += 32) m = fmaxf(m, load_ml(slot_of(base + lane)).x);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float ref = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-  const int lanes = a.DP < 128 ? a.DP / 4 : 32;  // lanes that hold four columns each (DP = 256: twice four)
-  for (int base = i0; base <= i1; base += 32) {
-    if (base > i0) ml = load_ml(base + lane, &pr);
-    // (a partial that kept nothing has l = 0; a NaN maximum gives a NaN factor)
-    const float f = ml.y == 0.f ? 0.f : exp2f((ml.x - ref) * kLog2eF);
-    float lp = ml.y * f;
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f, acc[kCols];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) lp += __shfl_xor_sync(0xffffffffu, lp, o);
-    l += lp;
-    const int n = min(32, i1 - base + 1);
-    for (int k0 = 0; k0 < n; k0 += 8) {
-      float4 x[8], y[8];
-      float fk[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        fk[i] = __shfl_sync(0xffffffffu, f, (k0 + i) & 31);
-        const long long pk = __shfl_sync(0xffffffffu, pr, (k0 + i) & 31);
-        const bool in = k0 + i < n && fk[i] != 0.f && lane < lanes;
-        const float4* src = reinterpret_cast<const float4*>(a.part_o + pk * a.DP) + lane;
-        x[i] = y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (in) x[i] = src[0];
-        if (in && a.DP > 128) y[i] = src[32];
+    for (int e = 0; e < kCols; ++e) acc[e] = 0.f;
+    for (int base = i0; base <= i1; base += 32) {
+      if (base > i0) {
+        slot = slot_of(base + lane);
+        ml = load_ml(slot);
       }
+      // (a partial that kept nothing has l = 0; a NaN maximum gives a NaN factor)
+      const float f = ml.y == 0.f ? 0.f : exp2f((ml.x - ref) * kLog2eF);
+      float lp = ml.y * f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        acc[0] = make_float4(fmaf(x[i].x, fk[i], acc[0].x), fmaf(x[i].y, fk[i], acc[0].y),
-                             fmaf(x[i].z, fk[i], acc[0].z), fmaf(x[i].w, fk[i], acc[0].w));
-        acc[1] = make_float4(fmaf(y[i].x, fk[i], acc[1].x), fmaf(y[i].y, fk[i], acc[1].y),
-                             fmaf(y[i].z, fk[i], acc[1].z), fmaf(y[i].w, fk[i], acc[1].w));
+      for (int o = 16; o > 0; o >>= 1) lp += __shfl_xor_sync(0xffffffffu, lp, o);
+      l += lp;
+      const int n = min(32, i1 - base + 1);
+      for (int k0 = 0; k0 < n; k0 += 8) {
+        float x[8][kCols], fk[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          fk[i] = __shfl_sync(0xffffffffu, f, (k0 + i) & 31);
+          const long long pk = __shfl_sync(0xffffffffu, slot, (k0 + i) & 31);
+          const bool in = k0 + i < n && fk[i] != 0.f && lane < lanes;
+          const float4* src = reinterpret_cast<const float4*>(a.part_o + (pk * a.BM + rl) * a.DP + lane * kCols);
+#pragma unroll
+          for (int q = 0; q < kCols / 4; ++q) {
+            const float4 y = in ? src[q] : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[i][4 * q] = y.x;
+            x[i][4 * q + 1] = y.y;
+            x[i][4 * q + 2] = y.z;
+            x[i][4 * q + 3] = y.w;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int e = 0; e < kCols; ++e) acc[e] = fmaf(x[i][e], fk[i], acc[e]);
       }
     }
-  }
-  const float inv = 1.f / l;
+    const float inv = 1.f / l;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const float v[4] = {acc[half].x, acc[half].y, acc[half].z, acc[half].w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int d = half * 128 + lane * 4 + e;
-      if (lane < lanes && d < a.D) out[d * a.os[3]] = from_f32<T>(l == 0.f ? 0.f : v[e] * inv);
+    for (int e = 0; e < kCols; ++e) {
+      const int d = lane * kCols + e;
+      if (lane < lanes && d < a.D) out[d * a.os[3]] = from_f32<T>(l == 0.f ? 0.f : acc[e] * inv);
     }
-  }
-  if (lane == 0) {
-    *lse = l == 0.f ? -INFINITY : m + logf(l);
-    if (a.stats) a.stats[(long long)(b * a.Hkv + g) * a.R + r] = make_float2(m, l == 0.f ? 0.f : inv);
+    if (lane == 0) {
+      *lse = l == 0.f ? -INFINITY : m + logf(l);
+      if (a.stats) a.stats[(long long)(b * a.Hkv + g) * a.R + r] = make_float2(m, l == 0.f ? 0.f : inv);
+    }
   }
 }
 
@@ -633,6 +639,14 @@ int cached_simt_d(const CachedArgs& a, cudaStream_t s) {
   return cached_simt<T, 4, 256>(a, s);
 }
 
+template <typename T>
+int merge(const CachedArgs& a, cudaStream_t s) {
+  const int rows = a.R < a.BM ? a.R : a.BM;
+  const dim3 grid((unsigned)(a.B * a.Hkv * a.RT), (unsigned)((rows + kMergeRows - 1) / kMergeRows));
+  return a.DP <= 128 ? launch_dependent(cached_merge_kernel<T, 4>, grid, 256, s, a)
+                     : launch_dependent(cached_merge_kernel<T, 8>, grid, 256, s, a);
+}
+
 }  // namespace
 
 int launch_prompt_simt(const PromptArgs& a, int dtype, cudaStream_t s) {
@@ -660,11 +674,9 @@ int launch_cached_simt(const CachedArgs& a, int dtype, cudaStream_t s) {
 }
 
 int launch_cached_merge(const CachedArgs& a, int dtype, cudaStream_t s) {
-  const int rows = a.R < a.BM ? a.R : a.BM;
-  const dim3 grid((unsigned)(a.B * a.Hkv * a.RT), (unsigned)((rows + 7) / 8));
-  if (dtype == KVBM_F32) return launch_dependent(cached_merge_kernel<float>, grid, 256, s, a);
-  if (dtype == KVBM_BF16) return launch_dependent(cached_merge_kernel<__nv_bfloat16>, grid, 256, s, a);
-  return launch_dependent(cached_merge_kernel<__half>, grid, 256, s, a);
+  if (dtype == KVBM_F32) return merge<float>(a, s);
+  if (dtype == KVBM_BF16) return merge<__nv_bfloat16>(a, s);
+  return merge<__half>(a, s);
 }
 
 int launch_cached_weights(const CachedArgs& a, cudaStream_t s) {

@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       *sched_b = b;
       *abort_flag = 0;
       *bad_flag = 0;
-      mbar_init(q_full, kLoaders);
+      mbar_init(q_full, kTma ? kLoaders - 32 : kLoaders);
       for (int i = 0; i < CF::kSlots; ++i) {
         mbar_init(&full[i], kTma ? 1 : kLoaders);
         mbar_init(&empty[i], 1);
@@ -274,33 +274,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (uint32_t seg = 0; ok && sg.next(a); ++seg) {
         const int b = sg.b, g = sg.g, len = sg.len, pre = len - a.T;
         const float* off = kBias ? a.off + b * a.ob + g * a.oh : nullptr;
-        if (seg > 0) ok = mbar_wait(seg_done, (seg - 1) & 1u, abort_flag);  // the queries' tile and O are free
-        ok = !bar_any<kLoaders>(kLoaderBarrier, !ok);
-        if (!ok) break;
-        // queries: eight pieces a thread in flight (one at a time, this took as long as 20 key tiles)
-        constexpr int kPieces = CF::kQTiles * TILE * CF::kChunks, kAhead = 8;
-        for (int i0 = lt; i0 < kPieces; i0 += kAhead * kLoaders) {
-          uint4 w[kAhead];
-#pragma unroll
-          for (int u = 0; u < kAhead; ++u) {
-            const int i = i0 + u * kLoaders, row = i / CF::kChunks, c = i % CF::kChunks;
+        // queries, by the scrub warps where warp 17 is free to start on the keys
+        constexpr int kFirst = kTma ? 32 : 0, kCount = kLoaders - kFirst;
+        if (lt >= kFirst) {
+          if (seg > 0) ok = mbar_wait(seg_done, (seg - 1) & 1u, abort_flag);  // the queries' tile and O are free
+          ok = !bar_any<kCount>(kLoaderBarrier, !ok);
+          if (!ok) break;
+          const uint32_t qa = smem_u32(q_tile);
+          const T* qbase = static_cast<const T*>(a.q);
+          for (int i = lt - kFirst; i < CF::kQTiles * TILE * CF::kChunks; i += kCount) {
+            const int row = i / CF::kChunks, c = i % CF::kChunks, rl = row % TILE;
             const int r = sg.rt * CF::kQTiles * TILE + row;
-            w[u] = make_uint4(0u, 0u, 0u, 0u);
-            if (i < kPieces && r < a.R && c * 8 < a.D)
-              w[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.qs[0] +
-                                                     (long long)(g * a.G + r / a.T) * a.qs[1] +
-                                                     (long long)(r % a.T) * a.qs[2] + c * 8);
+            const bool live = r < a.R && c * 8 < a.D;
+            cp16(qa + (row / TILE) * CF::kTileBytes + (c >> 3) * (TILE * 128) + rl * 128 + (((c & 7) ^ (rl & 7)) << 4),
+                 live ? qbase + b * a.qs[0] + (long long)(g * a.G + r / a.T) * a.qs[1] + (long long)(r % a.T) * a.qs[2] +
+                            c * 8
+                      : qbase,
+                 live);
           }
-#pragma unroll
-          for (int u = 0; u < kAhead; ++u) {
-            const int i = i0 + u * kLoaders, row = i / CF::kChunks, c = i % CF::kChunks, rl = row % TILE;
-            if (i < kPieces)
-              *reinterpret_cast<uint4*>(q_tile + (row / TILE) * CF::kTileBytes + (c >> 3) * (TILE * 128) + rl * 128 +
-                                        (((c & 7) ^ (rl & 7)) << 4)) = w[u];
-          }
+          asm volatile("cp.async.commit_group;" ::: "memory");
+          cp_wait<0>();
+          fence_proxy_async_smem();
+          mbar_arrive(q_full);
         }
-        fence_proxy_async_smem();
-        mbar_arrive(q_full);
 
         const int nk = sg.k1 - sg.k0;
         if constexpr (kTma) {
