@@ -21,7 +21,7 @@ namespace {
 constexpr int kSelThreads = 1024;
 constexpr int kGatherThreads = 512;  // one element a thread at D = 256: 2 * 256 threads a slot
 constexpr int kSmemKeys = 48 * 1024;
-constexpr int kGatherUnroll = 4;
+constexpr int kGatherUnroll = 8;
 
 struct EvictArgs {
   PagedView pg;
@@ -53,7 +53,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 // A cluster of kCluster CTAs per (sequence, weight head); each takes a run of
-// the row and reads its keys once into shared memory (runs past kSmemKeys:
+// the row and reads it once into shared memory (runs past kSmemKeys:
 // re-read from L2 in every pass).  Threshold: three histogram passes of 11, 11
 // and 10 bits over the candidates; in each warp the lanes that share the first
 // lane's bin add once together, since many weights are alike (keys nothing
@@ -64,7 +64,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 template <int kCluster>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a, int smem_keys) {
   namespace cg = cooperative_groups;
-  extern __shared__ uint32_t keys_s[];
+  extern __shared__ float row_s[];
   __shared__ unsigned int hist[2048];
   __shared__ int scan_buf[kSelThreads / 32], warp_ties[kSelThreads / 32], warp_gt[kSelThreads / 32];
   __shared__ unsigned int s_prefix;
@@ -104,10 +104,11 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a, 
   const int d_lo = max(lo, r_lo), d_hi = min(hi, r_hi);
   const bool cached = cta_run <= smem_keys;
   if (cached) {
-#pragma unroll 4
-    for (int c = r_lo + t; c < r_hi; c += kSelThreads) keys_s[c - r_lo] = weight_key(w[c]);
+#pragma unroll 8
+    for (int c = r_lo + t; c < r_hi; c += kSelThreads) row_s[c - r_lo] = w[c];
   }
-  auto key_at = [&](int c) { return cached ? keys_s[c - r_lo] : weight_key(w[c]); };
+  auto weight_at = [&](int c) { return cached ? row_s[c - r_lo] : w[c]; };
+  auto key_at = [&](int c) { return weight_key(weight_at(c)); };
   // 1. threshold key of the `take` highest candidates, and how many of its
   //    ties are taken (from the lowest index)
   uint32_t pre = 0;
@@ -214,7 +215,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a, 
     if (keep) {
       const int slot = out + __popc(km & below);
       kept[slot] = c;
-      if (wout) wout[slot] = w[c];
+      if (wout) wout[slot] = weight_at(c);
     }
     out += __popc(km);
     seen += __popc(tie);
@@ -275,11 +276,11 @@ int launch_select(const EvictArgs& a, cudaStream_t s) {
   auto kern = evict_select_kernel<kCluster>;
   const long long per = ((long long)a.Lmax + kCluster * kSelThreads - 1) / (kCluster * kSelThreads) * kSelThreads;
   const int keys = (int)(per < kSmemKeys ? per : kSmemKeys);
-  if (allow_smem(kern, kSmemKeys * sizeof(uint32_t)) != KVBM_OK) return KVBM_ERR_CUDA;
+  if (allow_smem(kern, kSmemKeys * sizeof(float)) != KVBM_OK) return KVBM_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.B * a.Hw * kCluster));
   cfg.blockDim = dim3(kSelThreads);
-  cfg.dynamicSmemBytes = keys * sizeof(uint32_t);
+  cfg.dynamicSmemBytes = keys * sizeof(float);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
