@@ -58,7 +58,7 @@ struct Cfg {
   // which an MMA issued before the wait for entry i frees); more hide latency.
   static constexpr int kSlots = DP == 128 ? (kPair ? 4 : 5) : 6;
   static constexpr int kLag = 2;  // copies still in flight when a tile is handed over
-  static constexpr int kBars = 1 + 3 * kSlots + 4 + 1;
+  static constexpr int kBars = 1 + 3 * kSlots + 4;
   static constexpr size_t kRing = (size_t)kTileBytes * (kQTiles + kSlots);
   static constexpr size_t kSmem = 1024 + kRing + 2 * TILE * 16 + 16 * kAttCols * 4 + 8 * TILE * 4 + 8 * kBars + 64;
   static_assert(kSmem <= 227 * 1024, "one CTA's shared memory");
@@ -121,11 +121,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* q_full = reinterpret_cast<uint64_t*>(max_s + 8 * TILE);
   uint64_t *full = q_full + 1, *empty = full + CF::kSlots, *raw = empty + CF::kSlots, *s_full = raw + CF::kSlots;
   uint64_t* p_ready = s_full + 2;
-  uint64_t* seg_done = p_ready + 2;
-  long long* sched = reinterpret_cast<long long*>(seg_done + 1);  // total, first
+  long long* sched = reinterpret_cast<long long*>(p_ready + 2);  // total, first
   int* sched_b = reinterpret_cast<int*>(sched + 2);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sched_b + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  // [8], by segment: the loaders are at most the ring's tiles, so three segments, ahead of the softmax warps
   volatile int* bad_flag = abort_flag + 1;
 
   cudaTriggerProgrammaticLaunchCompletion();  // the joining kernel may be set up beside this one
@@ -139,8 +139,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       sched[1] = first;
       *sched_b = b;
       *abort_flag = 0;
-      *bad_flag = 0;
-      mbar_init(q_full, kTma ? kLoaders - 32 : kLoaders);
+      for (int i = 0; i < 8; ++i) bad_flag[i] = 0;
+      mbar_init(q_full, kSoftmax / 32);
       for (int i = 0; i < CF::kSlots; ++i) {
         mbar_init(&full[i], kTma ? 1 : kLoaders);
         mbar_init(&empty[i], 1);
@@ -150,7 +150,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&s_full[i], 1);
         mbar_init(&p_ready[i], 2 * TILE / 32);
       }
-      mbar_init(seg_done, kSoftmax);
       fence_mbar_init();
     }
   } else if (warp == kMmaWarp) {
@@ -274,30 +273,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (uint32_t seg = 0; ok && sg.next(a); ++seg) {
         const int b = sg.b, g = sg.g, len = sg.len, pre = len - a.T;
         const float* off = kBias ? a.off + b * a.ob + g * a.oh : nullptr;
-        // queries, by the scrub warps where warp 17 is free to start on the keys
-        constexpr int kFirst = kTma ? 32 : 0, kCount = kLoaders - kFirst;
-        if (lt >= kFirst) {
-          if (seg > 0) ok = mbar_wait(seg_done, (seg - 1) & 1u, abort_flag);  // the queries' tile and O are free
-          ok = !bar_any<kCount>(kLoaderBarrier, !ok);
-          if (!ok) break;
-          const uint32_t qa = smem_u32(q_tile);
-          const T* qbase = static_cast<const T*>(a.q);
-          for (int i = lt - kFirst; i < CF::kQTiles * TILE * CF::kChunks; i += kCount) {
-            const int row = i / CF::kChunks, c = i % CF::kChunks, rl = row % TILE;
-            const int r = sg.rt * CF::kQTiles * TILE + row;
-            const bool live = r < a.R && c * 8 < a.D;
-            cp16(qa + (row / TILE) * CF::kTileBytes + (c >> 3) * (TILE * 128) + rl * 128 + (((c & 7) ^ (rl & 7)) << 4),
-                 live ? qbase + b * a.qs[0] + (long long)(g * a.G + r / a.T) * a.qs[1] + (long long)(r % a.T) * a.qs[2] +
-                            c * 8
-                      : qbase,
-                 live);
-          }
-          asm volatile("cp.async.commit_group;" ::: "memory");
-          cp_wait<0>();
-          fence_proxy_async_smem();
-          mbar_arrive(q_full);
-        }
-
         const int nk = sg.k1 - sg.k0;
         if constexpr (kTma) {
           const int P = a.pg.page_size, rows = P < TILE ? P : TILE;
@@ -377,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   const bool bad =
                       scrub_pieces<kBf16>(tile, st, kLoaders - 32, TILE * CF::kChunks,
                                           [&](int e) { return c0 + ((e >> 3) & (TILE - 1)) < pre; });
-                  if (bad) *bad_flag = 1;
+                  if (bad) bad_flag[seg & 7] = 1;
                 }
                 fence_proxy_async_smem();
               }
@@ -416,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (j * TILE + r >= pre)
                   bad |= drop_nonfinite<kBf16>(reinterpret_cast<uint4*>(tile + (ch >> 3) * (TILE * 128) + r * 128 +
                                                                         (((ch & 7) ^ (r & 7)) << 4)));
-              if (bad) *bad_flag = 1;
+              if (bad) bad_flag[seg & 7] = 1;
             }
             fence_proxy_async_smem();
             mbar_arrive(&full[i % CF::kSlots]);
@@ -480,11 +455,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float C = kBias ? kLog2eF : a.scale * kLog2eF;
     uint32_t sn = 0;  // s_full phases used
     bool ok = true;
-    while (ok && sg.next(a)) {
+    for (uint32_t seg = 0; ok && sg.next(a); ++seg) {
       const int b = sg.b, g = sg.g, len = sg.len, pre = len - a.T, nk = sg.k1 - sg.k0;
       const int r = (sg.rt * CF::kQTiles + (kPair ? t : 0)) * TILE + rl;  // row of the unit
       const int tok = r % a.T, h = g * a.G + r / a.T;
       const float* off = kBias ? a.off + b * a.ob + g * a.oh : nullptr;
+      {
+        // the queries, by the 512 threads that have nothing else to do yet (their tile is free: every MMA of the
+        // segment before has completed).  A few loader threads took 12 us of a 180 us call for it.
+        const uint32_t qa = smem_u32(q_tile);
+        const T* qbase = static_cast<const T*>(a.q) + b * a.qs[0];
+        const int c = threadIdx.x % CF::kChunks;
+        for (int row = threadIdx.x / CF::kChunks; row < CF::kQTiles * TILE; row += kSoftmax / CF::kChunks) {
+          const int qr = sg.rt * CF::kQTiles * TILE + row, ql = row % TILE;
+          const bool live = qr < a.R && c * 8 < a.D;
+          cp16(qa + (row / TILE) * CF::kTileBytes + (c >> 3) * (TILE * 128) + ql * 128 + (((c & 7) ^ (ql & 7)) << 4),
+               live ? qbase + (long long)(g * a.G + qr / a.T) * a.qs[1] + (long long)(qr % a.T) * a.qs[2] + c * 8 : qbase,
+               live);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        cp_wait<0>();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+      }
       // drafted tokens this row keeps
       unsigned long long tree = 0;
       if (sg.k1 * TILE > pre && r < a.R) {
@@ -594,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         f1 = ex2((m1 - base) * C1);
         l = (ls[rl] + ls[TILE + rl]) * f0 + (ls[2 * TILE + rl] + ls[3 * TILE + rl]) * f1;
       }
-      const bool bad = *bad_flag != 0;
+      const bool bad = bad_flag[seg & 7] != 0;
       const float m_nat = kBias ? m : m * kLn2F;
       const bool none = l == 0.f;
       const float inv = none ? 0.f : 1.f / l;
@@ -660,8 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_before();
       bar_any<kSoftmax>(kSoftmaxBarrier, false);  // everyone has read the flag, the sums and O
-      if (threadIdx.x == 0) *bad_flag = 0;
-      mbar_arrive(seg_done);
+      if (threadIdx.x == 0) bad_flag[seg & 7] = 0;
     }
     tc_fence_before();
   }
