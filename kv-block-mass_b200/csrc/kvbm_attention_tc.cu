@@ -39,6 +39,7 @@
 #include <algorithm>
 
 #include "kvbm_attention.cuh"
+#include "kvbm_attention_items.cuh"
 #include "kvbm_attention_tile.cuh"
 
 namespace kvbm {
@@ -65,102 +66,6 @@ struct Cfg {
   static constexpr int kBars = 3 + 6 * kStages + 8 + 4 + 1;
   static constexpr size_t kSmem = 1024 + (size_t)kTileBytes * (2 + 2 * kStages) + 8 * kBars + 128 + 12 * TILE * 4;
 };
-
-// A work item: 256-row tile qt of sequence b, head h.
-struct Item {
-  int b, h, qt;
-};
-
-// Tiles in order of falling qt (under causal the longest first), heads
-// fastest: the heads of a group read the same keys at the same time.  With
-// lengths on the device the CTA finds its tile by counting: cnt(q) = tiles of
-// level >= q.  One warp.
-__device__ __forceinline__ int tiles_of(const PromptArgs& a, int b) {
-  return (seq_view(a.lens, a.cu, true, b, a.N, a.total).n + ROWS - 1) / ROWS;
-}
-
-__device__ __forceinline__ long long count_from(const PromptArgs& a, int q) {
-  long long n = 0;
-  for (int b = threadIdx.x & 31; b < a.B; b += 32) n += max(0, tiles_of(a, b) - q);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  return n;
-}
-
-__device__ __forceinline__ Item find_item(const PromptArgs& a, long long L) {
-  Item it;
-  const int nt = (a.N + ROWS - 1) / ROWS;
-  const long long i = L / a.Hq;
-  it.h = (int)(L % a.Hq);
-  if (a.lens == nullptr && a.cu == nullptr) {
-    it.qt = nt - 1 - (int)(i / a.B);
-    it.b = (int)(i % a.B);
-    return it;
-  }
-  int lo = 0, hi = nt;  // cnt(lo) > i >= cnt(hi)
-  long long chi = 0;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    const long long c = count_from(a, mid);
-    if (c > i)
-      lo = mid;
-    else {
-      hi = mid;
-      chi = c;
-    }
-  }
-  it.qt = lo;
-  long long left = i - chi;  // the left-th sequence with more than lo tiles
-  const int lane = threadIdx.x & 31;
-  it.b = 0;
-  for (int base = 0; base < a.B; base += 32) {
-    const int b = base + lane;
-    const bool in = b < a.B && tiles_of(a, b) > lo;
-    const unsigned m = __ballot_sync(0xffffffffu, in);
-    const int n = __popc(m);
-    if (left < n) {
-      const bool me = in && __popc(m & ((1u << lane) - 1u)) == (int)left;
-      it.b = base + __ffs(__ballot_sync(0xffffffffu, me)) - 1;
-      break;
-    }
-    left -= n;
-  }
-  return it;
-}
-
-// Rows of no sequence: out 0, lse -inf; thread `who` of `of`.
-__device__ void fill_rows(const PromptArgs& a, long long who, long long of) {
-  // gap g: the rows between what sequence g - 1 covers and where sequence g starts
-  const int gaps = a.cu != nullptr ? a.B + 1 : a.B;
-  for (int g = 0; g < gaps; ++g) {
-    long long r0, r1, bo = 0, bl = 0;
-    if (a.cu != nullptr) {
-      r0 = 0;
-      if (g > 0) {
-        const SeqView p = seq_view(nullptr, a.cu, true, g - 1, a.N, a.total);
-        r0 = (long long)p.q_row + p.n;
-      }
-      r1 = g < a.B ? seq_view(nullptr, a.cu, true, g, a.N, a.total).q_row : a.total;
-    } else {
-      r0 = seq_view(a.lens, nullptr, true, g, a.N, a.total).n;
-      r1 = a.N;
-      bo = g * a.os[0];
-      bl = g * a.ls[0];
-    }
-    const int vecs = a.D / 8;
-    const long long n = (r1 - r0) * a.Hq;
-    if (n <= 0) continue;
-    for (long long e = who; e < n * vecs; e += of) {
-      const int d = (int)(e % vecs);
-      const long long rh = e / vecs;
-      const int h = (int)(rh % a.Hq);
-      const long long r = r0 + rh / a.Hq;
-      uint16_t* out = static_cast<uint16_t*>(a.out) + bo + h * a.os[1] + r * a.os[2];
-      *reinterpret_cast<uint4*>(out + d * 8) = make_uint4(0u, 0u, 0u, 0u);
-      if (d == 0) a.lse[bl + h * a.ls[1] + r * a.ls[2]] = -INFINITY;
-    }
-  }
-}
 
 // What the roles need of an item.
 struct Work {
@@ -266,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kTmaWarp) {
       const int nt = (a.N + ROWS - 1) / ROWS;
       const long long total =
-          (a.lens == nullptr && a.cu == nullptr ? (long long)a.B * nt : count_from(a, 0)) * a.Hq;
+          (a.lens == nullptr && a.cu == nullptr ? (long long)a.B * nt : count_from<ROWS>(a, 0)) * a.Hq;
       if (lane == 0) {
         prefetch_tmap(&tq);
         prefetch_tmap(&tk);
@@ -287,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         Item it{0, 0, -1};
         SeqView sv{};
         if (L < total) {
-          it = find_item(a, L);
+          it = find_item<ROWS>(a, L);
           sv = seq_view(a.lens, a.cu, true, it.b, a.N, a.total);
         }
         if (k >= 2) ok = mbar_wait(&item_empty[k & 1], (k / 2 - 1) & 1, abort_flag);
@@ -346,78 +251,82 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     } else if (warp == kMmaWarp) {
+      // the whole warp, in uniform control flow (see elect_one)
       const uint32_t idesc_s = idesc_mma(TILE, TILE, kBf16 ? 1u : 0u);
       const uint32_t idesc_o = idesc_mma(TILE, DP, kBf16 ? 1u : 0u) | kTransposeB;
-      const uint32_t qs = smem_u32(q_tile), ks = smem_u32(k_ring), vs = smem_u32(v_ring);
+      const uint32_t qs = smem_u32(q_tile), ks = smem_u32(k_ring), vs = smem_u32(v_ring), tm = uniform(tmem);
       uint32_t kn = 0, vn = 0;                              // key tiles taken so far (K: the next to be scored)
       uint32_t qph = 0, pph = 0, fph = 0;                   // parities, one bit a barrier
-      uint32_t vfull = 0, vready = 0;
-      bool o_used[2] = {false, false};
+      uint32_t vfull = 0, vready = 0, o_used = 0;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0;
+      };
+      auto wait_bit = [&](uint64_t* bars, uint32_t& bits, int i) {
+        const bool r = wait(&bars[i], (bits >> i) & 1u);
+        bits ^= 1u << i;
+        return r;
+      };
+      auto issue_s = [&](int t, uint32_t tile) {
+        issue_scores<DP>(tm + t * TILE, qs + t * CF::kTileBytes, ks + (tile % kStages) * CF::kTileBytes, idesc_s);
+      };
       Work w;
       for (uint32_t k = 0; next_item(k, &w); ++k) {
-        bool ok = true;
-        if (lane == 0) {
-          auto wait_bit = [&](uint64_t* bars, uint32_t& bits, int i) {
-            const bool r = mbar_wait(&bars[i], (bits >> i) & 1u, abort_flag);
-            bits ^= 1u << i;
-            return r;
-          };
-          auto issue_s = [&](int t, uint32_t tile) {
-            issue_scores<DP>(tmem + t * TILE, qs + t * CF::kTileBytes, ks + (tile % kStages) * CF::kTileBytes, idesc_s);
-          };
-          const int cnt[2] = {w.nA, w.nB};
-          ok = mbar_wait(&k_full[kn % kStages], (kn / kStages) & 1, abort_flag);
-          for (int t = 0; ok && t < 2; ++t) {
-            if (cnt[t] == 0) continue;
-            ok = wait_bit(q_full, qph, t);
-            if (!ok) break;
-            tc_fence_after();
-            issue_s(t, kn);
-            mma_commit(&s_full[t]);
-          }
-          if (ok) {
-            mma_commit(&k_empty[kn % kStages]);
-            if (w.nk == 1) mma_commit(q_empty);
-          }
-          ++kn;
-          for (int j = 0; ok && j < w.nk; ++j, ++vn) {
-            const int s = vn % kStages;
-            ok = j < w.js ? wait_bit(v_full, vfull, s) : wait_bit(v_ready, vready, s);
-            if (ok && j + 1 < w.nk) ok = mbar_wait(&k_full[kn % kStages], (kn / kStages) & 1, abort_flag);
-            for (int t = 0; ok && t < 2; ++t) {
-              if (j >= cnt[t]) continue;
-              ok = wait_bit(p_ready, pph, t);
-              if (ok && j == 0 && o_used[t]) ok = wait_bit(o_free, fph, t);  // the last item's output has been read
-              if (!ok) break;
-              tc_fence_after();
-              issue_output<DP>(tmem + 256 + t * TILE, tmem + t * TILE, vs + s * CF::kTileBytes, idesc_o, j > 0);
-              if (j + 1 < cnt[t]) {
-                issue_s(t, kn);
-                mma_commit(&s_full[t]);
-              } else {
-                mma_commit(&o_full[t]);
-                o_used[t] = true;
-              }
-            }
-            if (!ok) break;
-            mma_commit(&v_empty[s]);
-            if (j + 1 < w.nk) {
-              mma_commit(&k_empty[kn % kStages]);
-              ++kn;
-              if (j + 2 == w.nk) mma_commit(q_empty);  // the item's last scores
-            }
-          }
-          if (!ok) *abort_flag = 1;
+        const int nA = uniform(w.nA), nB = uniform(w.nB), nk = max(nA, nB), js = uniform(w.js);
+        bool ok = wait(&k_full[kn % kStages], (kn / kStages) & 1);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (!ok || (t == 0 ? nA : nB) == 0) continue;
+          ok = wait_bit(q_full, qph, t);
+          if (!ok) continue;
+          tc_fence_after();
+          issue_s(t, kn);
+          commit_warp(&s_full[t]);
         }
-        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-        if (!ok) break;
+        if (ok) {
+          commit_warp(&k_empty[kn % kStages]);
+          if (nk == 1) commit_warp(q_empty);
+        }
+        ++kn;
+        for (int j = 0; ok && j < nk; ++j, ++vn) {
+          const int s = vn % kStages;
+          ok = j < js ? wait_bit(v_full, vfull, s) : wait_bit(v_ready, vready, s);
+          if (ok && j + 1 < nk) ok = wait(&k_full[kn % kStages], (kn / kStages) & 1);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int cnt = t == 0 ? nA : nB;
+            if (!ok || j >= cnt) continue;
+            ok = wait_bit(p_ready, pph, t);
+            if (ok && j == 0 && ((o_used >> t) & 1u)) ok = wait_bit(o_free, fph, t);  // the last item's output has been read
+            if (!ok) continue;
+            tc_fence_after();
+            issue_output<DP>(tm + 256 + t * TILE, tm + t * TILE, vs + s * CF::kTileBytes, idesc_o, j > 0 ? 1u : 0u);
+            if (j + 1 < cnt) {
+              issue_s(t, kn);
+              commit_warp(&s_full[t]);
+            } else {
+              commit_warp(&o_full[t]);
+              o_used |= 1u << t;
+            }
+          }
+          if (!ok) break;
+          commit_warp(&v_empty[s]);
+          if (j + 1 < nk) {
+            commit_warp(&k_empty[kn % kStages]);
+            ++kn;
+            if (j + 2 == nk) commit_warp(q_empty);  // the item's last scores
+          }
+        }
+        if (!ok) {
+          *abort_flag = 1;
+          break;
+        }
         if (lane == 0) mbar_arrive(&item_empty[k & 1]);
       }
       // TMEM and shared memory stay until every MMA has finished
-      if (lane == 0) {
-        mma_commit(drained);
-        mbar_wait(drained, 0, never);
-      }
+      __syncwarp();
+      commit_warp(drained);
+      mbar_wait(drained, 0, never);
+      __syncwarp();
     } else {
       const int st = threadIdx.x - (kTmaWarp + 1) * 32;
       if (a.fill && (a.lens != nullptr || a.cu != nullptr))
@@ -658,20 +567,6 @@ int launch_prompt_tc(const PromptArgs& a, int dtype, cudaStream_t s) {
   return bf16 ? launch<128, true>(a, sms, s) : launch<128, false>(a, sms, s);
 }
 
-int read_and_clear_attention_error(cudaStream_t s, int* err) {
-  unsigned int v = 0;
-  if (cudaMemcpyFromSymbolAsync(&v, g_kvbm_device_error, sizeof(v), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
-      cudaStreamSynchronize(s) != cudaSuccess)
-    return KVBM_ERR_CUDA;
-  *err = v != 0;
-  if (v != 0) {
-    const unsigned int zero = 0;
-    if (cudaMemcpyToSymbolAsync(g_kvbm_device_error, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s) !=
-            cudaSuccess ||
-        cudaStreamSynchronize(s) != cudaSuccess)
-      return KVBM_ERR_CUDA;
-  }
-  return KVBM_OK;
-}
+int read_and_clear_attention_error(cudaStream_t s, int* err) { return sm100::read_and_clear_wait_error(s, err); }
 
 }  // namespace kvbm

@@ -187,43 +187,44 @@ __device__ __forceinline__ bool scrub_pieces(uint8_t* tile, int first, int step,
   return bad;
 }
 
-// Descriptors of a tile's K steps differ from the tile's first one by a
-// constant in the low word (addresses stay below 2^18, so no carry leaves the
-// address field).  The tile's own low word is made opaque, or the compiler
-// keeps every step's descriptor of every ring slot alive across the loop and
-// spills them: 70 local loads a tile in the issuing thread (16k prompt: 2.19 ms
-// with them).
-__device__ __forceinline__ uint32_t opaque(uint32_t x) {
-  uint32_t y;
-  asm volatile("mov.u32 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
-__device__ __forceinline__ uint64_t step_desc(uint64_t base, uint32_t low, uint32_t bytes) {
-  return (base & 0xFFFFFFFF00000000ull) | (uint64_t)(low + (bytes >> 4));
-}
-
-// S = Q K^T of a 128 x 128 tile, both K-major with 128-byte swizzle.
+// S = Q K^T of a 128 x 128 tile, both K-major with 128-byte swizzle.  By a whole
+// warp in uniform control flow (elect_one): descriptors of later K steps are
+// the first one plus a constant (addresses stay below 2^18, so no carry leaves
+// the address field).
 template <int DP>
 __device__ __forceinline__ void issue_scores(uint32_t d_tmem, uint32_t q, uint32_t k, uint32_t idesc) {
-  const uint64_t base = sw128_desc(0);
-  const uint32_t ql = opaque((uint32_t)sw128_desc(q)), kl = opaque((uint32_t)sw128_desc(k));
+  const uint64_t qd = sw128_desc(q), kd = sw128_desc(k);
+  if (elect_one()) {
 #pragma unroll
-  for (int i = 0; i < DP / 64; ++i)
+    for (int i = 0; i < DP / 64; ++i)
 #pragma unroll
-    for (int k4 = 0; k4 < 4; ++k4)
-      mma_f16(d_tmem, step_desc(base, ql, i * kAttTile * 128 + k4 * 32), step_desc(base, kl, i * kAttTile * 128 + k4 * 32),
-              idesc, (i | k4) != 0);
+      for (int k4 = 0; k4 < 4; ++k4) {
+        const uint64_t step = (uint64_t)((i * kAttTile * 128 + k4 * 32) >> 4);
+        mma_f16(d_tmem, qd + step, kd + step, idesc, (i | k4) != 0);
+      }
+  }
+  __syncwarp();
 }
 
 // O (+)= P V: P (128 x 128, 16 bit) in TMEM, the weights of each 32 keys over
 // the first 16 columns of their own scores; V [128 keys][DP] MN-major.
 template <int DP>
-__device__ __forceinline__ void issue_output(uint32_t d_tmem, uint32_t p_tmem, uint32_t v, uint32_t idesc, bool add) {
-  const uint64_t base = sw128_mn_desc(0, kAttTile * 128);
-  const uint32_t vl = opaque((uint32_t)sw128_mn_desc(v, kAttTile * 128));
+__device__ __forceinline__ void issue_output(uint32_t d_tmem, uint32_t p_tmem, uint32_t v, uint32_t idesc, uint32_t add) {
+  const uint64_t vd = sw128_mn_desc(v, kAttTile * 128);
+  if (elect_one()) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k)  // 16 keys a step
-    mma_f16_ts(d_tmem, p_tmem + (k >> 1) * 32 + (k & 1) * 8, step_desc(base, vl, k * 2048), idesc, (add || k > 0) ? 1u : 0u);
+    for (int k = 0; k < 8; ++k)  // 16 keys a step
+      mma_f16_ts(d_tmem, p_tmem + (k >> 1) * 32 + (k & 1) * 8, vd + (uint64_t)((k * 2048) >> 4), idesc,
+                 k > 0 ? 1u : add);
+  }
+  __syncwarp();
+}
+
+// Arrive on `bar` when the MMAs issued so far by this warp complete.  (The same
+// lane is elected every time.)
+__device__ __forceinline__ void commit_warp(uint64_t* bar) {
+  if (elect_one()) mma_commit(bar);
+  __syncwarp();
 }
 
 }  // namespace sm100

@@ -60,7 +60,7 @@ struct Cfg {
   static constexpr int kLag = 2;  // copies still in flight when a tile is handed over
   static constexpr int kBars = 1 + 3 * kSlots + 4;
   static constexpr size_t kRing = (size_t)kTileBytes * (kQTiles + kSlots);
-  static constexpr size_t kSmem = 1024 + kRing + 2 * TILE * 16 + 16 * kAttCols * 4 + 8 * TILE * 4 + 8 * kBars + 64;
+  static constexpr size_t kSmem = 1024 + kRing + 2 * TILE * 16 + 16 * kAttCols * 4 + 8 * TILE * 4 + 8 * kBars + 80 + 8 * kMaxTreeTokens;
   static_assert(kSmem <= 227 * 1024, "one CTA's shared memory");
 };
 
@@ -71,6 +71,12 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
 template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// A whole 32-byte sector at once.
+__device__ __forceinline__ void st_global8(float* p, const float* v) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+               "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
 }
 template <int kId, int kCount>
 __device__ __forceinline__ void bar_sync() {
@@ -127,6 +133,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   // [8], by segment: the loaders are at most the ring's tiles, so three segments, ahead of the softmax warps
   volatile int* bad_flag = abort_flag + 1;
+  unsigned long long* tree_s = reinterpret_cast<unsigned long long*>(sched + 10);  // [64]: tokens each token keeps
+  volatile int* never = bad_flag + 8;  // stays 0: the last waits run to their own limit even after an abort
 
   cudaTriggerProgrammaticLaunchCompletion();  // the joining kernel may be set up beside this one
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -139,6 +147,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       sched[1] = first;
       *sched_b = b;
       *abort_flag = 0;
+      *never = 0;
       for (int i = 0; i < 8; ++i) bad_flag[i] = 0;
       mbar_init(q_full, kSoftmax / 32);
       for (int i = 0; i < CF::kSlots; ++i) {
@@ -171,91 +180,101 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp >= kMmaWarp) {
     reg_dec<kRegsRest>();
     if (warp == kMmaWarp) {
-      if (lane == 0) {
-        const uint32_t idesc_s = idesc_mma(TILE, TILE, kBf16 ? 1u : 0u);
-        const uint32_t idesc_o = idesc_mma(TILE, DP, kBf16 ? 1u : 0u) | kTransposeB;
-        const uint32_t qa = smem_u32(q_tile), ra = smem_u32(ring);
-        long long idx = 0;             // ring index of this segment's k0
-        uint32_t pn[2] = {0, 0};       // p_ready phases used
-        uint32_t sn[2] = {0, 0};       // s_full commits made
-        bool ok = true;
-        for (uint32_t seg = 0; ok && sg.next(a); ++seg) {
-          const int nk = sg.k1 - sg.k0;
-          auto slot_of = [&](long long i) { return (int)(i % CF::kSlots); };
-          auto wait_full = [&](long long i) {
-            return mbar_wait(&full[slot_of(i)], (uint32_t)(i / CF::kSlots) & 1u, abort_flag);
-          };
-          auto issue_s = [&](int t, int j) {
-            issue_scores<DP>(tmem + t * TILE, qa + (kPair ? t : 0) * CF::kTileBytes,
-                             ra + slot_of(idx + 2 * j) * CF::kTileBytes, idesc_s);
-          };
-          auto commit_s = [&](int t) {
-            mma_commit(&s_full[t]);
-            ++sn[t];
-          };
-          ok = mbar_wait(q_full, seg & 1u, abort_flag);
-          if constexpr (kPair) {
-            ok = ok && wait_full(idx);
-            if (ok) {
-              tc_fence_after();
-              fence_proxy_async_smem();
-              for (int t = 0; t < 2; ++t) {
-                issue_s(t, 0);
-                commit_s(t);
-              }
-              mma_commit(&empty[slot_of(idx)]);
-            }
-            for (int j = 0; ok && j < nk; ++j) {
-              ok = wait_full(idx + 2 * j + 1);
-              if (ok && j + 1 < nk) ok = wait_full(idx + 2 * j + 2);
-              for (int t = 0; ok && t < 2; ++t) {
-                ok = mbar_wait(&p_ready[t], pn[t]++ & 1u, abort_flag);
-                if (!ok) break;
-                tc_fence_after();
-                issue_output<DP>(tmem + 256 + t * TILE, tmem + t * TILE,
-                                 ra + slot_of(idx + 2 * j + 1) * CF::kTileBytes, idesc_o, j > 0);
-                if (j + 1 < nk) issue_s(t, j + 1);
-                commit_s(t);  // the next S, or the finished O
-              }
-              if (!ok) break;
-              mma_commit(&empty[slot_of(idx + 2 * j + 1)]);
-              if (j + 1 < nk) mma_commit(&empty[slot_of(idx + 2 * j + 2)]);
-            }
-          } else {
-            for (int t = 0; ok && t < 2 && t < nk; ++t) {
-              ok = wait_full(idx + 2 * t);
-              if (!ok) break;
-              tc_fence_after();
-              issue_s(t, t);
+      // the whole warp, in uniform control flow (see elect_one)
+      const uint32_t idesc_s = idesc_mma(TILE, TILE, kBf16 ? 1u : 0u);
+      const uint32_t idesc_o = idesc_mma(TILE, DP, kBf16 ? 1u : 0u) | kTransposeB;
+      const uint32_t qa = smem_u32(q_tile), ra = smem_u32(ring), tm = uniform(tmem);
+      uint32_t idx = 0;     // ring index of this segment's k0
+      uint32_t pph = 0;     // p_ready parities
+      uint32_t used = 0;    // commits on s_full[t] so far: bit t, and their parity
+      uint32_t sph = 0;
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0;
+      };
+      auto wait_full = [&](uint32_t i) { return wait(&full[i % CF::kSlots], (i / CF::kSlots) & 1u); };
+      auto wait_p = [&](int t) {
+        const bool r = wait(&p_ready[t], (pph >> t) & 1u);
+        pph ^= 1u << t;
+        return r;
+      };
+      auto commit_s = [&](int t) {
+        commit_warp(&s_full[t]);
+        used |= 1u << t;
+        sph ^= 1u << t;
+      };
+      for (uint32_t seg = 0; ok && sg.next(a); ++seg) {
+        const int nk = uniform(sg.k1 - sg.k0);
+        auto slot_at = [&](uint32_t i) { return ra + (i % CF::kSlots) * CF::kTileBytes; };
+        auto issue_s = [&](int t, int j) {
+          issue_scores<DP>(tm + t * TILE, qa + (kPair ? t : 0) * CF::kTileBytes, slot_at(idx + 2 * j), idesc_s);
+        };
+        ok = wait(q_full, seg & 1u);
+        if constexpr (kPair) {
+          ok = ok && wait_full(idx);
+          if (ok) {
+            tc_fence_after();
+            fence_proxy_async_smem();
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              issue_s(t, 0);
               commit_s(t);
-              mma_commit(&empty[slot_of(idx + 2 * t)]);
             }
-            for (int j = 0; ok && j < nk; ++j) {
-              const int t = j & 1;
-              ok = wait_full(idx + 2 * j + 1) && mbar_wait(&p_ready[t], pn[t]++ & 1u, abort_flag);
+            commit_warp(&empty[idx % CF::kSlots]);
+          }
+          for (int j = 0; ok && j < nk; ++j) {
+            ok = wait_full(idx + 2 * j + 1);
+            if (ok && j + 1 < nk) ok = wait_full(idx + 2 * j + 2);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              ok = ok && wait_p(t);
+              if (!ok) continue;
+              tc_fence_after();
+              issue_output<DP>(tm + 256 + t * TILE, tm + t * TILE, slot_at(idx + 2 * j + 1), idesc_o, j > 0 ? 1u : 0u);
+              if (j + 1 < nk) issue_s(t, j + 1);
+              commit_s(t);  // the next S, or the finished O
+            }
+            if (!ok) break;
+            commit_warp(&empty[(idx + 2 * j + 1) % CF::kSlots]);
+            if (j + 1 < nk) commit_warp(&empty[(idx + 2 * j + 2) % CF::kSlots]);
+          }
+        } else {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (!ok || t >= nk) continue;
+            ok = wait_full(idx + 2 * t);
+            if (!ok) continue;
+            tc_fence_after();
+            issue_s(t, t);
+            commit_s(t);
+            commit_warp(&empty[(idx + 2 * t) % CF::kSlots]);
+          }
+          for (int j = 0; ok && j < nk; ++j) {
+            const int t = j & 1;
+            ok = wait_full(idx + 2 * j + 1) && wait_p(t);
+            if (!ok) break;
+            tc_fence_after();
+            issue_output<DP>(tm + 256 + t * TILE, tm + t * TILE, slot_at(idx + 2 * j + 1), idesc_o, j > 1 ? 1u : 0u);
+            commit_warp(&empty[(idx + 2 * j + 1) % CF::kSlots]);
+            if (j + 2 < nk) {
+              ok = wait_full(idx + 2 * j + 4);
               if (!ok) break;
               tc_fence_after();
-              issue_output<DP>(tmem + 256 + t * TILE, tmem + t * TILE,
-                               ra + slot_of(idx + 2 * j + 1) * CF::kTileBytes, idesc_o, j > 1);
-              mma_commit(&empty[slot_of(idx + 2 * j + 1)]);
-              if (j + 2 < nk) {
-                ok = wait_full(idx + 2 * j + 4);
-                if (!ok) break;
-                tc_fence_after();
-                issue_s(t, j + 2);
-                commit_s(t);
-                mma_commit(&empty[slot_of(idx + 2 * j + 4)]);
-              } else {
-                commit_s(t);  // the finished O
-              }
+              issue_s(t, j + 2);
+              commit_s(t);
+              commit_warp(&empty[(idx + 2 * j + 4) % CF::kSlots]);
+            } else {
+              commit_s(t);  // the finished O
             }
           }
-          idx += 2 * (long long)nk;
         }
-        // TMEM and shared memory stay until every MMA has finished
-        for (int t = 0; t < 2; ++t)
-          if (sn[t] > 0) mbar_wait(&s_full[t], (sn[t] - 1) & 1u, abort_flag);
+        idx += 2 * (uint32_t)nk;
       }
+      // TMEM and shared memory stay until every MMA has finished
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if ((used >> t) & 1u) mbar_wait(&s_full[t], ((sph >> t) & 1u) ^ 1u, never);
+      __syncwarp();
     } else {
       // ---- loaders
       const int lt = threadIdx.x - (kMmaWarp + 1) * 32;
@@ -263,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const T *kbase = static_cast<const T*>(a.k), *vbase = static_cast<const T*>(a.v);
       const int ch = lt % CF::kChunks;
       const bool in = ch * 8 < a.D;
-      long long idx = 0;
+      uint32_t idx = 0;  // ring index of this segment's first tile (two a key tile: below 2^32 for any call)
       uint32_t raw_phase = 0;  // per slot (kTma)
       bool ok = true;
       if (kTma && lt == 0) {
@@ -301,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const int slot_c = ((sg.k0 + j) * TILE + (lane / kBlk) * rows) % P;
 #pragma unroll 1
               for (int kv = 0; kv < 2; ++kv) {
-                const long long i = idx + 2 * j + kv;
+                const uint32_t i = idx + 2 * j + kv;
                 const int slot = (int)(i % CF::kSlots);
                 if (i >= CF::kSlots) ok = mbar_wait(&empty[slot], (uint32_t)(i / CF::kSlots - 1) & 1u, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
@@ -328,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
             const int st = lt - 32;
             for (int j = js; j < nk; ++j) {
-              const long long i = idx + 2 * j + 1;
+              const uint32_t i = idx + 2 * j + 1;
               const int slot = (int)(i % CF::kSlots);
               ok = mbar_wait(&raw[slot], (raw_phase >> slot) & 1u, abort_flag) && ok;
               raw_phase ^= 1u << slot;
@@ -379,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             return o;
           };
           // hand over ring entry i (its copies have landed for this thread)
-          auto hand_over = [&](long long i) {
+          auto hand_over = [&](uint32_t i) {
             const int j = sg.k0 + (int)((i - idx) >> 1);
             if (((i - idx) & 1) && (j + 1) * TILE > pre) {
               // v of drafted tokens: rows keep different ones; this thread's
@@ -410,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
 #pragma unroll 1
             for (int kv = 0; kv < 2; ++kv) {
-              const long long i = idx + 2 * j + kv;
+              const uint32_t i = idx + 2 * j + kv;
               const int slot = (int)(i % CF::kSlots);
               if (i >= CF::kSlots)
                 ok = mbar_wait(&empty[slot], (uint32_t)(i / CF::kSlots - 1) & 1u, abort_flag) && ok;
@@ -439,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           cp_wait<0>();
           hand_over(idx + 2 * nk - 1);
         }
-        idx += 2 * (long long)nk;
+        idx += 2 * (uint32_t)nk;
       }
       cp_wait<0>();
     }
@@ -481,11 +500,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // drafted tokens this row keeps
       unsigned long long tree = 0;
-      if (sg.k1 * TILE > pre && r < a.R) {
+      if (sg.k1 * TILE > pre) {
         if (a.tree != nullptr) {
-          const uint8_t* tm = a.tree + b * a.tb + tok * a.tr;
-#pragma unroll 8
-          for (int u = 0; u < a.T; ++u) tree |= (unsigned long long)(tm[u] != 0) << u;
+          // a warp reads whole mask rows and packs them (a thread reading its own row byte by byte: 9 us)
+          const uint8_t* tm = a.tree + b * a.tb;
+          for (int x = warp; x < a.T; x += kMmaWarp) {
+            const bool b0 = lane < a.T && tm[x * a.tr + lane] != 0, b1 = lane + 32 < a.T && tm[x * a.tr + lane + 32] != 0;
+            const uint32_t w0 = __ballot_sync(0xffffffffu, b0), w1 = __ballot_sync(0xffffffffu, b1);
+            if (lane == 0) tree_s[x] = (unsigned long long)w1 << 32 | w0;
+          }
+          bar_any<kSoftmax>(kSoftmaxBarrier, false);
+          tree = tree_s[tok];
         } else {
           tree = ~0ull >> (63 - tok);
         }
@@ -639,9 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           } else {
 #pragma unroll
-            for (int e = 0; e < kStep; e += 4)
-              *reinterpret_cast<float4*>(a.part_o + pr * a.DP + d0 + e) =
-                  make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            for (int e = 0; e < kStep; e += 8) st_global8(a.part_o + pr * a.DP + d0 + e, o + e);
           }
         }
         __syncwarp();  // the next load is the whole warp's
@@ -713,20 +736,6 @@ int launch_cached_tc(const CachedArgs& a, int dtype, cudaStream_t s) {
   return bf16 ? launch_d<128, true>(a, s) : launch_d<128, false>(a, s);
 }
 
-int read_and_clear_cached_error(cudaStream_t s, int* err) {
-  unsigned int v = 0;
-  if (cudaMemcpyFromSymbolAsync(&v, g_kvbm_device_error, sizeof(v), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
-      cudaStreamSynchronize(s) != cudaSuccess)
-    return KVBM_ERR_CUDA;
-  *err = v != 0;
-  if (v != 0) {
-    const unsigned int zero = 0;
-    if (cudaMemcpyToSymbolAsync(g_kvbm_device_error, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s) !=
-            cudaSuccess ||
-        cudaStreamSynchronize(s) != cudaSuccess)
-      return KVBM_ERR_CUDA;
-  }
-  return KVBM_OK;
-}
+int read_and_clear_cached_error(cudaStream_t s, int* err) { return sm100::read_and_clear_wait_error(s, err); }
 
 }  // namespace kvbm

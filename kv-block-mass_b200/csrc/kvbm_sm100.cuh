@@ -5,7 +5,10 @@
 #pragma once
 
 #include <cuda.h>
+#include <cuda_runtime.h>
 #include <stdint.h>
+
+#include "kvbm.h"
 
 namespace kvbm {
 namespace sm100 {
@@ -17,6 +20,23 @@ static __device__ unsigned int g_kvbm_device_error = 0;
 
 // A wait on an mbarrier gives up after this many nanoseconds of %globaltimer.
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s
+
+// Reads and clears this source file's copy of the error word (synchronises `s`).
+static inline int read_and_clear_wait_error(cudaStream_t s, int* err) {
+  unsigned int v = 0;
+  if (cudaMemcpyFromSymbolAsync(&v, g_kvbm_device_error, sizeof(v), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
+      cudaStreamSynchronize(s) != cudaSuccess)
+    return KVBM_ERR_CUDA;
+  *err = v != 0;
+  if (v != 0) {
+    const unsigned int zero = 0;
+    if (cudaMemcpyToSymbolAsync(g_kvbm_device_error, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s) !=
+            cudaSuccess ||
+        cudaStreamSynchronize(s) != cudaSuccess)
+      return KVBM_ERR_CUDA;
+  }
+  return KVBM_OK;
+}
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -354,6 +374,22 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// One lane of a converged warp.  MMAs are issued by a whole warp in uniform
+// control flow with this predicate: their descriptors then stay in uniform
+// registers, where a single-lane branch moves each of them there first.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+// A warp-uniform value, known as such to the compiler.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 // ---- packed fp32 pairs (sm_100 f32x2 instructions) ----
 __device__ __forceinline__ unsigned long long pk(float2 v) { return *reinterpret_cast<unsigned long long*>(&v); }

@@ -1782,21 +1782,6 @@ int launch_tc(const kvbm_problem* p, const WsLayout& L, void* mass_out, void* ws
   return KVBM_ERR_HEAD_DIM;
 }
 
-int read_and_clear_device_error(cudaStream_t s, int* err) {
-  unsigned int v = 0;
-  if (cudaMemcpyFromSymbolAsync(&v, sm100::g_kvbm_device_error, sizeof(v), 0, cudaMemcpyDeviceToHost, s) !=
-          cudaSuccess ||
-      cudaStreamSynchronize(s) != cudaSuccess)
-    return KVBM_ERR_CUDA;
-  *err = v != 0;
-  if (v != 0) {
-    const unsigned int zero = 0;
-    if (cudaMemcpyToSymbolAsync(sm100::g_kvbm_device_error, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s) !=
-            cudaSuccess ||
-        cudaStreamSynchronize(s) != cudaSuccess)
-      return KVBM_ERR_CUDA;
-  }
-  return KVBM_OK;
-}
+int read_and_clear_device_error(cudaStream_t s, int* err) { return sm100::read_and_clear_wait_error(s, err); }
 
 }  // namespace kvbm

@@ -45,7 +45,8 @@ def _check_dense(q, k, v, out, lse, causal, lens=None, mask=None, scale=None, ou
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("N,D,Hq,Hkv", [(1, 64, 2, 1), (2, 128, 4, 2), (63, 64, 3, 3), (64, 128, 2, 1), (65, 64, 8, 2),
                                         (127, 96, 2, 2), (128, 128, 4, 1), (129, 64, 2, 1), (255, 8, 1, 1),
-                                        (257, 128, 4, 1), (383, 72, 2, 1), (640, 128, 2, 1), (1025, 64, 2, 2)])
+                                        (257, 128, 4, 1), (383, 72, 2, 1), (640, 128, 2, 1), (1025, 64, 2, 2),
+                                        (513, 128, 2, 1), (1024, 96, 2, 1), (1537, 128, 3, 1)])
 def test_dense(cuda_device, dtype, causal, N, D, Hq, Hkv):
     q, k, v = _inputs(2, Hq, Hkv, N, D, dtype, N * 7 + D, cuda_device)
     out, lse = kb.attention_b200(q, k, v, causal=causal)
@@ -63,12 +64,13 @@ def test_head_dims(cuda_device, dtype, D):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("causal", [False, True])
-def test_lengths_and_masks(cuda_device, dtype, causal):
+@pytest.mark.parametrize("N,D,lens", [(390, 64, [390, 0, 1, 129, 256]), (1300, 128, [1300, 513, 700, 129, 512]),
+                                      (1101, 104, [1, 1101, 640, 0, 1024])])
+def test_lengths_and_masks(cuda_device, dtype, causal, N, D, lens):
     """Ragged lengths (0 and 1 among them), a key mask that drops the first keys (causal rows left empty), whole
     tiles and single keys; NaN and infinities wherever nothing may be read."""
-    B, N, D = 5, 390, 64
+    B = 5
     q, k, v = _inputs(B, 4, 2, N, D, dtype, 5, cuda_device)
-    lens = [390, 0, 1, 129, 256]
     g = torch.Generator().manual_seed(3)
     mask = (torch.rand(B, 1, N, generator=g) > 0.2).to(cuda_device)
     mask[0, 0, :3] = False      # causal: rows 0..2 keep nothing
@@ -90,14 +92,16 @@ def test_lengths_and_masks(cuda_device, dtype, causal):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("at", [0, 5, 127, 128, 200, 299])
-def test_nan_behind_the_diagonal(cuda_device, dtype, at):
+@pytest.mark.parametrize("N,D,at", [(300, 64, 0), (300, 64, 5), (300, 64, 127), (300, 64, 128), (300, 64, 200),
+                                    (300, 64, 299), (1100, 128, 0), (1100, 128, 200), (1100, 128, 511),
+                                    (1100, 128, 512), (1100, 96, 700), (1100, 128, 1099)])
+def test_nan_behind_the_diagonal(cuda_device, dtype, N, D, at):
     """A NaN or an infinity in v (or k) of position j reaches the rows from j on, and none before."""
-    N = 300
-    q, k, v = _inputs(1, 2, 1, N, 64, dtype, 9, cuda_device)
+    q, k, v = _inputs(1, 2, 1, N, D, dtype, 9, cuda_device)
     v[0, 0, at, 3] = math.nan
     v[0, 0, at, 9] = math.inf
     v[0, 0, at, 17] = -math.inf
+    v[0, 0, at, D - 1] = math.nan
     out, lse = kb.attention_b200(q, k, v, causal=True)
     _check_dense(q, k, v, out, lse, True)
     assert bool(torch.isfinite(out[:, :, :at]).all())
@@ -111,9 +115,10 @@ def test_nan_behind_the_diagonal(cuda_device, dtype, at):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("causal", [False, True])
-@pytest.mark.parametrize("lens", [[1], [5, 0, 130, 1, 64], [0, 0, 257], [300, 128, 2]])
-def test_packed(cuda_device, dtype, causal, lens):
-    Hq, Hkv, D, lead, tail = 4, 2, 64, 3, 5
+@pytest.mark.parametrize("lens,D", [([1], 64), ([5, 0, 130, 1, 64], 64), ([0, 0, 257], 64), ([300, 128, 2], 64),
+                                    ([600, 0, 1, 1000, 513, 64], 128), ([1025], 120), ([3, 2049, 512], 128)])
+def test_packed(cuda_device, dtype, causal, lens, D):
+    Hq, Hkv, lead, tail = 4, 2, 3, 5
     T = lead + sum(lens) + tail
     q, k, v = (t[0].transpose(0, 1).contiguous() for t in _inputs(1, Hq, Hkv, T, D, dtype, 11, cuda_device))
     q, k, v = q[:, :Hq], k[:, :Hkv], v[:, :Hkv]
@@ -197,8 +202,9 @@ def test_long_rows_sampled(cuda_device, dtype):
             check(lse[0, h, r:r + 1], l, lt, f"lse {r}")
 
 
-def test_deterministic_streams_and_graph(cuda_device):
-    q, k, v = _inputs(2, 8, 2, 700, 128, torch.bfloat16, 41, cuda_device)
+@pytest.mark.parametrize("N,D,Hq", [(300, 64, 8), (700, 128, 8), (2300, 128, 40)])
+def test_deterministic_streams_and_graph(cuda_device, N, D, Hq):
+    q, k, v = _inputs(2, Hq, 2, N, D, torch.bfloat16, 41, cuda_device)
     out, lse = kb.attention_b200(q, k, v, causal=True)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
