@@ -20,6 +20,8 @@ constexpr int kMaxTreeTokens = 64;
 
 // Keys of one tile of the cache kernels.
 constexpr int kCachedKeyTile = 64;
+// CTAs an SM of the mma.sync cache kernel (D <= 128).
+constexpr int kMmaCtas = 3;
 
 // Prompt attention as the kernels see it (strides in elements, dims [B, H, N, D]).
 struct PromptArgs {

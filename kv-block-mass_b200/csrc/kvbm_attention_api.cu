@@ -155,7 +155,8 @@ void plan_cached(const kvbm_cached_args* p, int sms, CachedPlan* pl) {
   a.RT = (a.R + a.BM - 1) / a.BM;
   // no more CTAs than key tiles of full-length sequences
   const long long tiles = (long long)a.B * a.Hkv * a.RT * ((a.Lmax + a.KT - 1) / a.KT);
-  a.C = (int)std::min<long long>(tiles, (long long)sms * (pl->kernel == 2 ? 1 : 2));
+  const int per_sm = pl->kernel == 2 ? 1 : pl->kernel == 1 && a.DP <= 128 ? kMmaCtas : 2;
+  a.C = (int)std::min<long long>(tiles, (long long)sms * per_sm);
   size_t o = 0;
   auto take = [&](size_t bytes) {
     const size_t at = o;

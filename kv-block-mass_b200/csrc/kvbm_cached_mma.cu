@@ -1,8 +1,11 @@
 // Attention of a few rows per kv head over a paged cache (R = G * T <= 16:
 // single tokens, small trees), bf16 / fp16, split over the keys.
 //
-// Bound by reading k and v once.  Every SM gets the same number of 64-key
-// tiles (kvbm_attention.cu describes the split and the joining).  A CTA of
+// Bound by reading k and v once.  Every CTA gets the same number of 64-key
+// tiles (kvbm_attention.cu describes the split and the joining); three CTAs an
+// SM with two tiles each in flight (32 sequences of 4-8k keys: 155 us, 5.3 TB/s)
+// hide a tile's chain of products and shuffles better than two CTAs with three
+// (174 us).  A CTA of
 // four warps keeps kStages tiles of k and v in flight with 16-byte cp.async
 // (page lookups one tile ahead), rows swizzled so that ldmatrix meets no bank
 // conflict; warp w takes keys 16 w .. 16 w + 15 of each tile with
@@ -94,7 +97,7 @@ template <int DP>
 struct Cfg {
   static constexpr int kChunks = DP / 8;              // 16-byte chunks of a row
   static constexpr int kTileBytes = KT * DP * 2;      // k or v of one tile
-  static constexpr int kStages = DP == 64 ? 6 : 3;
+  static constexpr int kStages = DP == 64 ? 4 : DP == 128 ? 2 : 3;
   static constexpr int kRowsPerPass = kThreads / kChunks;
   static constexpr int kPasses = KT / kRowsPerPass;
   static constexpr int kPitch = DP + 4;               // floats of a row of the joining buffer
@@ -104,7 +107,7 @@ struct Cfg {
 };
 
 template <int DP, bool kBf16>
-__global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) cached_mma_kernel(const __grid_constant__ CachedArgs a) {
+__global__ void __launch_bounds__(kThreads, DP <= 128 ? kMmaCtas : 1) cached_mma_kernel(const __grid_constant__ CachedArgs a) {
   using CF = Cfg<DP>;
   using T = std::conditional_t<kBf16, __nv_bfloat16, __half>;
   extern __shared__ __align__(128) uint8_t smem[];

@@ -74,10 +74,13 @@ def _same(name: str, t: torch.Tensor, like: torch.Tensor) -> None:
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
     """First and one-past-last byte a strided tensor can touch."""
+    p = t.data_ptr()
+    if t.is_contiguous():
+        return (p, p + t.nbytes)
     if t.numel() == 0:
         return (0, 0)
     last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return (t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size())
+    return (p, p + (last + 1) * t.element_size())
 
 
 def _no_overlap(name: str, t: torch.Tensor, others: dict) -> None:
@@ -91,7 +94,7 @@ def _no_overlap(name: str, t: torch.Tensor, others: dict) -> None:
 def _check_out(name: str, t: torch.Tensor, shape, dtype, device) -> None:
     if not isinstance(t, torch.Tensor) or tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device:
         raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on {device}")
-    if any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
+    if not t.is_contiguous() and any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
         raise ValueError(f"{name} has expanded (stride 0) dimensions")
 
 
@@ -258,6 +261,10 @@ def _per_key(name, t, B, Hkv, L, dev, writable=False):
     """A float32 [B|1, Hkv|1, L] per-key array with unit stride: (tensor, batch stride, head stride)."""
     if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != dev:
         raise ValueError(f"{name} must be a float32 tensor on {dev}")
+    if t.shape == (B, Hkv, L):  # the usual case
+        st = t.stride()
+        if st[2] == 1 and (B == 1 or st[0] > 0) and (Hkv == 1 or st[1] > 0):
+            return t, st[0], st[1]
     if t.dim() == 2:
         t = t.unsqueeze(1)
     ok = t.dim() == 3 and t.shape[2] == L
@@ -329,17 +336,22 @@ def _cached_args(q, k_cache, v_cache, block_table, seq_lens, tree_mask, log_offs
             weights_out = weights
         wo, a.weights_out_bstride, a.weights_out_hstride = _per_key("weights_out", weights_out, B, Hkv, L, q.device, True)
         _check_out("weights_out", wo, wo.shape, wo.dtype, wo.device)
-        w, a.weights_bstride, a.weights_hstride = _per_key("weights", weights, B, Hkv, L, q.device)
-        if w.shape[:2] != (B, Hkv):
-            raise ValueError(f"weights must be [{B}, {Hkv}, {L}], got {tuple(w.shape)}")
-        a.weights, a.weights_out = w.data_ptr(), wo.data_ptr()
-        if a.weights != a.weights_out or w.stride() != wo.stride():
-            _no_overlap("weights_out", wo, {"weights": w})
         ins = {"q": q, "k_cache": k_cache, "v_cache": v_cache}
         if log_offsets is not None:
             ins["log_offsets"] = t
+        if weights is weights_out:
+            a.weights, a.weights_bstride, a.weights_hstride = wo.data_ptr(), a.weights_out_bstride, a.weights_out_hstride
+        else:
+            w, a.weights_bstride, a.weights_hstride = _per_key("weights", weights, B, Hkv, L, q.device)
+            if w.shape[:2] != (B, Hkv):
+                raise ValueError(f"weights must be [{B}, {Hkv}, {L}], got {tuple(w.shape)}")
+            a.weights = w.data_ptr()
+            if a.weights != wo.data_ptr() or w.stride() != wo.stride():
+                ins["weights"] = w
+            keep.append(w)
+        a.weights_out = wo.data_ptr()
         _no_overlap("weights_out", wo, ins)
-        keep += [w, wo]
+        keep.append(wo)
     a.scale = float(1.0 / D ** 0.5 if scale is None else scale)
     if out is not None or lse_out is not None:
         ins = {"q": q, "k_cache": k_cache, "v_cache": v_cache}
