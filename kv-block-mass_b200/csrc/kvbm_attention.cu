@@ -13,7 +13,10 @@
 // Tiles: 16 x 16 threads own RPT x 4 scores each (RPT = 4: 64 rows, for
 // prompts and wide trees; RPT = 1: 16 rows, for single tokens), 64 keys a
 // tile, everything in fp32 registers and shared memory.  Bound by the FFMA
-// pipe (4 shared float4 reads feed 16 FFMAs per thread).
+// pipe (4 shared float4 reads feed 16 FFMAs per thread).  fp32 rows in 16-byte
+// pieces and D <= 128 (kAsync): k and v are double-buffered with cp.async, so that
+// a tile's products hide the next one's loads (2048-token causal prompt, 8 heads
+// of 64: 306 us without).
 #include <atomic>
 
 #include "kvbm_attention.cuh"
@@ -37,7 +40,9 @@ struct Tile {
   static constexpr int BM = 16 * RPT;
   static constexpr int kStride = DP + kPad;
   static constexpr int kPs = BN + kPad;
-  static constexpr size_t kBytes = sizeof(float) * ((size_t)(BM + 2 * BN) * kStride + (size_t)BM * kPs + BN);
+  static constexpr size_t bytes(int buffers) {
+    return sizeof(float) * ((size_t)(BM + 2 * BN * buffers) * kStride + (size_t)BM * kPs + BN * buffers);
+  }
   float o[RPT][DP / 16];
   float m[RPT], l[RPT];
 
@@ -74,20 +79,42 @@ __device__ __forceinline__ float4 load4(const T* row, int d, int D, long long ds
   return r;
 }
 
-// The tiles of shared memory: Q [BM], K [BN], V [BN] (fp32, rows of DP + 4),
-// P [BM][BN + 4], bias [BN].
+// The tiles of shared memory: Q [BM], P [BM][BN + 4], then for each buffer
+// K [BN], V [BN] (fp32, rows of DP + 4), bias [BN].
 template <int RPT, int DP>
 struct Smem {
   using TL = Tile<RPT, DP>;
   float *q, *k, *v, *p, *bias;
-  __device__ explicit Smem(float* base) {
+  __device__ explicit Smem(float* base, int buffer = 0) {
     q = base;
-    k = q + TL::BM * TL::kStride;
+    p = q + TL::BM * TL::kStride;
+    k = p + TL::BM * TL::kPs + buffer * (2 * BN * TL::kStride + BN);
     v = k + BN * TL::kStride;
-    p = v + BN * TL::kStride;
-    bias = p + TL::BM * TL::kPs;
+    bias = v + BN * TL::kStride;
   }
 };
+
+// load_rows by cp.async (fp32 rows in 16-byte pieces); `any`: a readable address.
+template <int DP, class F>
+__device__ __forceinline__ void copy_rows(float* dst, int rows, F&& f, int D, const float* any) {
+  constexpr int kVecs = DP / 4;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < rows * kVecs; i += kThreads) {
+    const int r = i / kVecs, d = (i % kVecs) * 4;
+    const float* row = f(r);
+    const bool live = row != nullptr && d < D;
+    const int n = live ? 16 : 0;  // 0: zero-filled, nothing is read
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                     (uint32_t)__cvta_generic_to_shared(dst + r * (DP + kPad) + d)),
+                 "l"(live ? row + d : any), "r"(n)
+                 : "memory");
+  }
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
 // rows(r) -> const T* of row r of the tile, or null
 template <typename T, int RPT, int DP, class F>
@@ -205,14 +232,19 @@ __device__ __forceinline__ void tile_step(Tile<RPT, DP>& t, const Smem<RPT, DP>&
 __device__ __forceinline__ int out_col(int e, int tx) { return (e / 4) * 64 + tx * 4 + (e & 3); }
 
 // ------------------------------------------------------------ prompt
-// Grid (row tiles from the last, B * Hq): under causal the longest run first.
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) prompt_simt_kernel(PromptArgs a, bool vec) {
-  extern __shared__ float smem[];
+// One CTA per 64-row tile, (b, h) fastest, the last (under causal the longest)
+// tiles first.  Where all CTAs fit two to an SM, the second half runs from the
+// shortest up instead, so that every SM gets a long tile and a short one (2048
+// causal tokens, 8 heads: the longest SM 33 key tiles instead of 45).
+template <typename T, int DP, bool kAsync>
+__global__ void __launch_bounds__(kThreads) prompt_simt_kernel(const __grid_constant__ PromptArgs a, bool vec, int sms) {
+  extern __shared__ __align__(16) float smem[];
   constexpr int RPT = 4, BM = 64;
   Smem<RPT, DP> s(smem);
-  const int b = blockIdx.y / a.Hq, h = blockIdx.y % a.Hq, g = h / a.G;
-  const int r0 = (int)(gridDim.x - 1 - blockIdx.x) * BM;
+  const unsigned n_cta = gridDim.x, bhs = a.B * a.Hq;
+  const unsigned L = n_cta <= 2u * sms && blockIdx.x >= (unsigned)sms ? n_cta - 1 - (blockIdx.x - sms) : blockIdx.x;
+  const int b = (L % bhs) / a.Hq, h = (L % bhs) % a.Hq, g = h / a.G;
+  const int r0 = (int)(n_cta / bhs - 1 - L / bhs) * BM;
   const SeqView sv = seq_view(a.lens, a.cu, true, b, a.N, a.total);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   T* out = static_cast<T*>(a.out) + sv.q_b * a.os[0] + h * a.os[1] + (long long)sv.q_row * a.os[2];
@@ -227,21 +259,41 @@ __global__ void __launch_bounds__(kThreads) prompt_simt_kernel(PromptArgs a, boo
     load_rows<T, RPT, DP>(s.q, BM, [&](int r) { return r0 + r < sv.n ? q + (long long)(r0 + r) * a.qs[2] : nullptr; },
                           a.D, a.qs[3], vec);
     const int end = a.causal ? min(sv.n, r0 + BM) : sv.n;
-    for (int c0 = 0; c0 < end; c0 += BN) {
-      __syncthreads();
-      // keys past the end and keys the mask drops: zero rows, never products with what they hold
-      auto live = [&](int j) { return c0 + j < end && (km == nullptr || km[c0 + j] != 0); };
-      load_rows<T, RPT, DP>(s.k, BN, [&](int j) { return live(j) ? k + (long long)(c0 + j) * a.ks[2] : nullptr; }, a.D,
-                            a.ks[3], vec);
-      load_rows<T, RPT, DP>(s.v, BN, [&](int j) { return live(j) ? v + (long long)(c0 + j) * a.vs[2] : nullptr; }, a.D,
-                            a.vs[3], vec);
-      if (threadIdx.x < BN) s.bias[threadIdx.x] = live(threadIdx.x) ? 0.f : -INFINITY;
+    // keys past the end and keys the mask drops: zero rows, never products with what they hold
+    auto live = [&](int c) { return c < end && (km == nullptr || km[c] != 0); };
+    auto load = [&](int c0, const Smem<RPT, DP>& to) {
+      auto krow = [&](int j) { return live(c0 + j) ? k + (long long)(c0 + j) * a.ks[2] : nullptr; };
+      auto vrow = [&](int j) { return live(c0 + j) ? v + (long long)(c0 + j) * a.vs[2] : nullptr; };
+      if constexpr (kAsync) {
+        copy_rows<DP>(to.k, BN, krow, a.D, k);
+        copy_rows<DP>(to.v, BN, vrow, a.D, v);
+      } else {
+        load_rows<T, RPT, DP>(to.k, BN, krow, a.D, a.ks[3], vec);
+        load_rows<T, RPT, DP>(to.v, BN, vrow, a.D, a.vs[3], vec);
+      }
+      if (threadIdx.x < BN) to.bias[threadIdx.x] = live(c0 + threadIdx.x) ? 0.f : -INFINITY;
+    };
+    if constexpr (kAsync) {
+      load(0, s);
+      copy_commit();
+    }
+    for (int c0 = 0, turn = 0; c0 < end; c0 += BN, turn ^= 1) {
+      const Smem<RPT, DP> now(smem, kAsync ? turn : 0);
+      if constexpr (kAsync) {
+        if (c0 + BN < end) load(c0 + BN, Smem<RPT, DP>(smem, turn ^ 1));
+        copy_commit();
+        copy_wait<1>();
+      } else {
+        __syncthreads();
+        load(c0, now);
+      }
       __syncthreads();
       const bool diag = a.causal && c0 + BN - 1 > r0;
       tile_step<RPT, DP>(
-          t, s, a.scale, false, diag,
-          [&](int r, int j) { return s.bias[j] == 0.f && (!a.causal || c0 + j <= r0 + r); },
+          t, now, a.scale, false, diag,
+          [&](int r, int j) { return now.bias[j] == 0.f && (!a.causal || c0 + j <= r0 + r); },
           [](int, int, float) {});
+      if constexpr (kAsync) __syncthreads();  // the buffer is free
     }
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
@@ -301,14 +353,14 @@ __global__ void __launch_bounds__(kThreads) prompt_fill_kernel(PromptArgs a) {
 // border leaves one partial (m, l, unnormalised output) per CTA, in slot 0
 // when it is the CTA's first unit and slot 1 when a later one, which
 // cached_merge_kernel joins in CTA order.
-template <typename T, int RPT, int DP>
+template <typename T, int RPT, int DP, bool kAsync>
 __global__ void __launch_bounds__(kThreads) cached_simt_kernel(const __grid_constant__ CachedArgs a, bool vec) {
-  extern __shared__ float smem[];
+  extern __shared__ __align__(16) float smem[];
   constexpr int BM = 16 * RPT;
   Smem<RPT, DP> s(smem);
   __shared__ long long sh_first, sh_total;
   __shared__ int sh_b;
-  __shared__ longlong2 offs[BN];  // element offsets of the tile's k and v rows (-1: a zero row)
+  __shared__ longlong2 offs[3][BN];  // element offsets of three tiles' k and v rows (-1: a zero row)
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   cudaTriggerProgrammaticLaunchCompletion();  // the joining kernel may be set up beside this one
   if (threadIdx.x < 32) {
@@ -353,42 +405,69 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(const __grid_cons
           return r < a.R ? qb + (long long)(g * a.G + r / a.T) * a.qs[1] + (long long)(r % a.T) * a.qs[2] : nullptr;
         },
         a.D, a.qs[3], vec);
+    auto put_offsets = [&](int kt) {
+      if (threadIdx.x >= BN || kt >= k1) return;
+      const int c = kt * BN + threadIdx.x;
+      longlong2 o = make_longlong2(-1, -1);
+      if (c < len && !(off != nullptr && off[c] == -INFINITY)) {
+        const int pi = c / a.pg.page_size, in = c - pi * a.pg.page_size;
+        const int page = a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
+        if (page >= 0 && page < a.pg.num_pages) {
+          o.x = (long long)page * a.ks[0] + (long long)in * a.ks[1] + g * a.ks[2];
+          o.y = (long long)page * a.vs[0] + (long long)in * a.vs[1] + g * a.vs[2];
+        } else {
+          atomicOr(&g_attention_page_error, 1u);
+        }
+      }
+      offs[(kt - k0) % 3][threadIdx.x] = o;
+    };
+    auto load = [&](int kt, const Smem<RPT, DP>& to) {
+      if (kt >= k1) return;
+      const T *kp = static_cast<const T*>(a.k), *vp = static_cast<const T*>(a.v);
+      const longlong2* of = offs[(kt - k0) % 3];
+      auto krow = [&](int j) { return of[j].x >= 0 ? kp + of[j].x : nullptr; };
+      auto vrow = [&](int j) { return of[j].y >= 0 ? vp + of[j].y : nullptr; };
+      if constexpr (kAsync) {
+        copy_rows<DP>(to.k, BN, krow, a.D, kp);
+        copy_rows<DP>(to.v, BN, vrow, a.D, vp);
+      } else {
+        load_rows<T, RPT, DP>(to.k, BN, krow, a.D, a.ks[3], vec);
+        load_rows<T, RPT, DP>(to.v, BN, vrow, a.D, a.vs[3], vec);
+      }
+      if (off != nullptr && threadIdx.x < BN) {
+        const int c = kt * BN + threadIdx.x;
+        to.bias[threadIdx.x] = c < len ? off[c] : -INFINITY;
+      }
+    };
+    put_offsets(k0);
+    if constexpr (kAsync) {
+      put_offsets(k0 + 1);
+      __syncthreads();
+      load(k0, s);
+      copy_commit();
+    }
     for (int kt = k0; kt < k1; ++kt) {
       const int c0 = kt * BN;
-      if (threadIdx.x < BN) {
-        const int c = c0 + threadIdx.x;
-        longlong2 o = make_longlong2(-1, -1);
-        if (c < len && !(off != nullptr && off[c] == -INFINITY)) {
-          const int pi = c / a.pg.page_size, in = c - pi * a.pg.page_size;
-          const int page = a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
-          if (page >= 0 && page < a.pg.num_pages) {
-            o.x = (long long)page * a.ks[0] + (long long)in * a.ks[1] + g * a.ks[2];
-            o.y = (long long)page * a.vs[0] + (long long)in * a.vs[1] + g * a.vs[2];
-          } else {
-            atomicOr(&g_attention_page_error, 1u);
-          }
-        }
-        offs[threadIdx.x] = o;
-      }
-      __syncthreads();
-      const T *kp = static_cast<const T*>(a.k), *vp = static_cast<const T*>(a.v);
-      load_rows<T, RPT, DP>(s.k, BN, [&](int j) { return offs[j].x >= 0 ? kp + offs[j].x : nullptr; }, a.D, a.ks[3],
-                            vec);
-      load_rows<T, RPT, DP>(s.v, BN, [&](int j) { return offs[j].y >= 0 ? vp + offs[j].y : nullptr; }, a.D, a.vs[3],
-                            vec);
-      if (off != nullptr && threadIdx.x < BN) {
-        const int c = c0 + threadIdx.x;
-        s.bias[threadIdx.x] = c < len ? off[c] : -INFINITY;
+      const Smem<RPT, DP> now(smem, kAsync ? (kt - k0) & 1 : 0);
+      if constexpr (kAsync) {
+        load(kt + 1, Smem<RPT, DP>(smem, (kt + 1 - k0) & 1));
+        copy_commit();
+        put_offsets(kt + 2);
+        copy_wait<1>();
+      } else {
+        __syncthreads();  // the tile's offsets are there, the buffer is free
+        load(kt, now);
+        put_offsets(kt + 1);
       }
       __syncthreads();
       const bool drafts = c0 + BN > pre;  // some key of the tile is a drafted token or past the end
       float* sc = a.scores ? a.scores + ((long long)(b * a.Hkv + g) * a.G) * a.Lmax + c0 : nullptr;
       tile_step<RPT, DP>(
-          t, s, a.scale, off != nullptr, drafts,
+          t, now, a.scale, off != nullptr, drafts,
           [&](int i, int j) {
             const int c = c0 + j, r = rt * BM + i;
             if (c >= len || r >= a.R) return false;
-            if (off != nullptr && s.bias[j] == -INFINITY) return false;
+            if (off != nullptr && now.bias[j] == -INFINITY) return false;
             if (c < pre) return true;
             const int tok = r % a.T;
             return tree ? tree[tok * a.tr + (c - pre)] != 0 : c - pre <= tok;
@@ -396,6 +475,7 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(const __grid_cons
           [&](int i, int j, float x) {
             if (sc != nullptr && rt * BM + i < a.R && c0 + j < len) sc[(long long)(rt * BM + i) * a.Lmax + j] = x;
           });
+      if constexpr (kAsync) __syncthreads();  // the buffer is free, and the offsets two tiles ahead are there
     }
     const bool whole = k0 == 0 && k1 == nt;
     const int slot = begin >= ufirst ? 0 : 1;
@@ -598,15 +678,27 @@ bool rows_aligned(const void* p, const long long* st, int D, int es) {
   return st[3] == 1 && D % 4 == 0 && (uintptr_t)p % (4 * es) == 0 && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
 }
 
+template <typename T, int DP, bool kAsync>
+int prompt_simt_run(const PromptArgs& a, bool vec, cudaStream_t s) {
+  auto kern = prompt_simt_kernel<T, DP, kAsync>;
+  constexpr size_t bytes = Tile<4, DP>::bytes(kAsync ? 2 : 1);
+  static_assert(bytes <= 227 * 1024, "one CTA's shared memory");
+  if (allow_smem(kern, bytes) != KVBM_OK) return KVBM_ERR_CUDA;
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess) return KVBM_ERR_CUDA;
+  const long long grid = (long long)((a.N + 63) / 64) * a.B * a.Hq;
+  if (grid > 0x7fffffffLL) return KVBM_ERR_SHAPE;
+  kern<<<(unsigned)grid, kThreads, bytes, s>>>(a, vec, attention_device_sms(dev));
+  return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
+}
+
 template <typename T, int DP>
 int prompt_simt(const PromptArgs& a, cudaStream_t s) {
   const bool vec = rows_aligned(a.q, a.qs, a.D, sizeof(T)) && rows_aligned(a.k, a.ks, a.D, sizeof(T)) &&
                    rows_aligned(a.v, a.vs, a.D, sizeof(T));
-  auto kern = prompt_simt_kernel<T, DP>;
-  constexpr size_t bytes = Tile<4, DP>::kBytes;
-  if (allow_smem(kern, bytes) != KVBM_OK) return KVBM_ERR_CUDA;
-  kern<<<dim3((unsigned)((a.N + 63) / 64), (unsigned)(a.B * a.Hq)), kThreads, bytes, s>>>(a, vec);
-  return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
+  if constexpr (sizeof(T) == 4 && DP <= 128)
+    if (vec) return prompt_simt_run<T, DP, true>(a, vec, s);
+  return prompt_simt_run<T, DP, false>(a, vec, s);
 }
 
 template <typename T>
@@ -616,15 +708,23 @@ int prompt_simt_d(const PromptArgs& a, cudaStream_t s) {
   return prompt_simt<T, 256>(a, s);
 }
 
+template <typename T, int RPT, int DP, bool kAsync>
+int cached_simt_run(const CachedArgs& a, bool vec, cudaStream_t s) {
+  auto kern = cached_simt_kernel<T, RPT, DP, kAsync>;
+  constexpr size_t bytes = Tile<RPT, DP>::bytes(kAsync ? 2 : 1);
+  static_assert(bytes <= 227 * 1024, "one CTA's shared memory");
+  if (allow_smem(kern, bytes) != KVBM_OK) return KVBM_ERR_CUDA;
+  kern<<<(unsigned)a.C, kThreads, bytes, s>>>(a, vec);
+  return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
+}
+
 template <typename T, int RPT, int DP>
 int cached_simt(const CachedArgs& a, cudaStream_t s) {
   const bool vec = rows_aligned(a.q, a.qs, a.D, sizeof(T)) && rows_aligned(a.k, a.ks, a.D, sizeof(T)) &&
                    rows_aligned(a.v, a.vs, a.D, sizeof(T));
-  auto kern = cached_simt_kernel<T, RPT, DP>;
-  constexpr size_t bytes = Tile<RPT, DP>::kBytes;
-  if (allow_smem(kern, bytes) != KVBM_OK) return KVBM_ERR_CUDA;
-  kern<<<(unsigned)a.C, kThreads, bytes, s>>>(a, vec);
-  return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
+  if constexpr (sizeof(T) == 4 && DP <= 128)
+    if (vec) return cached_simt_run<T, RPT, DP, true>(a, vec, s);
+  return cached_simt_run<T, RPT, DP, false>(a, vec, s);
 }
 
 template <typename T>
