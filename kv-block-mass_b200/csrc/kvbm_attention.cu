@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(const __grid_cons
 // D <= 128, else 8).
 constexpr int kMergeRows = 16;
 template <typename T, int kCols>
-__global__ void __launch_bounds__(256, 4) cached_merge_kernel(const __grid_constant__ CachedArgs a) {
+__global__ void __launch_bounds__(256) cached_merge_kernel(const __grid_constant__ CachedArgs a) {
   const int unit = blockIdx.x, b = unit / (a.Hkv * a.RT), u = unit % (a.Hkv * a.RT), g = u / a.RT, rt = u % a.RT;
   const int lane = threadIdx.x & 31;
   long long pre, total;

@@ -226,6 +226,43 @@ def test_lowest_value_offsets(cuda_device, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,Hq", [(5, 4), (20, 8), (40, 8)])
+def test_lowest_value_offsets_of_a_tree(cuda_device, dtype, T, Hq):
+    c = Case([150, 130, T], 16, Hq, 2, 64, T, dtype, cuda_device, seed=19)
+    low = torch.finfo(torch.float32).min
+    off = torch.full((3, 1, c.L), low, device=cuda_device)
+    off[1, :, 60:] = 0.0
+    tree = _tree(3, T, 2, cuda_device)
+    out, lse = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, tree_mask=tree, log_offsets=off)
+    u = torch.finfo(dtype).eps / 2
+    for b in (0, 2):  # every key alike
+        keep = cached_keep(c.lens[b], T, tree[b], cuda_device).double()
+        for h in range(Hq):
+            v = c.rows(b, h // (Hq // 2))[1].double()
+            want, mass = keep @ v / keep.sum(1, keepdim=True), keep @ v.abs() / keep.sum(1, keepdim=True)
+            check(out[b, h], want, 2 * u * mass + u * want.abs() + 2.0 ** -18 * mass, "uniform")
+        assert bool((lse[b] == low).all())
+    keep = cached_keep(130, T, tree[1], cuda_device)[:, 60:]
+    for h in range(Hq):
+        k, v = (t[60:] for t in c.rows(1, h // (Hq // 2)))
+        o, l, _, ot, lt, _ = softmax_rows(c.q[1, h], k, v, keep, 0.125, dtype=dtype)
+        check(out[1, h], o, ot, "kept part")
+        check(lse[1, h], l, lt, "kept part")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [1, 12, 40])
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 3.0])
+def test_scales(cuda_device, dtype, T, scale):
+    c = Case([200, T, 77], 16, 8, 2, 64, T, dtype, cuda_device, seed=29)
+    off = torch.rand(3, 2, c.L, device=cuda_device)
+    out, lse = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, scale=scale)
+    _check(c, out, lse, scale=scale)
+    out, lse = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, scale=scale, log_offsets=off)
+    _check(c, out, lse, scale=scale, off=off)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("Hq,Hkv,D", [(8, 8, 64), (8, 2, 128), (14, 2, 64), (40, 2, 64)])
 def test_weights(cuda_device, dtype, Hq, Hkv, D):
     c = Case([1, 64, 257, 0, 700], 16, Hq, Hkv, D, 1, dtype, cuda_device, seed=D).poison_tail()
