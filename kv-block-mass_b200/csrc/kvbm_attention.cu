@@ -508,12 +508,13 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(const __grid_cons
 }
 
 // Joins the partials of every split unit, and writes the rows of sequences
-// with no keys (out 0, lse -inf).  A warp takes kMergeRows / 8 rows, one after
-// another, grid (B * Hkv * RT, BM / kMergeRows); partials in CTA order: the same
-// bits on every run.  Lanes read 32 partials' (m, l) at once and then stream
-// their output rows, eight loads in flight.  kCols: columns a lane holds (4 for
-// D <= 128, else 8).
-constexpr int kMergeRows = 16;
+// with no keys (out 0, lse -inf).  One warp a row, grid (B * Hkv * RT, BM /
+// kMergeRows); partials in CTA order: the same bits on every run.  Lanes read 32
+// partials' (m, l) at once and then stream their output rows, kAhead loads in
+// flight.  A row is a chain of two memory round trips, so rows go side by side:
+// four rows a warp one after another took 7 us more at 13 tokens.  kCols: columns
+// a lane holds (4 for D <= 128, else 8).
+constexpr int kMergeRows = 8;
 template <typename T, int kCols>
 __global__ void __launch_bounds__(256) cached_merge_kernel(const __grid_constant__ CachedArgs a) {
   const int unit = blockIdx.x, b = unit / (a.Hkv * a.RT), u = unit % (a.Hkv * a.RT), g = u / a.RT, rt = u % a.RT;
@@ -535,8 +536,8 @@ __global__ void __launch_bounds__(256) cached_merge_kernel(const __grid_constant
   cudaGridDependencySynchronize();
   if (nt > 0 && i0 == i1) return;  // finished by its CTA
   const int lanes = a.DP < 32 * kCols ? a.DP / kCols : 32;
-  for (int rl = blockIdx.y * kMergeRows + threadIdx.x / 32; rl < (int)(blockIdx.y + 1) * kMergeRows; rl += 8) {
-    const int r = rt * a.BM + rl;
+  {
+    const int rl = blockIdx.y * kMergeRows + threadIdx.x / 32, r = rt * a.BM + rl;
     if (rl >= a.BM || r >= a.R) return;
     const int h = g * a.G + r / a.T, tok = r % a.T;
     T* out = static_cast<T*>(a.out) + b * a.os[0] + h * a.os[1] + tok * a.os[2];
@@ -544,7 +545,7 @@ __global__ void __launch_bounds__(256) cached_merge_kernel(const __grid_constant
     if (nt == 0) {
       for (int d = lane; d < a.D; d += 32) out[d * a.os[3]] = from_f32<T>(0.f);
       if (lane == 0) *lse = -INFINITY;
-      continue;
+      return;
     }
     auto load_ml = [&](long long slot) {
       return slot < 0 ? make_float2(-INFINITY, 0.f) : a.part_ml[slot * a.BM + rl];
@@ -571,10 +572,11 @@ __global__ void __launch_bounds__(256) cached_merge_kernel(const __grid_constant
       for (int o = 16; o > 0; o >>= 1) lp += __shfl_xor_sync(0xffffffffu, lp, o);
       l += lp;
       const int n = min(32, i1 - base + 1);
-      for (int k0 = 0; k0 < n; k0 += 8) {
-        float x[8][kCols], fk[8];
+      constexpr int kAhead = 16 / kCols;
+      for (int k0 = 0; k0 < n; k0 += kAhead) {
+        float x[kAhead][kCols], fk[kAhead];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < kAhead; ++i) {
           fk[i] = __shfl_sync(0xffffffffu, f, (k0 + i) & 31);
           const long long pk = __shfl_sync(0xffffffffu, slot, (k0 + i) & 31);
           const bool in = k0 + i < n && fk[i] != 0.f && lane < lanes;
@@ -589,7 +591,7 @@ __global__ void __launch_bounds__(256) cached_merge_kernel(const __grid_constant
           }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < kAhead; ++i)
 #pragma unroll
           for (int e = 0; e < kCols; ++e) acc[e] = fmaf(x[i][e], fk[i], acc[e]);
       }
@@ -656,22 +658,6 @@ __global__ void __launch_bounds__(256) cached_weights_kernel(const __grid_consta
 #pragma unroll
   for (int e = 0; e < kVec; ++e)
     if (c + e < len) wo[e] = old[e] + sum[e];
-}
-
-// Launches a kernel that may start before the one ahead of it on the stream
-// has ended (it waits for it itself, in cudaGridDependencySynchronize).
-template <typename... P, typename... A>
-int launch_dependent(void (*kernel)(P...), dim3 grid, unsigned threads, cudaStream_t s, const A&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
 }
 
 bool rows_aligned(const void* p, const long long* st, int D, int es) {

@@ -91,9 +91,14 @@ __device__ __forceinline__ int cached_len(const CachedArgs& a, int b) {
 
 // First CTA-linear tile of CTA i, and the CTA that holds tile t, when `total`
 // tiles are cut into C ranges [i * total / C, (i + 1) * total / C).
-__device__ __forceinline__ long long split_begin(long long i, long long total, long long C) { return i * total / C; }
+// (32-bit divisions where the products fit: a 64-bit one is 100 instructions.)
+__device__ __forceinline__ long long split_begin(long long i, long long total, long long C) {
+  const long long p = i * total;
+  return p < (1ll << 32) ? (long long)((uint32_t)p / (uint32_t)C) : p / C;
+}
 __device__ __forceinline__ long long split_owner(long long t, long long total, long long C) {
-  return ((t + 1) * C + total - 1) / total - 1;
+  const long long p = (t + 1) * C + total - 1;
+  return (p < (1ll << 32) ? (long long)((uint32_t)p / (uint32_t)total) : p / total) - 1;
 }
 
 // Key tiles of sequences [0, b) (times units per sequence) by one warp:
@@ -199,6 +204,22 @@ int allow_smem_of(const void* kernel, size_t bytes);
 template <typename K>
 int allow_smem(K* kernel, size_t bytes) {
   return allow_smem_of(reinterpret_cast<const void*>(kernel), bytes);
+}
+
+// Launches a kernel that may start before the one ahead of it on the stream
+// has ended (it waits for it itself, in cudaGridDependencySynchronize).
+template <typename... P, typename... A>
+int launch_dependent(void (*kernel)(P...), dim3 grid, unsigned threads, cudaStream_t s, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
 }
 
 int attention_device_kind(int dev);  // 1: sm_100

@@ -69,6 +69,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(EvictArgs a, 
   __shared__ int scan_buf[kSelThreads / 32], warp_ties[kSelThreads / 32], warp_gt[kSelThreads / 32];
   __shared__ unsigned int s_prefix;
   __shared__ int s_left, cta_ties, cta_gt;
+  cudaTriggerProgrammaticLaunchCompletion();
   cg::cluster_group cl = cg::this_cluster();
   const int rank = kCluster > 1 ? (int)cl.block_rank() : 0;
   auto all_ctas = [&] {
@@ -230,6 +231,7 @@ template <typename V>
 __global__ void __launch_bounds__(kGatherThreads) evict_gather_kernel(EvictArgs a, int dv, int rows) {
   const int spb = kGatherThreads / (2 * dv);  // slots a step
   const int t = threadIdx.x, s = t / (2 * dv), e = t % (2 * dv);
+  cudaGridDependencySynchronize();  // set up beside the selection, whose slots it moves
   if (s >= spb) return;
   const bool isv = e >= dv;
   const int d = isv ? e - dv : e;
@@ -306,8 +308,8 @@ int launch_gather(EvictArgs a, int es, cudaStream_t s) {
   const int rows = a.zero_tail ? a.capacity : a.budget;
   const int per_block = kGatherThreads / (2 * dv) * kGatherUnroll;
   const long long blocks = ((long long)rows + per_block - 1) / per_block;
-  evict_gather_kernel<V><<<dim3((unsigned)blocks, (unsigned)(a.B * a.Hkv)), kGatherThreads, 0, s>>>(a, dv, rows);
-  return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
+  return launch_dependent(evict_gather_kernel<V>, dim3((unsigned)blocks, (unsigned)(a.B * a.Hkv)), kGatherThreads, s, a,
+                          dv, rows);
 }
 
 bool vec16(const void* p, const int64_t* st, int es) {
