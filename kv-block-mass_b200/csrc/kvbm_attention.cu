@@ -410,8 +410,7 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(const __grid_cons
       const int c = kt * BN + threadIdx.x;
       longlong2 o = make_longlong2(-1, -1);
       if (c < len && !(off != nullptr && off[c] == -INFINITY)) {
-        const int pi = c / a.pg.page_size, in = c - pi * a.pg.page_size;
-        const int page = a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
+        const int in = a.pg.slot(c), page = a.pg.page(b, a.pg.page_index(c));
         if (page >= 0 && page < a.pg.num_pages) {
           o.x = (long long)page * a.ks[0] + (long long)in * a.ks[1] + g * a.ks[2];
           o.y = (long long)page * a.vs[0] + (long long)in * a.vs[1] + g * a.vs[2];

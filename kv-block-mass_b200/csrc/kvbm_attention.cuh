@@ -48,7 +48,20 @@ struct PagedView {
   const int32_t* table;
   long long ts;
   int num_pages, page_size, max_pages;
+  int shift;  // log2(page_size), or -1: integer divisions cost the page lookups more than their loads do
+  // Page index and slot of row c.
+  __device__ __forceinline__ int page_index(int c) const { return shift >= 0 ? c >> shift : c / page_size; }
+  __device__ __forceinline__ int slot(int c) const { return shift >= 0 ? c & (page_size - 1) : c % page_size; }
+  // Page id of page index pi of sequence b.
+  __device__ __forceinline__ int page(int b, int pi) const { return table ? table[b * ts + pi] : b * max_pages + pi; }
 };
+
+inline PagedView paged_view(const int32_t* table, long long ts, int num_pages, int page_size, int max_pages) {
+  int shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (page_size == 1 << i) shift = i;
+  return PagedView{table, ts, num_pages, page_size, max_pages, shift};
+}
 
 // Attention over a cache: unit (b, g) has R = G * T rows, row r = hh * T + t.
 struct CachedArgs {
@@ -169,11 +182,9 @@ __device__ __noinline__ void add_draft_nonfinite(const CachedArgs& a, int b, int
   for (int c = lo; c < hi; ++c) {
     if (!(tree ? tree[tok * a.tr + (c - pre)] != 0 : c - pre <= tok)) continue;
     if (off != nullptr && off[c] == -INFINITY) continue;
-    const int pi = c / a.pg.page_size;
-    const int page = a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
+    const int page = a.pg.page(b, a.pg.page_index(c));
     if (page < 0 || page >= a.pg.num_pages) continue;
-    const T* v = static_cast<const T*>(a.v) + (long long)page * a.vs[0] +
-                 (long long)(c - pi * a.pg.page_size) * a.vs[1] + g * a.vs[2];
+    const T* v = static_cast<const T*>(a.v) + (long long)page * a.vs[0] + (long long)a.pg.slot(c) * a.vs[1] + g * a.vs[2];
     float* o = &acc.x;
     for (int e = 0; e < 4; ++e) {
       if (d + e >= a.D) continue;

@@ -122,7 +122,7 @@ void plan_cached(const kvbm_cached_args* p, int sms, CachedPlan* pl) {
     a.os[i] = p->out_stride[i];
   }
   for (int i = 0; i < 3; ++i) a.ls[i] = p->lse_stride[i];
-  a.pg = PagedView{p->block_table, p->block_table_stride, p->num_pages, p->page_size, p->max_pages};
+  a.pg = paged_view(p->block_table, p->block_table_stride, p->num_pages, p->page_size, p->max_pages);
   a.B = p->B;
   a.Hq = p->Hq;
   a.Hkv = p->Hkv;

@@ -166,8 +166,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? kMmaCtas : 1) cached_mma
     auto page_of = [&](int tile, int i) -> int {  // the page id of row i of a tile (-1: none)
       const int c = tile * KT + i;
       if (tile >= k1 || c >= len) return -1;
-      const int pi = c / a.pg.page_size;
-      return a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
+      return a.pg.page(b, a.pg.page_index(c));
     };
     auto put_offsets = [&](int tile, int i, int page) {
       if (tile >= k1) return;
@@ -175,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? kMmaCtas : 1) cached_mma
       longlong2 o = make_longlong2(-1, -1);
       if (c < len && !(off != nullptr && off[c] == -INFINITY)) {
         if (page >= 0 && page < a.pg.num_pages) {
-          const int in = c % a.pg.page_size;
+          const int in = a.pg.slot(c);
           o.x = (long long)page * a.ks[0] + (long long)in * a.ks[1] + g * a.ks[2];
           o.y = (long long)page * a.vs[0] + (long long)in * a.vs[1] + g * a.vs[2];
         } else {

@@ -304,8 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             auto page_at = [&](int j) -> int {  // -2: past the sequence, -1: not a page
               const int c = (sg.k0 + j) * TILE + (lane / kBlk) * rows;
               if (lane / kBlk >= pieces || j >= nk || c >= len) return -2;
-              const int pi = c / P;
-              const int page = a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
+              const int page = a.pg.page(b, a.pg.page_index(c));
               if (page >= 0 && page < a.pg.num_pages) return page;
               atomicOr(a.page_error, 1u);
               return -1;
@@ -317,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const unsigned there = __ballot_sync(0xffffffffu, page >= 0 && lane % kBlk == 0);
               const bool gone = __any_sync(0xffffffffu, page == -1);
               const uint32_t bytes = (uint32_t)__popc(there) * rows * DP * 2;
-              const int slot_c = ((sg.k0 + j) * TILE + (lane / kBlk) * rows) % P;
+              const int slot_c = a.pg.slot((sg.k0 + j) * TILE + (lane / kBlk) * rows);
 #pragma unroll 1
               for (int kv = 0; kv < 2; ++kv) {
                 const uint32_t i = idx + 2 * j + kv;
@@ -382,8 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
           auto page_of = [&](int c) -> int {
             if (c >= len) return -1;
-            const int pi = c / a.pg.page_size;
-            return a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
+            return a.pg.page(b, a.pg.page_index(c));
           };
           auto offset_of = [&](int c, int page) {
             longlong2 o = make_longlong2(-1, -1);
@@ -392,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               atomicOr(a.page_error, 1u);
               return o;
             }
-            const int at = c % a.pg.page_size;
+            const int at = a.pg.slot(c);
             o.x = (long long)page * a.ks[0] + (long long)at * a.ks[1] + g * a.ks[2];
             o.y = (long long)page * a.vs[0] + (long long)at * a.vs[1] + g * a.vs[2];
             return o;

@@ -251,8 +251,7 @@ __global__ void __launch_bounds__(kGatherThreads) evict_gather_kernel(EvictArgs 
   }
 #pragma unroll
   for (int i = 0; i < kGatherUnroll; ++i) {
-    const int pi = c[i] / a.pg.page_size;
-    page[i] = c[i] < 0 ? -1 : a.pg.table ? a.pg.table[b * a.pg.ts + pi] : b * a.pg.max_pages + pi;
+    page[i] = c[i] < 0 ? -1 : a.pg.page(b, a.pg.page_index(c[i]));
   }
   V v[kGatherUnroll];
 #pragma unroll
@@ -260,7 +259,7 @@ __global__ void __launch_bounds__(kGatherThreads) evict_gather_kernel(EvictArgs 
     v[i] = V{};
     if (c[i] < 0) continue;
     if (page[i] >= 0 && page[i] < a.pg.num_pages)
-      v[i] = src[page[i] * st[0] + (long long)(c[i] % a.pg.page_size) * st[1]];
+      v[i] = src[page[i] * st[0] + (long long)a.pg.slot(c[i]) * st[1]];
     else if (d == 0)
       atomicOr(a.page_error, 1u);
   }
@@ -356,7 +355,7 @@ extern "C" int kvbm_evict_cache(const kvbm_evict_args* e, void* stream) {
   if (attention_device_kind(dev) != 1) return KVBM_ERR_DEVICE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   EvictArgs a;
-  a.pg = PagedView{e->block_table, e->block_table_stride, e->num_pages, e->page_size, e->max_pages};
+  a.pg = paged_view(e->block_table, e->block_table_stride, e->num_pages, e->page_size, e->max_pages);
   a.k = static_cast<const char*>(e->k_cache);
   a.v = static_cast<const char*>(e->v_cache);
   a.ko = static_cast<char*>(e->k_out);
