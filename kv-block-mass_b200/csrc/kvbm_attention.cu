@@ -12,11 +12,13 @@
 //
 // Tiles: 16 x 16 threads own RPT x 4 scores each (RPT = 4: 64 rows, for
 // prompts and wide trees; RPT = 1: 16 rows, for single tokens), 64 keys a
-// tile, everything in fp32 registers and shared memory.  Bound by the FFMA
-// pipe (4 shared float4 reads feed 16 FFMAs per thread).  fp32 rows in 16-byte
+// tile, everything in fp32 registers and shared memory.  fp32 rows in 16-byte
 // pieces and D <= 128 (kAsync): k and v are double-buffered with cp.async, so that
-// a tile's products hide the next one's loads (2048-token causal prompt, 8 heads
-// of 64: 306 us without).
+// a tile's products hide the next one's loads.  Measured (fp32, 2048-token causal
+// prompt, 8 heads of 64): 199 us, 21 TFLOP/s; 306 us without the double buffer.
+// Bound by issue slots and shared memory's reads together (each about half of
+// its peak: 8 float4 reads feed 64 FFMAs a thread); 8 x 4 scores a thread, with
+// half the threads to hide latencies, took 240 us.
 #include <atomic>
 
 #include "kvbm_attention.cuh"

@@ -16,14 +16,21 @@
 //                   diagonal tiles, since 0 * NaN is not 0
 // Why two row tiles: while one tile's softmax runs, the tensor pipe does the
 // other tile's P V and next S; per pair and key tile the four MMAs need 2048
-// cycles at D = 128 and the 32768 exponentials 2048 MUFU cycles (less the
-// share the FMA pipe takes), so both units are close to full.  TMEM holds S/P
-// and O of both tiles: 2 * 128 + 2 * 128 columns.
+// cycles at D = 128 and the 32768 exponentials 2048 MUFU cycles.  TMEM holds
+// S/P and O of both tiles: 2 * 128 + 2 * 128 columns.
+//
+// Measured (bf16, D = 128, 32 q heads on 8, causal): one prompt of 16384 tokens
+// 1.89 ms, 1.16 PFLOP/s, 70 % of cuBLAS' rate for the same work, and 2.17 ms
+// called without pause (power); packed prompts of 217 to 2100 tokens, 0.22
+// TFLOP, 0.27 ms.  Bound by the chain score - maximum - weights of a tile: about
+// 3600 cycles, of which the other tile's tensor work fills 2048.  Without any
+// softmax the loop took 1.62 ms.  A pair of CTAs on one tile of 256 rows
+// (cta_group::2) took 2.66 ms: each step waits on the other CTA's softmax too.
 //
 // The CTAs are persistent (one per SM, items from the longest in a snake over
 // the CTAs): the next item's queries, keys and first scores are under way while
-// the last one's output is scaled and stored.  A CTA per item instead cost
-// about 10 us an item in set-up and drain.
+// the last one's output is scaled and stored.  (A CTA per item: packed prompts
+// 314 us where this took 283.)
 //
 // The running maximum is raised (and O multiplied in TMEM by its softmax
 // thread) only when a row's scores grow by more than 2^8 over it: weights stay

@@ -1,17 +1,17 @@
 // The softmax of a 128 x 128 score tile, shared by the tcgen05 attention
 // kernels.  Two threads own a row, 64 scores each, 32 in registers at a time;
-// its weights go to TMEM as the A operand of P V, over the same
-// scores;
-// its output accumulator is in TMEM, half of the columns to each of the two.
+// its weights go to TMEM as the A operand of P V, over the same scores; its
+// output accumulator is in TMEM, half of the columns to each of the two.
 //
 // Why two threads a row: with two tiles in flight the tensor pipe waits for
 // one tile's softmax while it does the other's P V and next S (1024 cycles at
-// D = 128).  One thread a row took about 2600 cycles a tile (128 scores one
-// after another, registers spilled); two need half, and the only price is one
-// exchange of the row maximum through shared memory.  The first 32 scores are
-// read from TMEM twice (for the maximum, and again for the weights): with all
-// 64 in registers the loop spilled (16k causal prompt 2.10 ms, with eight
-// registers a thread less 4.2 ms).
+// D = 128); two threads halve the chain of 128 exponentials a row, and the
+// price is one exchange of the row maximum through shared memory (16k causal
+// prompt, calls one after another: one thread a row 2.25 ms, two 2.17).  The
+// first 32 scores are read from TMEM twice (for the maximum, and again for the
+// weights): with all 64 in registers the loop spilled (2.10 ms where it now
+// takes 1.89, single calls).  All exponentials are MUFU's: taking one or two
+// in eight from the FMA pipe cost 2 and 5 % of the call.
 #pragma once
 
 #include "kvbm_sm100.cuh"
@@ -30,16 +30,6 @@ constexpr int kAttCols = 64;  // scores of a row in one thread
 // Growth of a row's maximum (base 2) that makes it the new reference: weights
 // stay below 2^8, which both 16-bit types hold at full precision.
 constexpr float kAttGrow = 8.f;
-// Of 8 groups of four columns, kAttEmu take their exp2 from the FMA pipe.  None:
-// here the tensor pipe and the power it draws bind, not the exponentials, and
-// the polynomial's instructions cost more than the MUFU time they save (16k
-// causal prompt, single / repeated calls: 0 of 8 1.91 / 2.23 ms, 1 of 8 1.95 /
-// 2.26, 2 of 8 2.00 / 2.32).
-#ifndef KVBM_ATT_EMU
-#define KVBM_ATT_EMU 0
-#endif
-constexpr int kAttEmu = KVBM_ATT_EMU;
-__host__ __device__ constexpr bool att_emulated(int g) { return ((g + 1) * kAttEmu) / 8 != (g * kAttEmu) / 8; }
 
 // A NaN among the values makes the maximum NaN (and with it the row).
 __device__ __forceinline__ float max32_nan(const float (&v)[32]) {
@@ -68,7 +58,9 @@ __device__ __forceinline__ void scale_output(uint32_t to, float f) {
 }
 
 // Weights of 32 scores, rounded to 16 bits, to the 16 columns at `ts`; returns
-// their float32 sum (of the unrounded values).
+// their float32 sum (of the unrounded values).  The rounding is half a step of
+// every weight, of either sign, about as much as the output's own; weights in
+// two parts would double P V, half of the tensor work that binds these kernels.
 //   kShift false: 2^(v C + shift), shift = -(reference in base 2)
 //   kShift true:  2^((v + shift) C), shift = -(reference), so that a score of
 //                 float32's lowest value less itself is 0
@@ -89,14 +81,7 @@ __device__ __forceinline__ float put_weights(const float (&v)[32], float C, floa
   for (int e = 0; e < 8; ++e) {
     const int c = 4 * e;
     const float2 x0 = arg(v[c], v[c + 1]), x1 = arg(v[c + 2], v[c + 3]);
-    float2 p0, p1;
-    if (att_emulated(e)) {
-      p0 = exp2_fma2<4>(x0);
-      p1 = exp2_fma2<4>(x1);
-    } else {
-      p0 = make_float2(ex2(x0.x), ex2(x0.y));
-      p1 = make_float2(ex2(x1.x), ex2(x1.y));
-    }
+    const float2 p0 = make_float2(ex2(x0.x), ex2(x0.y)), p1 = make_float2(ex2(x1.x), ex2(x1.y));
     s0 = fadd2_ftz(s0, p0);
     s1 = fadd2_ftz(s1, p1);
     p16[2 * e] = pack16<kBf16>(p0.x, p0.y);

@@ -17,7 +17,10 @@
 //                    key tiles and are joined from TMEM at the end.
 // Either way the tensor pipe works for one stream while the other's softmax
 // runs.  With 256 rows a key tile of 64 KB takes 2048 tensor cycles, about as
-// long as its bytes take from DRAM.
+// long as its bytes take from DRAM.  Measured: 4 sequences of 32768 keys, 64
+// tokens, 32 q heads on 8, D = 128: 178 us with the joining (16 us of it), 3.1
+// TB/s and 0.77 PFLOP/s.  Bound as the prompt kernel by the softmax chain, 3600
+// cycles a key tile.
 //
 // Log offsets are added in the natural-log domain, and subtracted from before
 // the conversion to base 2, so that offsets of float32's lowest value act like

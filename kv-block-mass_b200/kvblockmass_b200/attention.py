@@ -355,6 +355,10 @@ def _cached_args(q, k_cache, v_cache, block_table, seq_lens, tree_mask, log_offs
     a.scale = float(1.0 / D ** 0.5 if scale is None else scale)
     if out is not None or lse_out is not None:
         ins = {"q": q, "k_cache": k_cache, "v_cache": v_cache}
+        if log_offsets is not None:
+            ins["log_offsets"] = t
+        if weights is not None:
+            ins["weights"], ins["weights_out"] = weights, weights_out
     if out is None:
         out = q.new_empty((B, Hq, T, D))
     else:
@@ -364,7 +368,7 @@ def _cached_args(q, k_cache, v_cache, block_table, seq_lens, tree_mask, log_offs
         lse_out = q.new_empty((B, Hq, T), dtype=torch.float32)
     else:
         _check_out("lse_out", lse_out, (B, Hq, T), torch.float32, q.device)
-        _no_overlap("lse_out", lse_out, ins)
+        _no_overlap("lse_out", lse_out, {**ins, "out": out})
     a.out, a.lse = out.data_ptr(), lse_out.data_ptr()
     a.out_stride, a.lse_stride = _I4(*out.stride()), _I3(*lse_out.stride())
     return a, keep, out, lse_out, weights_out

@@ -142,6 +142,29 @@ def test_packed(cuda_device, dtype, causal, lens, D):
     assert torch.equal(o2[~gone], out[~gone]) and torch.equal(l2[:, ~gone], lse[:, ~gone])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,D,Hq", [(70, 64, 2), (33, 128, 3), (200, 64, 1)])
+def test_many_sequences(cuda_device, dtype, B, D, Hq):
+    """More sequences than a warp has lanes, packed and padded, most of one row tile or two."""
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 270, (B,), generator=g).tolist()
+    lens[1], lens[31], lens[32], lens[-1] = 0, 1, 600, 300
+    N = max(lens)
+    q, k, v = _inputs(B, Hq, 1, N, D, dtype, 12, cuda_device)
+    rows = torch.tensor(lens, device=cuda_device)
+    out, lse = kb.attention_b200(q, k, v, causal=True, seq_lens=rows)
+    _check_dense(q, k, v, out, lse, True, lens)
+    inside = (torch.arange(N, device=cuda_device) < rows[:, None])
+    pq, pk, pv = (t.transpose(1, 2)[inside].contiguous() for t in (q, k, v))
+    cu = torch.tensor([sum(lens[:i]) for i in range(B + 1)], dtype=torch.int32, device=cuda_device)
+    pout, plse = kb.attention_varlen(pq, pk, pv, cu, N, causal=True)
+    back = torch.zeros_like(out).transpose(1, 2).contiguous()
+    back[inside] = pout
+    lback = torch.full_like(lse, -math.inf).transpose(1, 2).contiguous()
+    lback[inside] = plse.T
+    _check_dense(q, k, v, back.transpose(1, 2), lback.transpose(1, 2), True, lens)
+
+
 def test_packed_cut_and_wrong_offsets(cuda_device):
     """Sequences longer than max_seqlen are cut there; offsets outside the rows are clamped."""
     q, k, v = (t[0].transpose(0, 1).contiguous() for t in _inputs(1, 2, 1, 200, 64, torch.bfloat16, 12, cuda_device))
@@ -176,6 +199,26 @@ def test_strides_and_out(cuda_device, dtype):
     k1 = k[:, :1].expand(B, Hkv, N, D)
     out, lse = kb.attention_b200(q, k1, v, causal=True)
     _check_dense(q, k1, v, out, lse, True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_offsets_past_32_bits(cuda_device, dtype):
+    """Heads, and positions, more than 2^32 elements apart in one buffer."""
+    dev, N, D = cuda_device, 200, 64
+    q, k, v = _inputs(1, 2, 2, N, D, dtype, 21, dev)
+    room = torch.empty(2 ** 32 + 2 ** 20, dtype=dtype, device=dev)
+    apart = 2 ** 32 + 64 * 1024
+    for strides in ((0, apart, D, 1), (0, D, (2 ** 32 // (N - 1) + 999) // 8 * 8, 1)):
+        big = room.as_strided((1, 2, N, D), strides)
+        for a in range(3):
+            args = [q, k, v]
+            big.copy_(args[a])
+            args[a] = big
+            out, lse = kb.attention_b200(*args, causal=True)
+            _check_dense(*args, out, lse, True)
+        o = torch.as_strided(room, (1, 2, N, D), strides)
+        kb.attention_b200(q, k, v, causal=True, out=o)
+        assert torch.equal(o, kb.attention_b200(q, k, v, causal=True)[0])
 
 
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-3, 4.0])

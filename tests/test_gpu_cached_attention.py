@@ -102,6 +102,23 @@ def test_single_token(cuda_device, dtype, page, Hq, Hkv, D):
     kb.check_device_errors()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Hq,Hkv,D", [(64, 1, 64), (136, 1, 128), (72, 2, 96), (400, 1, 64)])
+@pytest.mark.parametrize("offsets", [False, True])
+def test_single_token_of_large_groups(cuda_device, dtype, Hq, Hkv, D, offsets):
+    """More rows per kv head than 32 with one token, and more than 256."""
+    c = Case([700, 1, 0, 129, 64], 16, Hq, Hkv, D, 1, dtype, cuda_device, seed=Hq)
+    off = None
+    if offsets:
+        off = torch.randn(len(c.lens), Hkv, c.L, generator=torch.Generator().manual_seed(3))
+        off[:, :, ::7] = -math.inf
+        off[3] = -math.inf  # keeps nothing
+        off = off.to(cuda_device)
+    c.poison_tail()
+    out, lse = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, log_offsets=off)
+    _check(c, out, lse, off=off)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T", [2, 5, 16, 33, 64])
 @pytest.mark.parametrize("Hq,Hkv,D", [(4, 4, 64), (8, 2, 128), (7, 1, 64), (2, 1, 192)])
@@ -315,6 +332,31 @@ def test_long_cache(cuda_device):
         check(lse[0, h], l, lt, "lse")
 
 
+@pytest.mark.parametrize("dtype,T,page", [(torch.bfloat16, 1, 64), (torch.float16, 40, 64), (torch.bfloat16, 40, 24),
+                                          (torch.float32, 1, 64), (torch.float32, 40, 24)])
+def test_offsets_past_32_bits(cuda_device, dtype, T, page):
+    """The last pages of a cache of more than 2^32 elements; their eviction."""
+    n, D, Hkv, dev = 1001, 128, 2, cuda_device
+    pages = 2 ** 32 // (page * Hkv * D) + 60
+    k = torch.empty(pages, page, Hkv, D, dtype=dtype, device=dev)
+    per = -(-n // page)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    k[-per:] = torch.randn(per, page, Hkv, D, generator=g, device=dev).to(dtype)
+    table = (pages - 1 - torch.arange(per, device=dev)).to(torch.int32)[None]
+    q = torch.randn(1, 4, T, D, generator=g, device=dev).to(dtype)
+    out, lse = kb.attention_cached(q, k, k, table, torch.tensor([n]))
+    pos = torch.arange(n, device=dev)
+    rows = k[table[0].long()[pos // page], pos % page]
+    for h in range(4):
+        o, l, _, ot, lt, _ = softmax_rows(q[0, h], rows[:, h // 2], rows[:, h // 2], cached_keep(n, T, None, dev),
+                                          1 / math.sqrt(D), dtype=dtype)
+        check(out[0, h], o, ot, "out")
+        check(lse[0, h], l, lt, "lse")
+    w = torch.rand(1, 1, per * page, generator=g, device=dev)
+    e = kb.evict_cache(k, k, table, torch.tensor([n]), w, 500)
+    assert torch.equal(e.k[0], rows[e.kept[0, 0].long()]) and torch.equal(e.v, e.k)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_strides_and_no_table(cuda_device, dtype):
     """Head-major memory without a table, rows with a gap, q and out transposed, k off 16-byte alignment."""
@@ -444,6 +486,29 @@ def test_evict_long(cuda_device, n):
     assert torch.equal(e.k[0, :, 0], k[0, want.to(dev), 0])
 
 
+@pytest.mark.parametrize("B,n", [(30, 9001), (60, 9001), (2, 30_000), (80, 50_001)])
+def test_evict_rows_and_clusters(cuda_device, B, n):
+    """Rows shared by 4, 2, 8 and 1 CTAs; the last ones longer than shared memory holds."""
+    dev = cuda_device
+    g = torch.Generator().manual_seed(n + B)
+    w = torch.rand(B, 1, n, generator=g).to(dev)
+    w[:, 0, ::5] = 0.25
+    k = torch.randn(B, n, 1, 8, generator=g).half().to(dev)
+    lens = torch.full((B,), n, dtype=torch.int32)
+    lens[1], lens[B // 2] = 17, n - 4099
+    budget = n // 3
+    e = kb.evict_cache(k, k, None, lens, w, budget)
+    for b in range(B):
+        m = int(lens[b])
+        if m <= budget:
+            want = torch.arange(m, device=dev)
+        else:
+            mid = torch.sort(w[b, 0, 4:m - 32], descending=True, stable=True).indices[:budget - 36] + 4
+            want = torch.cat([torch.arange(4, device=dev), mid, torch.arange(m - 32, m, device=dev)]).sort().values
+        assert torch.equal(e.kept[b, 0, :len(want)].long(), want) and bool((e.kept[b, 0, len(want):] == -1).all())
+        assert torch.equal(e.k[b, :len(want), 0], k[b, want, 0]) and torch.equal(e.v[b], e.k[b])
+
+
 def test_evict_into_given_memory(cuda_device):
     c = Case([60, 200, 10], 16, 4, 2, 64, 1, torch.float16, cuda_device, seed=1)
     w = torch.rand(3, 2, c.L, device=cuda_device)
@@ -534,6 +599,7 @@ def test_design_offsets(cuda_device):
 def test_refusals(cuda_device):
     c = Case([40, 20], 16, 4, 2, 64, 1, torch.bfloat16, cuda_device)
     w = torch.zeros(2, 2, c.L, device=cuda_device)
+    both = torch.zeros(512, device=cuda_device)
     call = lambda **kw: kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, **kw)  # noqa: E731
     bad = [
         lambda: kb.attention_cached(c.q.cpu(), c.k, c.v, c.table, c.seq_lens),
@@ -558,6 +624,8 @@ def test_refusals(cuda_device):
         lambda: call(tree_mask=torch.ones(2, 2)),
         lambda: call(scale=math.nan),
         lambda: call(out=c.q),
+        lambda: call(out=both.view(torch.bfloat16)[:512].view(2, 4, 1, 64), lse_out=both[200:208].view(2, 4, 1)),
+        lambda: call(weights=w, lse_out=w.view(-1)[8:16].view(2, 4, 1)),
         lambda: call(workspace=torch.empty(16, dtype=torch.uint8, device=cuda_device)),
         lambda: kb.evict_cache(c.k, c.v, c.table, c.seq_lens, w, 0),
         lambda: kb.evict_cache(c.k, c.v, c.table, c.seq_lens, w, 35),  # sinks + recency do not fit
