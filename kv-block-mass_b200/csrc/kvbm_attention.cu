@@ -19,6 +19,8 @@
 // Bound by issue slots and shared memory's reads together (each about half of
 // its peak: 8 float4 reads feed 64 FFMAs a thread); 8 x 4 scores a thread, with
 // half the threads to hide latencies, took 240 us.
+#include <cooperative_groups.h>
+
 #include <atomic>
 
 #include "kvbm_attention.cuh"
@@ -234,19 +236,60 @@ __device__ __forceinline__ void tile_step(Tile<RPT, DP>& t, const Smem<RPT, DP>&
 __device__ __forceinline__ int out_col(int e, int tx) { return (e / 4) * 64 + tx * 4 + (e & 3); }
 
 // ------------------------------------------------------------ prompt
-// One CTA per 64-row tile, (b, h) fastest, the last (under causal the longest)
-// tiles first.  Where all CTAs fit two to an SM, the second half runs from the
-// shortest up instead, so that every SM gets a long tile and a short one (2048
-// causal tokens, 8 heads: the longest SM 33 key tiles instead of 45).
+// The parts of a tile's rows in the CTAs of a cluster: CTA `part` gets the
+// joined m, l and o of its share of every thread's rows.
+template <int DP>
+__device__ __forceinline__ void join_parts(Tile<4, DP>& t, float* smem, int split, int part) {
+  constexpr int RPT = 4, kCols = DP / 16, kEach = kCols + 2;
+  static_assert(sizeof(float) * RPT * kEach * kThreads <= Tile<4, DP>::bytes(1), "the parts' room");
+  cooperative_groups::cluster_group cl = cooperative_groups::this_cluster();
+  __syncthreads();  // everyone is done with the tiles
+  float* own = smem + threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    own[i * kEach * kThreads] = t.m[i];
+    own[(i * kEach + 1) * kThreads] = t.l[i];
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) own[(i * kEach + 2 + e) * kThreads] = t.o[i][e];
+  }
+  cl.sync();
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    if (i * split / RPT != part) continue;
+    float m = -INFINITY;
+    for (int p = 0; p < split; ++p) m = fmaxf(m, cl.map_shared_rank(own, p)[i * kEach * kThreads]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f, o[kCols];
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) o[e] = 0.f;
+    for (int p = 0; p < split; ++p) {
+      const float* from = cl.map_shared_rank(own, p) + i * kEach * kThreads;
+      const float f = exp2f((from[0] - base) * kLog2eF);
+      l = fmaf(from[kThreads], f, l);
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) o[e] = fmaf(from[(2 + e) * kThreads], f, o[e]);
+    }
+    t.m[i] = m;
+    t.l[i] = l;
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) t.o[i][e] = o[e];
+  }
+  cl.sync();  // the others have read this CTA's part
+}
+
+// A cluster of `split` CTAs per 64-row tile, (b, h) fastest, the last (under
+// causal the longest) tiles first.  CTA p takes the key tiles p, p + split, ..;
+// the parts of a row are joined through the cluster's shared memory, in order.
 template <typename T, int DP, bool kAsync>
-__global__ void __launch_bounds__(kThreads) prompt_simt_kernel(const __grid_constant__ PromptArgs a, bool vec, int sms) {
+__global__ void __launch_bounds__(kThreads) prompt_simt_kernel(const __grid_constant__ PromptArgs a, bool vec, int split) {
   extern __shared__ __align__(16) float smem[];
   constexpr int RPT = 4, BM = 64;
   Smem<RPT, DP> s(smem);
-  const unsigned n_cta = gridDim.x, bhs = a.B * a.Hq;
-  const unsigned L = n_cta <= 2u * sms && blockIdx.x >= (unsigned)sms ? n_cta - 1 - (blockIdx.x - sms) : blockIdx.x;
+  const unsigned items = gridDim.x / split, bhs = a.B * a.Hq;
+  const unsigned L = blockIdx.x / split;
+  const int part = blockIdx.x % split;
   const int b = (L % bhs) / a.Hq, h = (L % bhs) % a.Hq, g = h / a.G;
-  const int r0 = (int)(n_cta / bhs - 1 - L / bhs) * BM;
+  const int r0 = (int)(items / bhs - 1 - L / bhs) * BM;
   const SeqView sv = seq_view(a.lens, a.cu, true, b, a.N, a.total);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   T* out = static_cast<T*>(a.out) + sv.q_b * a.os[0] + h * a.os[1] + (long long)sv.q_row * a.os[2];
@@ -275,14 +318,15 @@ __global__ void __launch_bounds__(kThreads) prompt_simt_kernel(const __grid_cons
       }
       if (threadIdx.x < BN) to.bias[threadIdx.x] = live(c0 + threadIdx.x) ? 0.f : -INFINITY;
     };
+    const int step = BN * split;
     if constexpr (kAsync) {
-      load(0, s);
+      load(part * BN, s);
       copy_commit();
     }
-    for (int c0 = 0, turn = 0; c0 < end; c0 += BN, turn ^= 1) {
+    for (int c0 = part * BN, turn = 0; c0 < end; c0 += step, turn ^= 1) {
       const Smem<RPT, DP> now(smem, kAsync ? turn : 0);
       if constexpr (kAsync) {
-        if (c0 + BN < end) load(c0 + BN, Smem<RPT, DP>(smem, turn ^ 1));
+        if (c0 + step < end) load(c0 + step, Smem<RPT, DP>(smem, turn ^ 1));
         copy_commit();
         copy_wait<1>();
       } else {
@@ -297,10 +341,11 @@ __global__ void __launch_bounds__(kThreads) prompt_simt_kernel(const __grid_cons
           [](int, int, float) {});
       if constexpr (kAsync) __syncthreads();  // the buffer is free
     }
+    if (split > 1) join_parts<DP>(t, smem, split, part);
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
       const int r = r0 + ty * RPT + i;
-      if (r >= sv.n) continue;
+      if (r >= sv.n || i * split / RPT != part) continue;
       const float inv = t.l[i] > 0.f ? 1.f / t.l[i] : (t.l[i] == 0.f ? 0.f : t.l[i]);
 #pragma unroll
       for (int e = 0; e < DP / 16; ++e) {
@@ -310,7 +355,7 @@ __global__ void __launch_bounds__(kThreads) prompt_simt_kernel(const __grid_cons
       if (tx == 0) lse[r * a.ls[2]] = t.l[i] == 0.f ? -INFINITY : t.m[i] + logf(t.l[i]);
     }
   }
-  if (a.fill && a.cu == nullptr) {
+  if (a.fill && a.cu == nullptr && part == 0) {
     for (int i = threadIdx.x; i < BM; i += kThreads) {
       const int r = r0 + i;
       if (r >= sv.n && r < a.N) lse[r * a.ls[2]] = -INFINITY;
@@ -673,10 +718,28 @@ int prompt_simt_run(const PromptArgs& a, bool vec, cudaStream_t s) {
   if (allow_smem(kern, bytes) != KVBM_OK) return KVBM_ERR_CUDA;
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess) return KVBM_ERR_CUDA;
-  const long long grid = (long long)((a.N + 63) / 64) * a.B * a.Hq;
-  if (grid > 0x7fffffffLL) return KVBM_ERR_SHAPE;
-  kern<<<(unsigned)grid, kThreads, bytes, s>>>(a, vec, attention_device_sms(dev));
-  return cudaGetLastError() == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
+  const long long tiles = (a.N + 63) / 64, items = tiles * a.B * a.Hq;
+  if (items > 0x7fffffffLL) return KVBM_ERR_SHAPE;
+  // CTAs an item: while the items leave CTA slots empty, or barely fill them, the
+  // longest item decides (2048 causal tokens, 8 heads of 64, 256 items: 1 CTA 242
+  // us, 2 164, 4 178; 512 tokens, 64 items: 53, 31, 23); beyond, splitting costs
+  // the joining (1024 items of D = 128: 1217, 1304, 1618 us).
+  const long long slots = (long long)attention_device_sms(dev) * (Tile<4, DP>::bytes(kAsync ? 2 : 1) <= 113 * 1024 ? 2 : 1);
+  int split = 1;
+  while (split < 4 && items * split <= slots && 2 * split <= tiles) split *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(items * split));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = split > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, a, vec, split) == cudaSuccess ? KVBM_OK : KVBM_ERR_CUDA;
 }
 
 template <typename T, int DP>
