@@ -15,15 +15,18 @@
 // tile, everything in fp32 registers and shared memory.  fp32 rows in 16-byte
 // pieces and D <= 128 (kAsync): k and v are double-buffered with cp.async, so that
 // a tile's products hide the next one's loads.  Measured (fp32, 2048-token causal
-// prompt, 8 heads of 64): 199 us, 21 TFLOP/s; 306 us without the double buffer.
-// Bound by issue slots and shared memory's reads together (each about half of
-// its peak: 8 float4 reads feed 64 FFMAs a thread); 8 x 4 scores a thread, with
-// half the threads to hide latencies, took 240 us.
+// prompt, 8 heads of 64): 157 us, 27 TFLOP/s; 32 heads of 128: 1045 us, 33.
+// Bound by shared memory's reads: 8 float4 a thread feed 64 FFMAs, and a float4
+// read of a warp takes 4 passes, twice the FFMAs' time.  8 x 4 scores a thread
+// need 6 instead of 8, but leave half the warps to hide latencies (158 us, and
+// 1219 at D = 128); 2 x 8 need 10 (180 us).
 #include <cooperative_groups.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "kvbm_attention.cuh"
+#include "kvbm_sm100.cuh"
 
 namespace kvbm {
 namespace {
@@ -134,18 +137,22 @@ __device__ __forceinline__ void load_rows(float* dst, int rows, F&& f, int D, lo
 // One key tile: scores of the tile's 64 keys (K, V, bias already in shared
 // memory), softmax update, output update.  keep(r, j): whether row r keeps
 // key j of the tile.  sink(r, j, x): called for each kept-or-not score.
-// kSelect: some row may drop a key that another keeps, so products of dropped
+// select: some row may drop a key that another keeps, so products of dropped
 // pairs are left out one by one (0 * NaN is not 0).
+// Products go two by two (fma.rn.f32x2): half the issue slots, and the slots
+// bound as much as shared memory's reads (2048-token causal prompt, 8 heads of
+// 64: 165 -> 157 us; 32 heads of 128: 1218 -> 1045).
 template <int RPT, int DP, class Keep, class Sink>
 __device__ __forceinline__ void tile_step(Tile<RPT, DP>& t, const Smem<RPT, DP>& s, float scale, bool has_bias,
                                           bool select, Keep&& keep, Sink&& sink) {
   using TL = Tile<RPT, DP>;
+  constexpr int KC = DP / 16;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float x[RPT][4];
+  float2 x2[RPT][4];  // sums over the even and the odd elements
 #pragma unroll
   for (int i = 0; i < RPT; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[i][j] = 0.f;
+    for (int j = 0; j < 4; ++j) x2[i][j] = make_float2(0.f, 0.f);
 #pragma unroll 4
   for (int d = 0; d < DP; d += 4) {
     float4 qv[RPT], kv[4];
@@ -158,27 +165,25 @@ __device__ __forceinline__ void tile_step(Tile<RPT, DP>& t, const Smem<RPT, DP>&
     for (int i = 0; i < RPT; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        x[i][j] = fmaf(qv[i].x, kv[j].x, x[i][j]);
-        x[i][j] = fmaf(qv[i].y, kv[j].y, x[i][j]);
-        x[i][j] = fmaf(qv[i].z, kv[j].z, x[i][j]);
-        x[i][j] = fmaf(qv[i].w, kv[j].w, x[i][j]);
+        x2[i][j] = sm100::ffma2(make_float2(qv[i].x, qv[i].y), make_float2(kv[j].x, kv[j].y), x2[i][j]);
+        x2[i][j] = sm100::ffma2(make_float2(qv[i].z, qv[i].w), make_float2(kv[j].z, kv[j].w), x2[i][j]);
       }
   }
 #pragma unroll
   for (int i = 0; i < RPT; ++i) {
     const int r = ty * RPT + i;
-    float top = -INFINITY;
+    float x[4], top = -INFINITY;
     bool kp[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = tx + 16 * j;
       // natural-log domain: an offset of the type's lowest value stays finite
-      x[i][j] = x[i][j] * scale;
-      if (has_bias) x[i][j] += s.bias[c];
+      x[j] = (x2[i][j].x + x2[i][j].y) * scale;
+      if (has_bias) x[j] += s.bias[c];
       kp[j] = keep(r, c);
-      if (!kp[j]) x[i][j] = -INFINITY;
-      sink(r, c, x[i][j]);
-      top = fmaxf(top, x[i][j]);
+      if (!kp[j]) x[j] = -INFINITY;
+      sink(r, c, x[j]);
+      top = fmaxf(top, x[j]);
     }
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -188,7 +193,7 @@ __device__ __forceinline__ void tile_step(Tile<RPT, DP>& t, const Smem<RPT, DP>&
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float p = exp2f((x[i][j] - base) * kLog2eF);
+      const float p = exp2f((x[j] - base) * kLog2eF);
       sum += p;
       s.p[r * TL::kPs + tx + 16 * j] = kp[j] ? p : -0.f;
     }
@@ -197,39 +202,47 @@ __device__ __forceinline__ void tile_step(Tile<RPT, DP>& t, const Smem<RPT, DP>&
     t.l[i] = t.l[i] * corr + sum;
     t.m[i] = mn;
 #pragma unroll
-    for (int d = 0; d < DP / 16; ++d) t.o[i][d] *= corr;
+    for (int d = 0; d < KC; ++d) t.o[i][d] *= corr;
   }
   __syncwarp();  // a row's 64 weights come from its own half warp
-  float acc[RPT][DP / 16];  // this tile's share, added once: short sums lose less
+  float2 acc[RPT][KC / 2];  // this tile's share, added once: short sums lose less
 #pragma unroll
   for (int i = 0; i < RPT; ++i)
 #pragma unroll
-    for (int d = 0; d < DP / 16; ++d) acc[i][d] = 0.f;
-  for (int c = 0; c < BN; c += 4) {
-    float4 pv[RPT];
+    for (int d = 0; d < KC / 2; ++d) acc[i][d] = make_float2(0.f, 0.f);
+  auto product = [&](auto selects) {
+#pragma unroll 2
+    for (int c = 0; c < BN; c += 4) {
+      float4 pv[RPT];
 #pragma unroll
-    for (int i = 0; i < RPT; ++i) pv[i] = *reinterpret_cast<const float4*>(s.p + (ty * RPT + i) * TL::kPs + c);
+      for (int i = 0; i < RPT; ++i) pv[i] = *reinterpret_cast<const float4*>(s.p + (ty * RPT + i) * TL::kPs + c);
 #pragma unroll
-    for (int cc = 0; cc < 4; ++cc) {
+      for (int cc = 0; cc < 4; ++cc) {
 #pragma unroll
-      for (int dc = 0; dc < DP / 64; ++dc) {
-        const float4 vv = *reinterpret_cast<const float4*>(s.v + (c + cc) * TL::kStride + dc * 64 + tx * 4);
+        for (int dc = 0; dc < KC / 4; ++dc) {
+          const float4 vv = *reinterpret_cast<const float4*>(s.v + (c + cc) * TL::kStride + dc * 64 + tx * 4);
 #pragma unroll
-        for (int i = 0; i < RPT; ++i) {
-          const float p = cc == 0 ? pv[i].x : cc == 1 ? pv[i].y : cc == 2 ? pv[i].z : pv[i].w;
-          if (select && masked_p(p)) continue;
-          acc[i][dc * 4 + 0] = fmaf(p, vv.x, acc[i][dc * 4 + 0]);
-          acc[i][dc * 4 + 1] = fmaf(p, vv.y, acc[i][dc * 4 + 1]);
-          acc[i][dc * 4 + 2] = fmaf(p, vv.z, acc[i][dc * 4 + 2]);
-          acc[i][dc * 4 + 3] = fmaf(p, vv.w, acc[i][dc * 4 + 3]);
+          for (int i = 0; i < RPT; ++i) {
+            const float p = cc == 0 ? pv[i].x : cc == 1 ? pv[i].y : cc == 2 ? pv[i].z : pv[i].w;
+            if (decltype(selects)::value && masked_p(p)) continue;
+            acc[i][dc * 2] = sm100::ffma2(make_float2(p, p), make_float2(vv.x, vv.y), acc[i][dc * 2]);
+            acc[i][dc * 2 + 1] = sm100::ffma2(make_float2(p, p), make_float2(vv.z, vv.w), acc[i][dc * 2 + 1]);
+          }
         }
       }
     }
-  }
+  };
+  if (select)
+    product(std::true_type{});
+  else
+    product(std::false_type{});
 #pragma unroll
   for (int i = 0; i < RPT; ++i)
 #pragma unroll
-    for (int d = 0; d < DP / 16; ++d) t.o[i][d] += acc[i][d];
+    for (int d = 0; d < KC / 2; ++d) {
+      t.o[i][2 * d] += acc[i][d].x;
+      t.o[i][2 * d + 1] += acc[i][d].y;
+    }
 }
 
 // Output column of accumulator e of a thread.
