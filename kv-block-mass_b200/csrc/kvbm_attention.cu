@@ -595,76 +595,74 @@ __global__ void __launch_bounds__(256) cached_merge_kernel(const __grid_constant
   cudaGridDependencySynchronize();
   if (nt > 0 && i0 == i1) return;  // finished by its CTA
   const int lanes = a.DP < 32 * kCols ? a.DP / kCols : 32;
-  {
-    const int rl = blockIdx.y * kMergeRows + threadIdx.x / 32, r = rt * a.BM + rl;
-    if (rl >= a.BM || r >= a.R) return;
-    const int h = g * a.G + r / a.T, tok = r % a.T;
-    T* out = static_cast<T*>(a.out) + b * a.os[0] + h * a.os[1] + tok * a.os[2];
-    float* lse = a.lse + b * a.ls[0] + h * a.ls[1] + tok * a.ls[2];
-    if (nt == 0) {
-      for (int d = lane; d < a.D; d += 32) out[d * a.os[3]] = from_f32<T>(0.f);
-      if (lane == 0) *lse = -INFINITY;
-      return;
+  const int rl = blockIdx.y * kMergeRows + threadIdx.x / 32, r = rt * a.BM + rl;
+  if (rl >= a.BM || r >= a.R) return;
+  const int h = g * a.G + r / a.T, tok = r % a.T;
+  T* out = static_cast<T*>(a.out) + b * a.os[0] + h * a.os[1] + tok * a.os[2];
+  float* lse = a.lse + b * a.ls[0] + h * a.ls[1] + tok * a.ls[2];
+  if (nt == 0) {
+    for (int d = lane; d < a.D; d += 32) out[d * a.os[3]] = from_f32<T>(0.f);
+    if (lane == 0) *lse = -INFINITY;
+    return;
+  }
+  auto load_ml = [&](long long slot) {
+    return slot < 0 ? make_float2(-INFINITY, 0.f) : a.part_ml[slot * a.BM + rl];
+  };
+  long long slot = first;
+  float2 ml = load_ml(slot);
+  float m = ml.x;
+  for (int base = i0 + 32; base <= i1; base += 32) m = fmaxf(m, load_ml(slot_of(base + lane)).x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f, acc[kCols];
+#pragma unroll
+  for (int e = 0; e < kCols; ++e) acc[e] = 0.f;
+  for (int base = i0; base <= i1; base += 32) {
+    if (base > i0) {
+      slot = slot_of(base + lane);
+      ml = load_ml(slot);
     }
-    auto load_ml = [&](long long slot) {
-      return slot < 0 ? make_float2(-INFINITY, 0.f) : a.part_ml[slot * a.BM + rl];
-    };
-    long long slot = first;
-    float2 ml = load_ml(slot);
-    float m = ml.x;
-    for (int base = i0 + 32; base <= i1; base += 32) m = fmaxf(m, load_ml(slot_of(base + lane)).x);
+    // (a partial that kept nothing has l = 0; a NaN maximum gives a NaN factor)
+    const float f = ml.y == 0.f ? 0.f : exp2f((ml.x - ref) * kLog2eF);
+    float lp = ml.y * f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f, acc[kCols];
+    for (int o = 16; o > 0; o >>= 1) lp += __shfl_xor_sync(0xffffffffu, lp, o);
+    l += lp;
+    const int n = min(32, i1 - base + 1);
+    constexpr int kAhead = 16 / kCols;
+    for (int k0 = 0; k0 < n; k0 += kAhead) {
+      float x[kAhead][kCols], fk[kAhead];
 #pragma unroll
-    for (int e = 0; e < kCols; ++e) acc[e] = 0.f;
-    for (int base = i0; base <= i1; base += 32) {
-      if (base > i0) {
-        slot = slot_of(base + lane);
-        ml = load_ml(slot);
-      }
-      // (a partial that kept nothing has l = 0; a NaN maximum gives a NaN factor)
-      const float f = ml.y == 0.f ? 0.f : exp2f((ml.x - ref) * kLog2eF);
-      float lp = ml.y * f;
+      for (int i = 0; i < kAhead; ++i) {
+        fk[i] = __shfl_sync(0xffffffffu, f, (k0 + i) & 31);
+        const long long pk = __shfl_sync(0xffffffffu, slot, (k0 + i) & 31);
+        const bool in = k0 + i < n && fk[i] != 0.f && lane < lanes;
+        const float4* src = reinterpret_cast<const float4*>(a.part_o + (pk * a.BM + rl) * a.DP + lane * kCols);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) lp += __shfl_xor_sync(0xffffffffu, lp, o);
-      l += lp;
-      const int n = min(32, i1 - base + 1);
-      constexpr int kAhead = 16 / kCols;
-      for (int k0 = 0; k0 < n; k0 += kAhead) {
-        float x[kAhead][kCols], fk[kAhead];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          fk[i] = __shfl_sync(0xffffffffu, f, (k0 + i) & 31);
-          const long long pk = __shfl_sync(0xffffffffu, slot, (k0 + i) & 31);
-          const bool in = k0 + i < n && fk[i] != 0.f && lane < lanes;
-          const float4* src = reinterpret_cast<const float4*>(a.part_o + (pk * a.BM + rl) * a.DP + lane * kCols);
-#pragma unroll
-          for (int q = 0; q < kCols / 4; ++q) {
-            const float4 y = in ? src[q] : make_float4(0.f, 0.f, 0.f, 0.f);
-            x[i][4 * q] = y.x;
-            x[i][4 * q + 1] = y.y;
-            x[i][4 * q + 2] = y.z;
-            x[i][4 * q + 3] = y.w;
-          }
+        for (int q = 0; q < kCols / 4; ++q) {
+          const float4 y = in ? src[q] : make_float4(0.f, 0.f, 0.f, 0.f);
+          x[i][4 * q] = y.x;
+          x[i][4 * q + 1] = y.y;
+          x[i][4 * q + 2] = y.z;
+          x[i][4 * q + 3] = y.w;
         }
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i)
-#pragma unroll
-          for (int e = 0; e < kCols; ++e) acc[e] = fmaf(x[i][e], fk[i], acc[e]);
       }
-    }
-    const float inv = 1.f / l;
 #pragma unroll
-    for (int e = 0; e < kCols; ++e) {
-      const int d = lane * kCols + e;
-      if (lane < lanes && d < a.D) out[d * a.os[3]] = from_f32<T>(l == 0.f ? 0.f : acc[e] * inv);
+      for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) acc[e] = fmaf(x[i][e], fk[i], acc[e]);
     }
-    if (lane == 0) {
-      *lse = l == 0.f ? -INFINITY : m + logf(l);
-      if (a.stats) a.stats[(long long)(b * a.Hkv + g) * a.R + r] = make_float2(m, l == 0.f ? 0.f : inv);
-    }
+  }
+  const float inv = 1.f / l;
+#pragma unroll
+  for (int e = 0; e < kCols; ++e) {
+    const int d = lane * kCols + e;
+    if (lane < lanes && d < a.D) out[d * a.os[3]] = from_f32<T>(l == 0.f ? 0.f : acc[e] * inv);
+  }
+  if (lane == 0) {
+    *lse = l == 0.f ? -INFINITY : m + logf(l);
+    if (a.stats) a.stats[(long long)(b * a.Hkv + g) * a.R + r] = make_float2(m, l == 0.f ? 0.f : inv);
   }
 }
 

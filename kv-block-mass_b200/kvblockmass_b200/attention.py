@@ -154,11 +154,11 @@ def attention_b200(q, k, v, attn_mask=None, causal=False, scale=None, *, seq_len
     strides); ``out`` has it too, ``lse`` (natural log) is float32.
     ``attn_mask``: a key mask ``[N]`` or ``[B|1, 1, N]`` (True = keep); with
     ``causal`` a key must also not lie behind its query.  ``seq_lens [B]``:
-    sequence ``b`` is its first ``seq_lens[b]`` positions.  A row that keeps no
-    key gets ``out`` 0 and ``lse`` -inf, and so do rows past a sequence's end,
-    unless ``out=`` or ``lse_out=`` is given: those rows of both are then left
-    as they were.  What masked keys and rows past the end hold (NaN included)
-    reaches no result.
+    sequence ``b`` is its first ``seq_lens[b]`` positions (clamped into ``[0,
+    N]``). A row that keeps no key gets ``out`` 0 and ``lse`` -inf, and so do
+    rows past a sequence's end, unless ``out=`` or ``lse_out=`` is given: those
+    rows of both are then left as they were. What masked keys and rows past the
+    end hold (NaN included) reaches no result.
     """
     _check_qkv(q, k, v, "attention_b200")
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
@@ -395,7 +395,8 @@ def attention_cached(q, k_cache, v_cache, block_table, seq_lens, *, tree_mask=No
     ``i`` of sequence ``b``.  ``seq_lens [B]``: the cached tokens of each
     sequence, these ``T`` among them: token ``u`` sits in slot
     ``seq_lens[b] - T + u``, and its k and v are in the cache already.  A
-    sequence of length 0 gives ``out`` 0 and ``lse`` -inf.
+    sequence of length 0 gives ``out`` 0 and ``lse`` -inf; lengths outside ``[0,
+    max_pages * page_size]`` are clamped into it.
 
     Every token attends to the slots before the ``T`` tokens; among them token
     ``t`` attends to ``u`` where ``tree_mask [T, T]`` or ``[B|1, T, T]`` holds

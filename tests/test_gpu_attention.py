@@ -267,6 +267,38 @@ def test_deterministic_streams_and_graph(cuda_device, N, D, Hq):
     assert torch.equal(out.flip(0), o3) and torch.equal(lse.flip(0), l3)
 
 
+@pytest.mark.parametrize("N,D,Hq", [(300, 64, 8), (1000, 128, 4), (1030, 64, 40), (200, 200, 4)])
+def test_fp32_deterministic_streams_and_graph(cuda_device, N, D, Hq):
+    q, k, v = _inputs(2, Hq, 2, N, D, torch.float32, 42, cuda_device)
+    lens = torch.tensor([N, N // 3], dtype=torch.int32, device=cuda_device)
+    out, lse = kb.attention_b200(q, k, v, causal=True, seq_lens=lens)
+    _check_dense(q, k, v, out, lse, True, lens.tolist())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        o2, l2 = kb.attention_b200(q, k, v, causal=True, seq_lens=lens)
+    o1, l1 = kb.attention_b200(q, k, v, causal=True, seq_lens=lens)
+    side.synchronize()
+    assert torch.equal(out, o2) and torch.equal(lse, l2) and torch.equal(out, o1) and torch.equal(lse, l1)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o3, l3 = kb.attention_b200(q, k, v, causal=True, seq_lens=lens)
+    lens.copy_(torch.tensor([1, N]))
+    g.replay()
+    want = kb.attention_b200(q, k, v, causal=True, seq_lens=lens)
+    assert torch.equal(o3, want[0]) and torch.equal(l3, want[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_lengths_out_of_range(cuda_device, dtype):
+    """Lengths past N count as N, negative ones as 0."""
+    q, k, v = _inputs(3, 4, 2, 150, 64, dtype, 43, cuda_device)
+    for causal in (False, True):
+        a = kb.attention_b200(q, k, v, causal=causal, seq_lens=torch.tensor([150, 0, 77]))
+        b = kb.attention_b200(q, k, v, causal=causal, seq_lens=torch.tensor([2 ** 31 - 1, -1, 77]))
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 def test_feeds_block_mass(cuda_device):
     """The run of a prompt: attention, its lse into the block mass, and the mass of a call without it."""
     q, k, v = _inputs(2, 8, 2, 1000, 128, torch.bfloat16, 51, cuda_device)

@@ -435,6 +435,56 @@ def test_two_calls_and_graphs(cuda_device, T):
         assert torch.equal(out, w[0]) and torch.equal(lse, w[1])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_captured_run(cuda_device, dtype):
+    """A decode step that accumulates weights, an eviction and a tree over the compact cache, captured as one graph with
+    its own memory, replayed on new inputs beside eager calls of the same kind."""
+    T = 5
+    c = Case([900, 333, 64, 700], 16, 8, 2, 64, 1, dtype, cuda_device, seed=3)
+    w = torch.rand(4, 2, c.L, device=cuda_device)
+    qt = torch.randn(4, 8, T, 64, device=cuda_device).to(dtype)
+    room = tuple(torch.zeros(4, 208, 2, 64, dtype=dtype, device=cuda_device) for _ in range(2))
+
+    def run(w, room):
+        out, lse, w2 = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, weights=w, weights_out=torch.zeros_like(w))
+        e = kb.evict_cache(c.k, c.v, c.table, c.seq_lens, w2, 200, out=room)
+        return (out, lse, w2, e.kept, e.weights, e.seq_lens, *kb.attention_cached(qt, e.k, e.v, None, e.seq_lens))
+
+    run(w, room)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(w, room)
+    other = tuple(t.clone() for t in room)
+    for lens in ([900, 333, 64, 700], [200, 0, 201, 64], [899, 900, 900, 900]):
+        c.seq_lens.copy_(torch.tensor(lens))
+        w.copy_(torch.rand(w.shape))
+        graph.replay()
+        want = run(w, other)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T", [1, 3, 40])
+def test_lengths_out_of_range(cuda_device, dtype, T):
+    """Lengths past the table's pages count as all of them, negative ones as 0."""
+    c = Case([320, 320, 100], 16, 8, 2, 64, T, dtype, cuda_device, seed=4)
+    right = torch.tensor([320, 0, 100], dtype=torch.int32, device=cuda_device)
+    wrong = torch.tensor([2 ** 31 - 1, -5, 100], dtype=torch.int32, device=cuda_device)
+    for a, b in zip(kb.attention_cached(c.q, c.k, c.v, c.table, right),
+                    kb.attention_cached(c.q, c.k, c.v, c.table, wrong)):
+        assert torch.equal(a, b)
+    w = torch.rand(3, 2, c.L, device=cuda_device)
+    e, f = (kb.evict_cache(c.k, c.v, c.table, n, w, 64) for n in (right, wrong))
+    for name in ("k", "v", "seq_lens", "kept", "weights"):
+        assert torch.equal(getattr(e, name), getattr(f, name))
+    if T == 1:
+        a = kb.attention_cached(c.q, c.k, c.v, c.table, right, weights=w.clone())
+        b = kb.attention_cached(c.q, c.k, c.v, c.table, wrong, weights=w.clone())
+        assert torch.equal(a[2], b[2]) and torch.equal(a[2][1], w[1])
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, torch.float64])
 @pytest.mark.parametrize("shared", [False, True])
 @pytest.mark.parametrize("budget,n_sinks,recency", [(1, 0, 0), (1, 1, 0), (40, 4, 32), (36, 4, 32), (100, 0, 7),
