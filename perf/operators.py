@@ -13,7 +13,6 @@ Three operators that a serving loop runs one after another:
 64 bits.
 """
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -26,7 +25,6 @@ _DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 _BYTES = {"bf16": 2, "fp16": 2, "fp32": 4}
 
 
-@functools.cache
 def _package():
     path = str(Path(__file__).resolve().parent.parent / "kv-block-mass_b200")
     if path not in sys.path:
