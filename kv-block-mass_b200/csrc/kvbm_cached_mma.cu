@@ -267,9 +267,10 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? kMmaCtas : 1) cached_mma
       if (a.T > 1 && c0 + 16 > pre && c0 < len) {
         // drafted tokens: rows differ in which they keep.  Their non-finite
         // v elements are taken out here and added to the rows that keep them
-        // at the end.
+        // at the end.  (Slots before them stay as they are: every row keeps them.)
         bool bad = false;
         for (int i = lane; i < 16 * CF::kChunks; i += 32) {
+          if (c0 + i / CF::kChunks < pre) continue;
           uint4* p = reinterpret_cast<uint4*>(ring + (vt - ring_a) + i * 16);
           const uint4 w = *p;
           uint32_t x[4] = {w.x, w.y, w.z, w.w};
