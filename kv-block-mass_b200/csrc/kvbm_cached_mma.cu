@@ -161,6 +161,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? kMmaCtas : 1) cached_mma
     const int pre = len - a.T;
     const float* off = a.off ? a.off + b * a.ob + g * a.oh : nullptr;
     const uint8_t* tree = a.tree ? a.tree + b * a.tb : nullptr;
+    const bool drafts = a.T > 1 || tree != nullptr;  // rows may drop slots from `pre` on (a single token without a mask keeps its own)
 
     // ---- element offsets of a tile's rows, kStages tiles ahead of their use
     auto page_of = [&](int tile, int i) -> int {  // the page id of row i of a tile (-1: none)
@@ -264,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? kMmaCtas : 1) cached_mma
       }
       const uint32_t kt = ring_a + ((tile - k0) % CF::kStages) * 2 * CF::kTileBytes + warp * 16 * (DP * 2);
       const uint32_t vt = kt + CF::kTileBytes;
-      if (a.T > 1 && c0 + 16 > pre && c0 < len) {
+      if (drafts && c0 + 16 > pre && c0 < len) {
         // drafted tokens: rows differ in which they keep.  Their non-finite
         // v elements are taken out here and added to the rows that keep them
         // at the end.  (Slots before them stay as they are: every row keeps them.)
@@ -322,14 +323,14 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? kMmaCtas : 1) cached_mma
           for (int e = 0; e < 4; ++e)
             if (bias[nt2 * 2 + (e & 1)] == -INFINITY) s[nt2][e] = -INFINITY;
       }
-      if (c0 + 16 > (a.T > 1 ? pre : len)) {
+      if (c0 + 16 > (drafts ? pre : len)) {
 #pragma unroll
         for (int nt2 = 0; nt2 < 2; ++nt2)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int c = c0 + nt2 * 8 + cq + (e & 1), tok = (rt * BM + rq + (e >> 1) * 8) % a.T;
             bool keep = c < len;
-            if (keep && a.T > 1 && c >= pre) keep = tree ? tree[tok * a.tr + (c - pre)] != 0 : c - pre <= tok;
+            if (keep && drafts && c >= pre) keep = tree ? tree[tok * a.tr + (c - pre)] != 0 : c - pre <= tok;
             if (!keep) s[nt2][e] = -INFINITY;
           }
       }

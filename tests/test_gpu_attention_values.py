@@ -30,3 +30,29 @@ def test_nan_before_the_drafts(cuda_device, dtype, T, Hq, D):
     out, lse = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, tree_mask=tree)
     _check(c, out, lse, tree)
     assert bool(torch.isnan(out[..., 1:4]).all()) and bool(torch.isfinite(out[..., 4:]).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 64), (80, 2, 64), (4, 1, 192)])
+@pytest.mark.parametrize("weights", [False, True])
+def test_tree_mask_of_a_single_token(cuda_device, dtype, Hq, Hkv, D, weights):
+    """With one token the mask's one entry says whether it keeps its own slot; a dropped slot may hold anything."""
+    c = Case([1, 1, 2, 64, 65, 65, 200, 0], 16, Hq, Hkv, D, 1, dtype, cuda_device, seed=D)
+    tree = torch.tensor([0, 1, 0, 0, 0, 1, 0, 1], dtype=torch.bool, device=cuda_device).view(8, 1, 1)
+    for b, n in enumerate(c.lens):
+        if n and not bool(tree[b, 0, 0]):
+            _put(c, c.k, b, n - 1, slice(None), math.nan)
+            _put(c, c.v, b, n - 1, slice(0, None, 2), math.nan)
+            _put(c, c.v, b, n - 1, slice(1, None, 2), math.inf)
+    kw = {}
+    if weights:
+        kw["weights"] = torch.rand(8, Hkv, c.L, device=cuda_device)
+        kw["weights_out"] = torch.full_like(kw["weights"], 3.0)
+    got = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, tree_mask=tree, **kw)
+    _check(c, got[0], got[1], tree, weights=kw.get("weights"), wout=kw.get("weights_out"))
+    assert bool((got[0][0] == 0).all()) and bool((got[1][0] == -math.inf).all())
+    all_on = torch.ones(1, 1, dtype=torch.bool, device=cuda_device)
+    d = Case([1, 64, 200], 16, Hq, Hkv, D, 1, dtype, cuda_device, seed=D)
+    a = kb.attention_cached(d.q, d.k, d.v, d.table, d.seq_lens, tree_mask=all_on)
+    b = kb.attention_cached(d.q, d.k, d.v, d.table, d.seq_lens)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
