@@ -448,7 +448,17 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? kMmaCtas : 1) cached_mma
           acc.z = fmaf(x.z, f[w], acc.z);
           acc.w = fmaf(x.w, f[w], acc.w);
         }
-        if (bad && d < a.D) add_draft_nonfinite<T>(a, b, g, tok, max(max(pre, 0), k0 * KT), min(len, k1 * KT), pre, d, acc);
+        if (bad && d < a.D) add_nonfinite<T>(a, b, g, tok, max(max(pre, 0), k0 * KT), min(len, k1 * KT), pre, d, acc);
+        // The second part of a weight is zero or of either sign, so an infinite v of a kept key makes its column NaN:
+        // such a column is the sum of its non-finite values (their weights are positive).
+        if ((isnan(acc.x) || isnan(acc.y) || isnan(acc.z) || isnan(acc.w)) && !isnan(ll) && d < a.D) {
+          float4 odd = make_float4(0.f, 0.f, 0.f, 0.f);
+          add_nonfinite<T>(a, b, g, tok, k0 * KT, min(len, k1 * KT), pre, d, odd);
+          if (isnan(acc.x) && odd.x != 0.f) acc.x = odd.x;
+          if (isnan(acc.y) && odd.y != 0.f) acc.y = odd.y;
+          if (isnan(acc.z) && odd.z != 0.f) acc.z = odd.z;
+          if (isnan(acc.w) && odd.w != 0.f) acc.w = odd.w;
+        }
         if (whole) {
           if (d < a.D) {
             const bool none = ll == 0.f;

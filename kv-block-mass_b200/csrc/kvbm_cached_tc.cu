@@ -644,8 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int e = 0; e < kStep; e += 4) {
               float4 x = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
               if (d0 + e < a.D)
-                add_draft_nonfinite<T>(a, b, g, tok, max(max(pre, 0), sg.k0 * TILE), min(len, sg.k1 * TILE), pre, d0 + e,
-                                       x);
+                add_nonfinite<T>(a, b, g, tok, max(max(pre, 0), sg.k0 * TILE), min(len, sg.k1 * TILE), pre, d0 + e, x);
               o[e] = x.x;
               o[e + 1] = x.y;
               o[e + 2] = x.z;

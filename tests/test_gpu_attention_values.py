@@ -56,3 +56,33 @@ def test_tree_mask_of_a_single_token(cuda_device, dtype, Hq, Hkv, D, weights):
     a = kb.attention_cached(d.q, d.k, d.v, d.table, d.seq_lens, tree_mask=all_on)
     b = kb.attention_cached(d.q, d.k, d.v, d.table, d.seq_lens)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,Hq,D", [(1, 8, 64), (1, 8, 128), (1, 4, 192), (3, 8, 64), (13, 4, 128), (40, 8, 64)])
+@pytest.mark.parametrize("lens", [[1, 64, 65, 200], [5003]])
+def test_infinite_values_of_kept_keys(cuda_device, dtype, T, Hq, D, lens):
+    """Infinities in the v of kept keys: one of a sign gives it, both signs and a NaN give NaN; every other column is
+    finite; those of dropped keys reach nothing."""
+    lens = [n + T - 1 for n in lens]
+    c = Case(lens, 16, Hq, 2, D, T, dtype, cuda_device, seed=T + D)
+    off = torch.zeros(len(lens), 1, c.L, device=cuda_device)
+    for b, n in enumerate(lens):
+        last = max(n - T, 0)  # kept by every token
+        _put(c, c.v, b, last, 1, math.inf)
+        _put(c, c.v, b, last, 2, -math.inf)
+        _put(c, c.v, b, last // 2, 2, -math.inf)
+        if last > 3:
+            _put(c, c.v, b, 0, 3, math.inf)
+            _put(c, c.v, b, last, 3, -math.inf)
+            _put(c, c.v, b, 1, 4, math.nan)
+            _put(c, c.v, b, 2, slice(5, None, 2), math.inf)
+            off[b, 0, 2] = -math.inf
+    out, lse = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, log_offsets=off)
+    _check(c, out, lse, off=off)
+    assert bool((out[..., 1] == math.inf).all()) and bool((out[..., 2] == -math.inf).all())
+    if T == 1:
+        w = torch.zeros(len(lens), 2, c.L, device=cuda_device)
+        a = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, log_offsets=off, weights=w)
+        assert torch.equal(a[0].isnan(), out.isnan()) and torch.equal(a[0].nan_to_num(), out.nan_to_num())
+        assert bool(torch.isfinite(w).all())
