@@ -490,8 +490,9 @@ KVBM_API int kvbm_design(const kvbm_design_args* d, const kvbm_design_out* out, 
  * a row past a sequence's end) holds, NaN and infinities included, reaches no
  * result.  lse is what kvbm_block_mass_lse and kvbm_options.lse take.
  *
- * float32, bfloat16 or float16 (out in the same type; sums, maxima and lse in
- * float32), D <= 256, any strides (elements, dims [B, H, N, D]; lse [B, H, N]).
+ * float32, bfloat16 or float16 (out in the same type; sums, maxima, lse and
+ * scale in float32: a smaller scale is 0, a larger one KVBM_ERR_SHAPE),
+ * D <= 256, any strides (elements, dims [B, H, N, D]; lse [B, H, N]).
  * Layouts as kvbm_options: dense, padded with seq_lens, or packed with
  * cu_seqlens (q, k, v, out and lse packed alike, [total_tokens, H, D]: strides
  * {unused, head, row, d}).  fill_outside != 0: rows of `out` and `lse` that

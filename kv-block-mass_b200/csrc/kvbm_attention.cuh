@@ -196,6 +196,10 @@ __device__ __noinline__ void add_nonfinite(const CachedArgs& a, int b, int g, in
   }
 }
 
+// Scales the tcgen05 kernels take: positive (the maximum of the raw scores is
+// the maximum), and finite as a factor of base-2 exponents.
+inline bool tc_scale(float scale) { return scale > 0.f && scale * kLog2eF < INFINITY; }
+
 // Launchers (kvbm_status).
 int launch_prompt_simt(const PromptArgs& a, int dtype, cudaStream_t s);
 int launch_prompt_fill(const PromptArgs& a, int dtype, cudaStream_t s);

@@ -14,6 +14,12 @@ size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
 bool dtype_ok(int dtype) { return dtype == KVBM_F32 || dtype == KVBM_BF16 || dtype == KVBM_F16; }
 
+// The kernels take the scale in float32 (below its smallest value: 0).
+bool scale_ok(double scale) {
+  const float f = (float)scale;
+  return f - f == 0.f;  // neither NaN nor infinite
+}
+
 int check_prompt(const kvbm_attention_args* p) {
   if (p == nullptr) return KVBM_ERR_NULL;
   if (!dtype_ok(p->dtype)) return KVBM_ERR_DTYPE;
@@ -27,7 +33,7 @@ int check_prompt(const kvbm_attention_args* p) {
     if (p->q_stride[i] < 0 || p->k_stride[i] < 0 || p->v_stride[i] < 0 || p->out_stride[i] < 0) return KVBM_ERR_SHAPE;
   for (int i = 0; i < 3; ++i)
     if (p->lse_stride[i] < 0) return KVBM_ERR_SHAPE;
-  if (!(p->scale - p->scale == 0.0)) return KVBM_ERR_SHAPE;  // NaN or infinite scale
+  if (!scale_ok(p->scale)) return KVBM_ERR_SHAPE;
   const bool no_rows = p->cu_seqlens != nullptr && p->total_tokens == 0;  // an empty tensor's pointer may be NULL
   if (!no_rows && !(p->q && p->k && p->v && p->out && p->lse)) return KVBM_ERR_NULL;
   return KVBM_OK;
@@ -80,7 +86,7 @@ int check_cached(const kvbm_cached_args* p) {
     if (p->q_stride[i] < 0 || p->k_stride[i] < 0 || p->v_stride[i] < 0 || p->out_stride[i] < 0) return KVBM_ERR_SHAPE;
   for (int i = 0; i < 3; ++i)
     if (p->lse_stride[i] < 0) return KVBM_ERR_SHAPE;
-  if (!(p->scale - p->scale == 0.0)) return KVBM_ERR_SHAPE;
+  if (!scale_ok(p->scale)) return KVBM_ERR_SHAPE;
   if ((p->weights != nullptr) != (p->weights_out != nullptr)) return KVBM_ERR_NULL;
   if (p->weights != nullptr && p->T != 1) return KVBM_ERR_SHAPE;
   if (!p->q || !p->k_cache || !p->v_cache || !p->seq_lens || !p->out || !p->lse) return KVBM_ERR_NULL;
@@ -149,7 +155,7 @@ void plan_cached(const kvbm_cached_args* p, int sms, CachedPlan* pl) {
   // 16-bit types: up to 32 rows, mma.sync, which reads the cache once per 16
   // rows; above, tcgen05, whose tiles of 128 rows cost a 16-row unit eight
   // times its tensor work.
-  pl->kernel = !cached_mma_supported(p) ? 0 : (a.R > kMmaRows && a.D <= 128 && a.w == nullptr && p->scale > 0.0) ? 2 : 1;
+  pl->kernel = !cached_mma_supported(p) ? 0 : (a.R > kMmaRows && a.D <= 128 && a.w == nullptr && tc_scale(a.scale)) ? 2 : 1;
   a.BM = pl->kernel == 2 ? (a.R > 128 ? 256 : 128) : pl->kernel == 1 || a.R <= 16 ? 16 : 64;
   a.KT = pl->kernel == 2 ? 128 : kCachedKeyTile;
   a.RT = (a.R + a.BM - 1) / a.BM;

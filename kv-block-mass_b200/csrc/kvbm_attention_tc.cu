@@ -556,7 +556,7 @@ int launch(const PromptArgs& a, int sms, cudaStream_t s) {
 
 bool prompt_tc_supported(const PromptArgs& a, int dtype) {
   if (dtype != KVBM_BF16 && dtype != KVBM_F16) return false;
-  if (a.D > 128 || a.D % 8 != 0 || !(a.scale > 0.f) || !tc_path_enabled()) return false;
+  if (a.D > 128 || a.D % 8 != 0 || !tc_scale(a.scale) || !tc_path_enabled()) return false;
   const bool packed = a.cu != nullptr;
   const int B = packed ? 1 : a.B, N = packed ? (int)a.total : a.N;
   const int qd[3] = {B, a.Hq, N}, kd[3] = {B, a.Hkv, N};

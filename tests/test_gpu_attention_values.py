@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import kvblockmass_b200 as kb
+from test_gpu_attention import _check_dense, _inputs
 from test_gpu_cached_attention import Case, _check, _tree
 
 pytestmark = pytest.mark.gpu
@@ -86,3 +87,24 @@ def test_infinite_values_of_kept_keys(cuda_device, dtype, T, Hq, D, lens):
         a = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, log_offsets=off, weights=w)
         assert torch.equal(a[0].isnan(), out.isnan()) and torch.equal(a[0].nan_to_num(), out.nan_to_num())
         assert bool(torch.isfinite(w).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scales_outside_float32(cuda_device, dtype):
+    """A scale below float32's smallest value is 0 (equal weights); one above its largest is refused."""
+    q, k, v = _inputs(1, 2, 1, 200, 64, dtype, 21, cuda_device)
+    for scale in (1e-60, -1e-60):
+        out, lse = kb.attention_b200(q, k, v, causal=True, scale=scale)
+        _check_dense(q, k, v, out, lse, True, scale=scale)
+    for T in (1, 12, 40):
+        c = Case([200, T, 77], 16, 8, 2, 64, T, dtype, cuda_device, seed=29)
+        off = torch.rand(3, 2, c.L, device=cuda_device)
+        for scale in (1e-60, -1e-60):
+            for o in (None, off):
+                out, lse = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, scale=scale, log_offsets=o)
+                _check(c, out, lse, scale=scale, off=o)
+        for scale in (1e60, -1e60):
+            with pytest.raises(ValueError):
+                kb.attention_b200(q, k, v, scale=scale)
+            with pytest.raises(ValueError):
+                kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, scale=scale)
