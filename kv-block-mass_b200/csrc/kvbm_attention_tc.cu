@@ -432,8 +432,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = false;
           break;
         }
-        mt = fmax_nan(mt, mx[(half ^ 1) * TILE + rl]) * C;
-        const bool grow = !(mt <= m + kAttGrow);  // (true from -inf to anything finite, and for NaN)
+        mt = __fmul_rn(fmax_nan(mt, mx[(half ^ 1) * TILE + rl]), C);  // rounded as the weights' products are
+        const bool grow = mt - m > kAttGrow || mt != mt;  // (true from -inf to anything finite, and for NaN)
         if (__any_sync(0xffffffffu, grow)) {
           const float mn = grow ? mt : m;
           const float f = m == mn ? 1.f : ex2(m - mn);

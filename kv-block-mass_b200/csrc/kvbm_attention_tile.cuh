@@ -28,7 +28,8 @@ namespace sm100 {
 constexpr int kAttTile = 128;
 constexpr int kAttCols = 64;  // scores of a row in one thread
 // Growth of a row's maximum (base 2) that makes it the new reference: weights
-// stay below 2^8, which both 16-bit types hold at full precision.
+// stay below 2^8, which both 16-bit types hold at full precision.  (The
+// difference is compared: adding the growth to a large reference rounds it.)
 constexpr float kAttGrow = 8.f;
 
 // A NaN among the values makes the maximum NaN (and with it the row).
@@ -61,7 +62,11 @@ __device__ __forceinline__ void scale_output(uint32_t to, float f) {
 // their float32 sum (of the unrounded values).  The rounding is half a step of
 // every weight, of either sign, about as much as the output's own; weights in
 // two parts would double P V, half of the tensor work that binds these kernels.
-//   kShift false: 2^(v C + shift), shift = -(reference in base 2)
+//   kShift false: 2^(fl(v C) + shift), shift = -(reference in base 2).  The product
+//                 is rounded before the sum, as it was in the reference: in one FMA
+//                 the reference's rounding stays in every exponent of the row, up
+//                 to half its step, and scores past 2^24 leave the 16-bit range
+//                 (16k causal prompt 2.18 ms that way, 2.21 this)
 //   kShift true:  2^((v + shift) C), shift = -(reference), so that a score of
 //                 float32's lowest value less itself is 0
 template <bool kBf16, bool kShift>
@@ -73,7 +78,7 @@ __device__ __forceinline__ float put_weights(const float (&v)[32], float C, floa
       const float2 d = fadd2(make_float2(a, b), N2);
       return ffma2(d, C2, make_float2(0.f, 0.f));
     } else {
-      return ffma2(make_float2(a, b), C2, N2);
+      return fadd2(ffma2(make_float2(a, b), C2, make_float2(0.f, 0.f)), N2);
     }
   };
   uint32_t p16[16];

@@ -572,8 +572,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         mt = fmax_nan(mt, mx[(half ^ 1) * TILE + rl]);
-        if (!kBias) mt *= C;
-        const bool grow = !(mt <= m + (kBias ? kAttGrow * kLn2F : kAttGrow));
+        if (!kBias) mt = __fmul_rn(mt, C);  // rounded as the weights' products are
+        const bool grow = mt - m > (kBias ? kAttGrow * kLn2F : kAttGrow) || mt != mt;
         if (__any_sync(0xffffffffu, grow)) {
           const float mn = grow ? mt : m;
           const float f = m == mn ? 1.f : ex2(kBias ? (m - mn) * kLog2eF : m - mn);

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import kvblockmass_b200 as kb
+from _attention_ref import F64, cached_keep, check, half_step
 from test_gpu_attention import _check_dense, _inputs
 from test_gpu_cached_attention import Case, _check, _tree
 
@@ -108,3 +109,41 @@ def test_scales_outside_float32(cuda_device, dtype):
                 kb.attention_b200(q, k, v, scale=scale)
             with pytest.raises(ValueError):
                 kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("big,small", [(22528.0, 22400.0), (352.0, 350.0)])
+def test_scores_past_float32_steps(cuda_device, dtype, big, small):
+    """Scores of 3e10 (and 5e8), whose float32 steps are 2048 and 32: the highest ones, which are equal, share the
+    weight, and nothing overflows.  Every product and sum here is exact in float32, so the weights are 1 / count:
+    rounded once (2 u of the mass), as the sums, and the result once (u).  The lse is the score: the scale, its
+    product, and with a maximum in base 2 the two factors and their products, 2^-24 each."""
+    dev, D = cuda_device, 64
+    u = half_step(dtype)
+
+    def close(out, lse, v, keep, what):
+        p = keep.double() / keep.sum(1, keepdim=True)
+        check(out, p @ v.double(), (2 * u + 2.0 ** -18) * (p @ v.double().abs()) + u * (p @ v.double()).abs(), what)
+        top = 20480.0 * big * 64
+        want = torch.full((keep.shape[0],), top, dtype=F64, device=dev) + keep.sum(1).double().log()
+        check(lse, want, 6 * 2.0 ** -24 * want, what)
+
+    def rows(n):
+        t = torch.full((n, D), big, device=dev)
+        t[1::2] = small
+        return t.to(dtype)
+
+    N = 300
+    v = torch.randn(1, 1, N, D, device=dev).to(dtype)
+    q = torch.full((1, 1, N, D), 20480.0, device=dev).to(dtype)
+    even = (torch.arange(N, device=dev) % 2 == 0)[None]
+    out, lse = kb.attention_b200(q, rows(N)[None, None], v, causal=True, scale=1.0)
+    close(out[0, 0], lse[0, 0], v[0, 0], even & torch.ones(N, N, dtype=torch.bool, device=dev).tril(), "prompt")
+    for T in (1, 7, 40):
+        c = Case([N], N, 2, 1, D, T, dtype, dev, spare=0)
+        c.q.fill_(20480.0)
+        c.k[0, :, 0] = rows(N)
+        for off in (None, torch.zeros(1, 1, N, device=dev)):
+            out, lse = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, scale=1.0, log_offsets=off)
+            for h in range(2):
+                close(out[0, h], lse[0, h], c.v[0, :, 0], even & cached_keep(N, T, None, dev), f"T={T}")
