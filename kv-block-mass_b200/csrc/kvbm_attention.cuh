@@ -196,6 +196,17 @@ __device__ __noinline__ void add_nonfinite(const CachedArgs& a, int b, int g, in
   }
 }
 
+// How far below a row's maximum (powers of two) its reference is put when the
+// maximum raises it: weights of the maximum are 2^kHead.  fp16 holds 2^-14 at
+// full precision, and with the growth of less than 2^8 that a reference is left
+// alone for, weights of up to 2^15: the 2^7 in between goes to the small ones.
+// A weight of an fp16 kernel is then rounded to 11 bits or to 2^-32 of the
+// row's largest, whichever is coarser: n keys lose at most n 2^-32 of their
+// values.  (Without, n 2^-25, and 131071 keys 17.5 nats below a first one lost
+// the whole of their 0.3 %.)  bf16 has float32's range.
+template <bool kBf16>
+constexpr float kHead = kBf16 ? 0.f : 7.f;
+
 // Scales the tcgen05 kernels take: positive (the maximum of the raw scores is
 // the maximum), and finite as a factor of base-2 exponents.
 inline bool tc_scale(float scale) { return scale > 0.f && scale * kLog2eF < INFINITY; }

@@ -34,8 +34,8 @@
 //
 // The running maximum is raised (and O multiplied in TMEM by its softmax
 // thread) only when a row's scores grow by more than 2^8 over it: weights stay
-// below 2^8, which both 16-bit types hold at full precision, sums are fp32,
-// and after the first key tiles almost no tile pays for it.  S of the next
+// below 2^8 (fp16, whose small weights need the range: 2^15, see kHead), sums are
+// fp32, and after the first key tiles almost no tile pays for it.  S of the next
 // tile is issued after P V of this one, and MMAs of a CTA complete in order,
 // so a full S also means that O is up to date.
 #include <cuda.h>
@@ -433,9 +433,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         mt = __fmul_rn(fmax_nan(mt, mx[(half ^ 1) * TILE + rl]), C);  // rounded as the weights' products are
-        const bool grow = mt - m > kAttGrow || mt != mt;  // (true from -inf to anything finite, and for NaN)
+        const bool grow = mt - m > kAttGrow + kHead<kBf16> || mt != mt;  // (true from -inf to anything finite, and for NaN)
         if (__any_sync(0xffffffffu, grow)) {
-          const float mn = grow ? mt : m;
+          const float mn = grow ? mt - kHead<kBf16> : m;
           const float f = m == mn ? 1.f : ex2(m - mn);
           l *= f;
           m = mn;

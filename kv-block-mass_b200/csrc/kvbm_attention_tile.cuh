@@ -27,9 +27,10 @@ namespace sm100 {
 
 constexpr int kAttTile = 128;
 constexpr int kAttCols = 64;  // scores of a row in one thread
-// Growth of a row's maximum (base 2) that makes it the new reference: weights
-// stay below 2^8, which both 16-bit types hold at full precision.  (The
-// difference is compared: adding the growth to a large reference rounds it.)
+// Growth of a row's maximum (base 2) over the reference (and kHead) that moves
+// the reference: weights stay below 2^8, fp16 ones below 2^15, which the types
+// hold.  (The difference is compared: adding the growth to a large reference
+// rounds it.)
 constexpr float kAttGrow = 8.f;
 
 // A NaN among the values makes the maximum NaN (and with it the row).

@@ -28,7 +28,7 @@ namespace {
 constexpr int KT = kCachedKeyTile;  // 64 keys a tile
 constexpr int kThreads = 128;
 constexpr int BM = 16;
-constexpr float kGrow = 5.5f;  // growth (natural log) of a row's maximum that makes it the new reference
+constexpr float kGrow = 5.5f;  // growth (natural log) of a row's maximum over the reference (and kHead) that moves it
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -351,9 +351,11 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? kMmaCtas : 1) cached_mma
         float top = max_nan(max_nan(s[0][2 * hrow], s[0][2 * hrow + 1]), max_nan(s[1][2 * hrow], s[1][2 * hrow + 1]));
         top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        if (!(top <= m[hrow] + kGrow)) {
-          f[hrow] = m[hrow] == top ? 1.f : ex2f((m[hrow] - top) * kLog2eF);
-          m[hrow] = top;
+        constexpr float head = kHead<kBf16> * kLn2F;
+        if (top - m[hrow] > kGrow + head || top != top) {  // (true from -inf to anything finite, and for NaN)
+          const float mn = top - head;
+          f[hrow] = m[hrow] == mn ? 1.f : ex2f((m[hrow] - mn) * kLog2eF);
+          m[hrow] = mn;
           grew = true;
         }
       }
@@ -380,7 +382,8 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? kMmaCtas : 1) cached_mma
         l[1] += (p[0][2] + p[0][3]) + (p[1][2] + p[1][3]);
         // For the product with v a weight is split into two 16-bit parts, high and
         // rest: 3 % of the time (153 -> 158 us at 32 sequences), and the rounding of
-        // the result is then the only one (one part alone: 1.4 times its error).
+        // the result is then the only one of its size (one part alone: 1.4 times its
+        // error), but for fp16 weights so small that both parts are subnormal (kHead).
         pf[0] = pack2<kBf16>(p[0][0], p[0][1]);
         pf[1] = pack2<kBf16>(p[0][2], p[0][3]);
         pf[2] = pack2<kBf16>(p[1][0], p[1][1]);

@@ -573,9 +573,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mt = fmax_nan(mt, mx[(half ^ 1) * TILE + rl]);
         if (!kBias) mt = __fmul_rn(mt, C);  // rounded as the weights' products are
-        const bool grow = mt - m > (kBias ? kAttGrow * kLn2F : kAttGrow) || mt != mt;
+        constexpr float kUnit = kBias ? kLn2F : 1.f;  // natural logarithms, or base 2
+        const bool grow = mt - m > (kAttGrow + kHead<kBf16>) * kUnit || mt != mt;
         if (__any_sync(0xffffffffu, grow)) {
-          const float mn = grow ? mt : m;
+          const float mn = grow ? mt - kHead<kBf16> * kUnit : m;
           const float f = m == mn ? 1.f : ex2(kBias ? (m - mn) * kLog2eF : m - mn);
           l *= f;
           m = mn;

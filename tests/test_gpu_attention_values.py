@@ -147,3 +147,39 @@ def test_scores_past_float32_steps(cuda_device, dtype, big, small):
             out, lse = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, scale=1.0, log_offsets=off)
             for h in range(2):
                 close(out[0, h], lse[0, h], c.v[0, :, 0], even & cached_keep(N, T, None, dev), f"T={T}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gap", [12.0, 17.5, 20.0])
+def test_many_small_weights(cuda_device, dtype, gap):
+    """One key `gap` nats above n equal ones.  Their weights, n exp(-gap) together, are summed at the rounding of each
+    to the type (u) or, fp16, to its subnormal step of 2^-25 at 2^7 times the weight: n 2^-32 of the values in all."""
+    dev, D = cuda_device, 64
+    u = half_step(dtype)
+
+    def close(out, n, what):
+        p = n * math.exp(-gap) / (1 + n * math.exp(-gap))
+        sub = n * 2.0 ** -32 if dtype == torch.float16 else 0.0
+        want = torch.full(out.shape, p, dtype=F64, device=dev)
+        # scores are exact but for the scale and the exponential's argument and value: 2^-18 relative; sums (n / 16 + 64) 2^-24
+        tol = (2 * u + 2.0 ** -18 + 2 * gap * 2.0 ** -24 + (n / 16 + 64) * 2.0 ** -24) * p + sub + 1e-30
+        check(out, want, torch.full_like(want, tol), what)
+
+    n = 131071
+    q = torch.zeros(1, 1, n + 1, D, device=dev, dtype=dtype)
+    q[..., 0] = 8.0
+    k = torch.zeros(1, 1, n + 1, D, device=dev, dtype=dtype)
+    k[0, 0, 0, 0] = gap
+    v = torch.ones(1, 1, n + 1, D, device=dev, dtype=dtype)
+    v[0, 0, 0] = 0
+    if dtype != torch.float32:
+        out, _ = kb.attention_b200(q, k, v, causal=True)
+        for r in (n, n // 2, 4000):
+            close(out[0, 0, r], r, f"prompt row {r}")
+    cache_k, cache_v = k.transpose(1, 2).contiguous(), v.transpose(1, 2).contiguous()
+    for T, Hq in ((1, 4), (3, 8), (40, 8)):
+        for off in (None, torch.zeros(1, 1, n + 1, device=dev)):
+            out, _ = kb.attention_cached(q[:, :, :1].expand(1, Hq, T, D).contiguous(), cache_k, cache_v, None,
+                                         torch.tensor([n + 1]), log_offsets=off)
+            for t in range(T):
+                close(out[0, :, t], n - (T - 1 - t), f"T={T}")
