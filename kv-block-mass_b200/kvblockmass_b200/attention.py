@@ -24,7 +24,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _VALUE_ERRORS, _as_mask
+from .ops import _DTYPES, _VALUE_ERRORS, _as_mask, _to_int32
 
 __all__ = ["attention_b200", "attention_varlen", "attention_cached", "cached_attention_workspace_bytes"]
 
@@ -62,7 +62,7 @@ def _int32_on(t: torch.Tensor, dev, name: str) -> torch.Tensor:
         return t
     if t.dtype.is_floating_point or t.dtype == torch.bool:
         raise ValueError(f"{name} must hold integers, got {t.dtype}")
-    return t.to(device=dev, dtype=torch.int32).contiguous()
+    return _to_int32(t, dev).contiguous()
 
 
 def _same(name: str, t: torch.Tensor, like: torch.Tensor) -> None:
@@ -253,7 +253,7 @@ def _table(block_table, B, k_cache, q):
         raise ValueError("q, the caches and block_table must be on one device")
     if block_table.shape[1] == 0:
         raise ValueError("block_table names no pages")
-    t = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)
+    t = block_table if block_table.dtype == torch.int32 else _to_int32(block_table, block_table.device)
     return (t if t.stride(1) == 1 else t.contiguous()), t.shape[1]
 
 

@@ -80,12 +80,20 @@ class _Prepared:
         return self.opts
 
 
+def _to_int32(t: torch.Tensor, dev) -> torch.Tensor:
+    """Integers as int32 on ``dev``; values outside its range become its ends (their low 32 bits would name another
+    page or length)."""
+    if t.dtype in (torch.int64, torch.uint32, torch.uint64):
+        t = t.to(torch.int64).clamp(-2 ** 31, 2 ** 31 - 1)
+    return t.to(device=dev, dtype=torch.int32)
+
+
 def _int32_on(t: torch.Tensor, dev, name: str) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or t.dim() != 1:
         raise ValueError(f"{name} must be a 1-D integer tensor")
     if t.dtype.is_floating_point or t.dtype == torch.bool:
         raise ValueError(f"{name} must hold integers, got {t.dtype}")
-    return t.to(device=dev, dtype=torch.int32).contiguous()
+    return _to_int32(t, dev).contiguous()
 
 
 def _fill_problem(q_ptr, q_strides, k_ptr, k_strides, dtype, B, Hq, Hkv, N, D, dev, keep, attn_mask, causal,
@@ -683,7 +691,7 @@ def make_paged_problem(q, k_cache, block_table, attn_mask=None, causal=False, bl
         qs = q.stride()
     if block_table.shape[1] * page_size < N:
         raise ValueError(f"block_table covers {block_table.shape[1] * page_size} keys < N={N}")
-    table = block_table.to(torch.int32)
+    table = _to_int32(block_table, block_table.device)
     if table.stride(1) != 1:
         table = table.contiguous()
     Hq = q.shape[1]

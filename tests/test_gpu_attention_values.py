@@ -183,3 +183,45 @@ def test_many_small_weights(cuda_device, dtype, gap):
                                          torch.tensor([n + 1]), log_offsets=off)
             for t in range(T):
                 close(out[0, :, t], n - (T - 1 - t), f"T={T}")
+
+
+@pytest.mark.parametrize("wrong", [2 ** 32, -2 ** 32, 2 ** 40 + 3])
+def test_ids_and_lengths_past_32_bits(cuda_device, wrong):
+    """int64 lengths are clamped and int64 page ids are outside the cache, whatever their low 32 bits say."""
+    c = Case([100, 40], 16, 4, 2, 64, 1, torch.bfloat16, cuda_device, seed=2)
+    full = torch.tensor([c.L if wrong > 0 else 0, 40], device=cuda_device)
+    for lens in (torch.tensor([wrong + 9, 40]), torch.tensor([wrong + 9, 40], device=cuda_device)):
+        a = kb.attention_cached(c.q, c.k, c.v, c.table, full)
+        b = kb.attention_cached(c.q, c.k, c.v, c.table, lens)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        w = torch.rand(2, 2, c.L, device=cuda_device)
+        e, f = (kb.evict_cache(c.k, c.v, c.table, x, w, 40) for x in (full, lens))
+        assert torch.equal(e.kept, f.kept) and torch.equal(e.seq_lens, f.seq_lens) and torch.equal(e.k, f.k)
+    q, k, v = _inputs(2, 4, 2, 150, 64, torch.bfloat16, 43, cuda_device)
+    a = kb.attention_b200(q, k, v, seq_lens=torch.tensor([150 if wrong > 0 else 0, 77]))
+    b = kb.attention_b200(q, k, v, seq_lens=torch.tensor([wrong + 5, 77]))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    qp, kp, vp = (t[0].transpose(0, 1).contiguous() for t in (q, k, v))
+    cu = torch.tensor([0, 70, wrong + 100] if wrong > 0 else [wrong, 70, 150])
+    a = kb.attention_varlen(qp, kp, vp, torch.tensor([0, 70, 150]), 150, causal=True)
+    b = kb.attention_varlen(qp, kp, vp, cu, 150, causal=True)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    for table in (c.table.long(),):
+        kb.check_device_errors()
+        table[0, 2] += wrong
+        out, lse = kb.attention_cached(c.q, c.k, c.v, table, c.seq_lens)
+        with pytest.raises(RuntimeError):
+            kb.check_device_errors()
+        kb.evict_cache(c.k, c.v, table, c.seq_lens, torch.rand(2, 2, c.L, device=cuda_device), 60)
+        with pytest.raises(RuntimeError):
+            kb.check_device_errors()
+        kb.block_mass_paged(q[:, :, :100].expand(2, 4, 100, 64).contiguous(), c.k, table, seq_lens=c.seq_lens)
+        with pytest.raises(RuntimeError):
+            kb.check_device_errors()
+        pg = int(c.table[0, 2])
+        c.k[pg] = 0
+        c.v[pg] = 0
+        _check(c, out, lse)
+    a = kb.block_mass_b200(q, k, causal=True, seq_lens=torch.tensor([150 if wrong > 0 else 0, 77]))
+    b = kb.block_mass_b200(q, k, causal=True, seq_lens=torch.tensor([wrong + 5, 77]))
+    assert torch.equal(a, b)
