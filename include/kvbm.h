@@ -488,7 +488,9 @@ KVBM_API int kvbm_design(const kvbm_design_args* d, const kvbm_design_out* out, 
  * key_mask[b * key_mask_bstride + c] != 0 where a key mask is given.  A row
  * that keeps no key gets out 0 and lse -inf.  What a key that is not kept (or
  * a row past a sequence's end) holds, NaN and infinities included, reaches no
- * result.  lse is what kvbm_block_mass_lse and kvbm_options.lse take.
+ * result.  A NaN in v of a kept key makes its column NaN; an infinity makes it
+ * infinite, or NaN where the key's weight rounds to 0 (float32's and bfloat16's
+ * smallest value, 2^-32 of the row's largest weight in float16).  lse is what kvbm_block_mass_lse and kvbm_options.lse take.
  *
  * float32, bfloat16 or float16 (out in the same type; sums, maxima, lse and
  * scale in float32: a smaller scale is 0, a larger one KVBM_ERR_SHAPE),

@@ -637,7 +637,8 @@ __global__ void __launch_bounds__(256) cached_merge_kernel(const __grid_constant
       for (int i = 0; i < kAhead; ++i) {
         fk[i] = __shfl_sync(0xffffffffu, f, (k0 + i) & 31);
         const long long pk = __shfl_sync(0xffffffffu, slot, (k0 + i) & 31);
-        const bool in = k0 + i < n && fk[i] != 0.f && lane < lanes;
+        // (a part whose factor is 0 counts too: its finite values add nothing, its NaN and infinities do)
+        const bool in = k0 + i < n && pk >= 0 && lane < lanes;
         const float4* src = reinterpret_cast<const float4*>(a.part_o + (pk * a.BM + rl) * a.DP + lane * kCols);
 #pragma unroll
         for (int q = 0; q < kCols / 4; ++q) {

@@ -225,3 +225,22 @@ def test_ids_and_lengths_past_32_bits(cuda_device, wrong):
     a = kb.block_mass_b200(q, k, causal=True, seq_lens=torch.tensor([150 if wrong > 0 else 0, 77]))
     b = kb.block_mass_b200(q, k, causal=True, seq_lens=torch.tensor([wrong + 5, 77]))
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,Hq", [(1, 8), (3, 8), (40, 8)])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_non_finite_values_of_small_weight(cuda_device, dtype, T, Hq, value):
+    """A non-finite v of a kept key does not vanish where the part of a split cache that holds it weighs next to
+    nothing: its column is not finite (a weight that rounds to 0 makes NaN of an infinity), every other one is."""
+    n = 6001
+    c = Case([n], 16, Hq, 2, 64, T, dtype, cuda_device, seed=T)
+    off = torch.zeros(1, 1, c.L, device=cuda_device)
+    off[..., :3000] = -1000.0
+    for slot, col in ((0, 3), (777, 9), (2999, 20)):
+        _put(c, c.v, 0, slot, col, value)
+    out, lse = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens, log_offsets=off)
+    odd = torch.zeros(64, dtype=torch.bool, device=cuda_device)
+    odd[[3, 9, 20]] = True
+    assert torch.equal(~torch.isfinite(out), odd.expand(out.shape))
+    assert bool(torch.isfinite(lse).all())
