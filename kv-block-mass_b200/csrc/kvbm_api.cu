@@ -5,6 +5,7 @@
 #include <stdio.h>
 
 #include <atomic>
+#include <mutex>
 
 #include "kvbm_attention.cuh"
 #include "kvbm_internal.cuh"
@@ -97,6 +98,23 @@ int device_sms(int dev) {
   }
   return n;
 }
+
+namespace {
+
+// The error words of the kernels' source files, read and cleared at once.
+struct ErrorWords {
+  unsigned int *wait[3], *page[2];
+};
+__device__ unsigned int g_errors_read;  // bit 0: a wait ran out, bit 1: a bad table entry
+
+__global__ void read_errors_kernel(ErrorWords w) {
+  unsigned int r = 0;
+  for (unsigned int* p : w.wait) r |= atomicExch(p, 0u) != 0 ? 1u : 0u;
+  for (unsigned int* p : w.page) r |= atomicExch(p, 0u) != 0 ? 2u : 0u;
+  g_errors_read = r;
+}
+
+}  // namespace
 
 int attention_device_kind(int dev) { return device_kind(dev); }
 int attention_device_sms(int dev) { return device_sms(dev); }
@@ -667,18 +685,22 @@ int kvbm_copy_2d_async(void* dst, int64_t dst_pitch, const void* src, int64_t sr
 }
 
 int kvbm_check_device_errors(void* stream) {
-  int err = 0, aerr = 0, cerr = 0, perr = 0, aperr = 0;
-  int st = read_and_clear_device_error(static_cast<cudaStream_t>(stream), &err);
-  if (st != KVBM_OK) return st;
-  st = read_and_clear_attention_error(static_cast<cudaStream_t>(stream), &aerr);
-  if (st != KVBM_OK) return st;
-  st = read_and_clear_cached_error(static_cast<cudaStream_t>(stream), &cerr);
-  if (st != KVBM_OK) return st;
-  st = read_and_clear_page_error(static_cast<cudaStream_t>(stream), &perr);
-  if (st != KVBM_OK) return st;
-  st = read_and_clear_attention_page_error(static_cast<cudaStream_t>(stream), &aperr);
-  if (st != KVBM_OK) return st;
-  return err || aerr || cerr ? KVBM_ERR_TIMEOUT : (perr || aperr ? KVBM_ERR_PAGE : KVBM_OK);
+  const ErrorWords w = {{device_error_word(), attention_error_word(), cached_error_word()},
+                        {page_error_word(), attention_page_error_word()}};
+  for (unsigned int* p : w.wait)
+    if (p == nullptr) return KVBM_ERR_CUDA;
+  for (unsigned int* p : w.page)
+    if (p == nullptr) return KVBM_ERR_CUDA;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  static std::mutex one;  // g_errors_read is one word
+  const std::lock_guard<std::mutex> lock(one);
+  unsigned int r = 0;
+  void* args[] = {const_cast<ErrorWords*>(&w)};
+  if (cudaLaunchKernel(reinterpret_cast<const void*>(&read_errors_kernel), dim3(1), dim3(1), args, 0, s) != cudaSuccess ||
+      cudaMemcpyFromSymbolAsync(&r, g_errors_read, sizeof(r), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
+      cudaStreamSynchronize(s) != cudaSuccess)
+    return KVBM_ERR_CUDA;
+  return r & 1u ? KVBM_ERR_TIMEOUT : (r & 2u ? KVBM_ERR_PAGE : KVBM_OK);
 }
 
 }  // extern "C"

@@ -849,22 +849,6 @@ int launch_cached_weights(const CachedArgs& a, cudaStream_t s) {
              : launch_dependent(cached_weights_kernel<1>, grid, 256, s, a);
 }
 
-int read_and_clear_attention_page_error(cudaStream_t s, int* err) {
-  unsigned int v = 0;
-  if (cudaMemcpyFromSymbolAsync(&v, g_attention_page_error, sizeof(v), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
-      cudaStreamSynchronize(s) != cudaSuccess)
-    return KVBM_ERR_CUDA;
-  *err = v != 0;
-  if (v != 0) {
-    const unsigned int zero = 0;
-    if (cudaMemcpyToSymbolAsync(g_attention_page_error, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s) !=
-            cudaSuccess ||
-        cudaStreamSynchronize(s) != cudaSuccess)
-      return KVBM_ERR_CUDA;
-  }
-  return KVBM_OK;
-}
-
 // Looked up once per device (every device has a copy of the word).
 unsigned int* attention_page_error_word() {
   constexpr int kMaxDevices = 64;

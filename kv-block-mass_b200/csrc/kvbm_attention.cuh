@@ -221,10 +221,11 @@ int launch_cached_mma(const CachedArgs& a, int dtype, cudaStream_t s);  // R <= 
 int launch_cached_tc(const CachedArgs& a, int dtype, cudaStream_t s);   // row tiles of 128 or 256, 16-bit types, D <= 128
 int launch_cached_merge(const CachedArgs& a, int dtype, cudaStream_t s);
 int launch_cached_weights(const CachedArgs& a, cudaStream_t s);
-int read_and_clear_attention_error(cudaStream_t s, int* err);         // waits that ran out
-int read_and_clear_cached_error(cudaStream_t s, int* err);
-int read_and_clear_attention_page_error(cudaStream_t s, int* err);    // bad table entries (attention, eviction)
-unsigned int* attention_page_error_word();                            // its device address (or null)
+// Device addresses of the error words (or null): waits that ran out in the
+// prompt and the cache kernels, bad table entries (attention, eviction).
+unsigned int* attention_error_word();
+unsigned int* cached_error_word();
+unsigned int* attention_page_error_word();
 
 // Allows a kernel its dynamic shared memory (kvbm_attention_api.cu): set once
 // per kernel and device, 4 us of a call otherwise.

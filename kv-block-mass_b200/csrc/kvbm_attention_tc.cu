@@ -574,6 +574,6 @@ int launch_prompt_tc(const PromptArgs& a, int dtype, cudaStream_t s) {
   return bf16 ? launch<128, true>(a, sms, s) : launch<128, false>(a, sms, s);
 }
 
-int read_and_clear_attention_error(cudaStream_t s, int* err) { return sm100::read_and_clear_wait_error(s, err); }
+unsigned int* attention_error_word() { return sm100::wait_error_word(); }
 
 }  // namespace kvbm

@@ -737,6 +737,6 @@ int launch_cached_tc(const CachedArgs& a, int dtype, cudaStream_t s) {
   return bf16 ? launch_d<128, true>(a, s) : launch_d<128, false>(a, s);
 }
 
-int read_and_clear_cached_error(cudaStream_t s, int* err) { return sm100::read_and_clear_wait_error(s, err); }
+unsigned int* cached_error_word() { return sm100::wait_error_word(); }
 
 }  // namespace kvbm

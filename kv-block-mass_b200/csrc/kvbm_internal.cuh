@@ -248,8 +248,8 @@ int launch_lse_import(const kvbm_problem* p, const WsLayout& L, const float* lse
 int launch_reduce(const kvbm_problem* p, const WsLayout& L, void* mass_out, void* ws,
                   cudaStream_t s, bool per_sequence);
 
-// Device error word: set when a bounded wait in a tcgen05 kernel gives up.
-int read_and_clear_device_error(cudaStream_t s, int* err);
+// Address of the device error word: set when a bounded wait in a tcgen05 kernel gives up.
+unsigned int* device_error_word();
 // kvbm_tc.cu: a bounded wait that nothing satisfies (kvbm_selftest_wait_timeout).
 int selftest_wait_timeout(cudaStream_t s, unsigned long long limit_ns, int* waited);
 
@@ -260,7 +260,7 @@ int selftest_wait_timeout(cudaStream_t s, unsigned long long limit_ns, int* wait
 // as zeros without reading the block table.
 int launch_page_gather(const kvbm_paged_kv* kv, int dtype, int b0, int g0, int nb, int ng, int N, int D,
                        const int32_t* lens, const int32_t* cu, long long total, void* out, cudaStream_t s);
-// Page error word: set when a block-table entry was outside [0, num_pages).
-int read_and_clear_page_error(cudaStream_t s, int* err);
+// Address of the page error word: set when a block-table entry was outside [0, num_pages).
+unsigned int* page_error_word();
 
 }  // namespace kvbm

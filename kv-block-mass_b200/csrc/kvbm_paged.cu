@@ -105,19 +105,13 @@ int launch_page_gather(const kvbm_paged_kv* kv, int dtype, int b0, int g0, int n
   return launch_gather<unsigned short>(kv, esize, b0, g0, nb, ng, N, D, lens, cu, total, out, s);
 }
 
-int read_and_clear_page_error(cudaStream_t s, int* err) {
-  unsigned int v = 0;
-  if (cudaMemcpyFromSymbolAsync(&v, g_page_error, sizeof(v), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
-      cudaStreamSynchronize(s) != cudaSuccess)
-    return KVBM_ERR_CUDA;
-  *err = v != 0;
-  if (v != 0) {
-    const unsigned int zero = 0;
-    if (cudaMemcpyToSymbolAsync(g_page_error, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s) != cudaSuccess ||
-        cudaStreamSynchronize(s) != cudaSuccess)
-      return KVBM_ERR_CUDA;
+unsigned int* page_error_word() {
+  void* p = nullptr;
+  if (cudaGetSymbolAddress(&p, g_page_error) != cudaSuccess) {
+    cudaGetLastError();
+    return nullptr;
   }
-  return KVBM_OK;
+  return static_cast<unsigned int*>(p);
 }
 
 }  // namespace kvbm

@@ -15,27 +15,20 @@ namespace sm100 {
 
 // Device-wide error word: nonzero once a bounded wait gave up (see kvbm.h,
 // kvbm_check_device_errors).  Every source file that includes this header
-// holds a copy of its own and a reader for it.
+// holds a copy of its own; those with waits name its address below.
 static __device__ unsigned int g_kvbm_device_error = 0;
 
 // A wait on an mbarrier gives up after this many nanoseconds of %globaltimer.
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s
 
-// Reads and clears this source file's copy of the error word (synchronises `s`).
-static inline int read_and_clear_wait_error(cudaStream_t s, int* err) {
-  unsigned int v = 0;
-  if (cudaMemcpyFromSymbolAsync(&v, g_kvbm_device_error, sizeof(v), 0, cudaMemcpyDeviceToHost, s) != cudaSuccess ||
-      cudaStreamSynchronize(s) != cudaSuccess)
-    return KVBM_ERR_CUDA;
-  *err = v != 0;
-  if (v != 0) {
-    const unsigned int zero = 0;
-    if (cudaMemcpyToSymbolAsync(g_kvbm_device_error, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s) !=
-            cudaSuccess ||
-        cudaStreamSynchronize(s) != cudaSuccess)
-      return KVBM_ERR_CUDA;
+// The device address of this source file's copy (or null).
+static inline unsigned int* wait_error_word() {
+  void* p = nullptr;
+  if (cudaGetSymbolAddress(&p, g_kvbm_device_error) != cudaSuccess) {
+    cudaGetLastError();
+    return nullptr;
   }
-  return KVBM_OK;
+  return static_cast<unsigned int*>(p);
 }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

@@ -1782,6 +1782,6 @@ int launch_tc(const kvbm_problem* p, const WsLayout& L, void* mass_out, void* ws
   return KVBM_ERR_HEAD_DIM;
 }
 
-int read_and_clear_device_error(cudaStream_t s, int* err) { return sm100::read_and_clear_wait_error(s, err); }
+unsigned int* device_error_word() { return sm100::wait_error_word(); }
 
 }  // namespace kvbm

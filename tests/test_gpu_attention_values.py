@@ -1,12 +1,14 @@
 """Values at the edges of what the attention kernels can hold, against 64 bits: non-finite values of kept keys, masks of
 single tokens, scales and scores of extreme size, small weights, wide integer ids.  Bounds: ``_attention_ref``."""
 
+import ctypes
 import math
 
 import pytest
 import torch
 
 import kvblockmass_b200 as kb
+from kvblockmass_b200 import _lib
 from _attention_ref import F64, cached_keep, check, half_step
 from test_gpu_attention import _check_dense, _inputs
 from test_gpu_cached_attention import Case, _check, _tree
@@ -244,3 +246,23 @@ def test_non_finite_values_of_small_weight(cuda_device, dtype, T, Hq, value):
     odd[[3, 9, 20]] = True
     assert torch.equal(~torch.isfinite(out), odd.expand(out.shape))
     assert bool(torch.isfinite(lse).all())
+
+
+def test_device_errors_are_read_together(cuda_device):
+    """Words of different kernels set at once: one check reports them (a wait that ran out first) and clears all."""
+    lib = _lib.load()
+    stream = torch.cuda.current_stream(cuda_device).cuda_stream
+    c = Case([100, 40], 16, 4, 2, 64, 1, torch.bfloat16, cuda_device, seed=2)
+    c.table[0, 2] = -1
+    kb.check_device_errors()
+    for attend, mass, wait in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (1, 1, 1)):
+        if attend:
+            kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens)
+        if mass:
+            kb.block_mass_paged(c.q.expand(2, 4, 100, 64).contiguous(), c.k, c.table, seq_lens=c.seq_lens)
+        if wait:
+            waited = ctypes.c_int(-1)
+            assert lib.kvbm_selftest_wait_timeout(stream, 20_000, ctypes.byref(waited)) == _lib.KVBM_OK
+        want = _lib.KVBM_ERR_TIMEOUT if wait else _lib.KVBM_ERR_PAGE
+        assert lib.kvbm_check_device_errors(stream) == want
+        assert lib.kvbm_check_device_errors(stream) == _lib.KVBM_OK
