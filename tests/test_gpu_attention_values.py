@@ -9,7 +9,7 @@ import torch
 
 import kvblockmass_b200 as kb
 from kvblockmass_b200 import _lib
-from _attention_ref import F64, cached_keep, check, half_step
+from _attention_ref import F64, cached_keep, check, half_step, softmax_rows
 from test_gpu_attention import _check_dense, _inputs
 from test_gpu_cached_attention import Case, _check, _tree
 
@@ -266,3 +266,20 @@ def test_device_errors_are_read_together(cuda_device):
         want = _lib.KVBM_ERR_TIMEOUT if wait else _lib.KVBM_ERR_PAGE
         assert lib.kvbm_check_device_errors(stream) == want
         assert lib.kvbm_check_device_errors(stream) == _lib.KVBM_OK
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,Hq,D", [(1, 8, 64), (1, 32, 128), (4, 8, 128), (1, 4, 256)])
+def test_weights_in_two_parts(cuda_device, dtype, T, Hq, D):
+    """Up to 32 rows a kv head the weights enter the product with v in two 16-bit parts, u^2 off together: the
+    result's own rounding (u) is the only one of its size."""
+    c = Case([900, 2500, 77], 16, Hq, 2, D, T, dtype, cuda_device, seed=D + T)
+    out, _ = kb.attention_cached(c.q, c.k, c.v, c.table, c.seq_lens)
+    u = half_step(dtype)
+    for b, n in enumerate(c.lens):
+        for h in range(Hq):
+            k, v = c.rows(b, h // (Hq // 2))
+            o, _, p, tol, _, _ = softmax_rows(c.q[b, h], k, v, cached_keep(n, T, None, cuda_device), 1 / math.sqrt(D),
+                                              dtype=torch.float32)
+            sub = n * 2.0 ** -32 * float(v.abs().max()) if dtype == torch.float16 else 0.0
+            check(out[b, h], o, tol + u * o.abs() + u * u * (1 + 2 * u) * (p @ v.double().abs()) + sub, f"out[{b},{h}]")
