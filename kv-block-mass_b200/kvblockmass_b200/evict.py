@@ -49,6 +49,11 @@ def evict_cache(k_cache, v_cache, block_table, seq_lens, weights, budget, *, n_s
     sequence (default ``budget``), zeros past the new length; ``out=(k, v)``
     gives the memory instead (``[B, capacity, H_kv, D]``, not overlapping the
     inputs), whose slots past the new length are left as they were.
+
+    Decoding over the result needs ``capacity > budget``: token ``u`` of the
+    next call goes to slot ``seq_lens[b] + u`` of sequence ``b``, which differs
+    between sequences shorter and longer than ``budget``, and a length past
+    ``capacity`` would be clamped.
     """
     if not all(isinstance(t, torch.Tensor) for t in (k_cache, v_cache)):
         raise TypeError("evict_cache: k_cache and v_cache must be torch tensors")

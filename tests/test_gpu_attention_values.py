@@ -9,7 +9,7 @@ import torch
 
 import kvblockmass_b200 as kb
 from kvblockmass_b200 import _lib
-from _attention_ref import F64, cached_keep, check, half_step, softmax_rows
+from _attention_ref import F64, cached_keep, check, evict_rows, half_step, softmax_rows
 from test_gpu_attention import _check_dense, _inputs
 from test_gpu_cached_attention import Case, _check, _tree
 
@@ -283,3 +283,67 @@ def test_weights_in_two_parts(cuda_device, dtype, T, Hq, D):
                                               dtype=torch.float32)
             sub = n * 2.0 ** -32 * float(v.abs().max()) if dtype == torch.float16 else 0.0
             check(out[b, h], o, tol + u * o.abs() + u * u * (1 + 2 * u) * (p @ v.double().abs()) + sub, f"out[{b},{h}]")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shared", [False, True])
+def test_decoding_on_after_evictions(cuda_device, dtype, shared):
+    """Evictions of uneven caches (empty, shorter than the budget, longer) with decoding in between: each sequence's
+    new tokens go to its own next slots, its weights into an array of the compact cache's size."""
+    dev, Hq, Hkv, D, budget, room = cuda_device, 8, 2, 64, 60, 12
+    c = Case([40, 300, 0, 61, 150], 16, Hq, Hkv, D, 1, dtype, dev, seed=31)
+    B, G = len(c.lens), Hq // Hkv
+    g = torch.Generator().manual_seed(5)
+    rows = torch.arange(B, device=dev)
+    k, v, table, lens = c.k, c.v, c.table, c.seq_lens
+    w = torch.rand(B, 1 if shared else Hkv, c.L, generator=g).to(dev)
+    for turn in range(2):
+        old = [[(c.rows(b, h) if turn == 0 else (k[b, :int(lens[b]), h], v[b, :int(lens[b]), h])) for h in range(Hkv)]
+               for b in range(B)]
+        e = kb.evict_cache(k, v, table, lens, w, budget, n_sinks=4, recency=16, capacity=budget + room)
+        want = lens.clamp(max=budget)
+        assert torch.equal(e.seq_lens, want)
+        for b in range(B):
+            for h in range(Hkv):
+                kept = evict_rows(w[b, h % w.shape[1]].tolist(), int(lens[b]), budget, 4, 16)
+                assert e.kept[b, h % w.shape[1], :len(kept)].tolist() == kept
+                assert torch.equal(e.k[b, :len(kept), h], old[b][h][0][kept])
+                assert torch.equal(e.v[b, :len(kept), h], old[b][h][1][kept])
+        k, v, table, lens = e.k, e.v, None, e.seq_lens
+        w = torch.zeros(B, Hkv, budget + room, device=dev)
+        w[:, :, :budget] = e.weights
+        for _ in range(3):  # one token at a time
+            k[rows, lens], v[rows, lens] = (torch.randn(B, Hkv, D, generator=g).to(dtype).to(dev) for _ in range(2))
+            lens = lens + 1
+            q = torch.randn(B, Hq, 1, D, generator=g).to(dtype).to(dev)
+            before = w.clone()
+            out, lse, w = kb.attention_cached(q, k, v, table, lens, weights=w)
+            for b in range(B):
+                n = int(lens[b])
+                for h in range(Hkv):
+                    total, tol = before[b, h, :n].double(), 0.0
+                    for i in range(h * G, (h + 1) * G):
+                        o, l, p, ot, lt, pt = softmax_rows(q[b, i], k[b, :n, h], v[b, :n, h],
+                                                           cached_keep(n, 1, None, dev), 1 / math.sqrt(D), dtype=dtype)
+                        check(out[b, i], o, ot, f"out[{b},{i}]")
+                        check(lse[b, i], l, lt, f"lse[{b},{i}]")
+                        total, tol = total + p[0], tol + pt[0]
+                    check(w[b, h, :n], total, tol + 2.0 ** -23 * total, f"weights[{b},{h}]")
+                    assert bool((w[b, h, n:] == 0).all())
+        # drafted tokens, dropped again afterwards
+        T = 5
+        tree = _tree(B, T, turn, dev)
+        slots = lens[:, None] + torch.arange(T, device=dev)
+        k[rows[:, None], slots], v[rows[:, None], slots] = (torch.randn(B, T, Hkv, D, generator=g).to(dtype).to(dev)
+                                                            for _ in range(2))
+        q = torch.randn(B, Hq, T, D, generator=g).to(dtype).to(dev)
+        out, lse = kb.attention_cached(q, k, v, table, lens + T, tree_mask=tree)
+        for b in range(B):
+            n = int(lens[b]) + T
+            for i in range(Hq):
+                o, l, _, ot, lt, _ = softmax_rows(q[b, i], k[b, :n, i // G], v[b, :n, i // G],
+                                                  cached_keep(n, T, tree[b], dev), 1 / math.sqrt(D), dtype=dtype)
+                check(out[b, i], o, ot, f"tree out[{b},{i}]")
+                check(lse[b, i], l, lt, f"tree lse[{b},{i}]")
+        if shared:
+            w = w.sum(1, keepdim=True)
