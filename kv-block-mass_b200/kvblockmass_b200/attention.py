@@ -84,8 +84,11 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
 
 
 def _no_overlap(name: str, t: torch.Tensor, others: dict) -> None:
+    """``others``: the tensors the kernels use besides ``t`` (absent ones, None, and copies made for the call pass)."""
     a0, a1 = _span(t)
     for other, o in others.items():
+        if o is None:
+            continue
         b0, b1 = _span(o)
         if a0 < b1 and b0 < a1:
             raise ValueError(f"{name} overlaps {other}: the kernels write it while they read the inputs")
@@ -114,7 +117,19 @@ def _heads(Hq: int, Hkv: int) -> None:
         raise ValueError(f"GQA requires H_q % H_kv == 0, got H_q={Hq}, H_kv={Hkv}")
 
 
-def _prompt(q, k, v, dims, strides, attn_mask, causal, scale, out, out_strides, lse, lse_strides, fill, lens=None,
+def _key_mask(attn_mask, B: int, N: int, dev):
+    """A contiguous bool key mask [B|1, 1, N], or None."""
+    if attn_mask is None:
+        return None
+    m = _as_mask(attn_mask, dev)
+    if m.dim() == 1:
+        m = m.reshape(1, 1, -1)
+    if m.dim() != 3 or m.shape[0] not in (1, B) or m.shape[1] != 1 or m.shape[2] != N:
+        raise ValueError(f"attn_mask must be a key mask [N] or [B|1, 1, N] with N={N}, got {tuple(m.shape)}")
+    return m.contiguous()
+
+
+def _prompt(q, k, v, dims, strides, mask, causal, scale, out, out_strides, lse, lse_strides, fill, lens=None,
             cu=None, total=0):
     B, Hq, Hkv, N, D = dims
     dev = q.device
@@ -124,16 +139,8 @@ def _prompt(q, k, v, dims, strides, attn_mask, causal, scale, out, out_strides, 
     a.out_stride, a.lse_stride = _I4(*out_strides), _I3(*lse_strides)
     a.dtype = _DTYPES[q.dtype]
     a.B, a.Hq, a.Hkv, a.N, a.D = B, Hq, Hkv, N, D
-    keep = []
-    if attn_mask is not None:
-        m = _as_mask(attn_mask, dev)
-        if m.dim() == 1:
-            m = m.reshape(1, 1, -1)
-        if m.dim() != 3 or m.shape[0] not in (1, B) or m.shape[1] != 1 or m.shape[2] != N:
-            raise ValueError(f"attn_mask must be a key mask [N] or [B|1, 1, N] with N={N}, got {tuple(m.shape)}")
-        m = m.contiguous()
-        a.key_mask, a.key_mask_bstride = m.data_ptr(), (m.stride(0) if m.shape[0] > 1 else 0)
-        keep.append(m)
+    if mask is not None:
+        a.key_mask, a.key_mask_bstride = mask.data_ptr(), (mask.stride(0) if mask.shape[0] > 1 else 0)
     a.scale = float(1.0 / D ** 0.5 if scale is None else scale)
     a.causal = int(bool(causal))
     if lens is not None:
@@ -172,6 +179,8 @@ def attention_b200(q, k, v, attn_mask=None, causal=False, scale=None, *, seq_len
         lens = _int32_on(seq_lens, q.device, "seq_lens")
         if lens.shape[0] != B:
             raise ValueError(f"seq_lens must have B={B} entries, got {lens.shape[0]}")
+    mask = _key_mask(attn_mask, B, N, q.device)
+    ins = {"q": q, "k": k, "v": v, "seq_lens": lens, "attn_mask": mask}
     fill = out is None and lse_out is None
     if out is None:
         out = torch.empty_like(q) if fill or lens is None else torch.zeros_like(q)
@@ -179,14 +188,14 @@ def attention_b200(q, k, v, attn_mask=None, causal=False, scale=None, *, seq_len
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     else:
         _check_out("out", out, q.shape, q.dtype, q.device)
-        _no_overlap("out", out, {"q": q, "k": k, "v": v})
+        _no_overlap("out", out, ins)
     if lse_out is None:
         lse_out = q.new_empty((B, Hq, N), dtype=torch.float32) if fill or lens is None else \
             torch.full((B, Hq, N), float("-inf"), dtype=torch.float32, device=q.device)
     else:
         _check_out("lse_out", lse_out, (B, Hq, N), torch.float32, q.device)
-        _no_overlap("lse_out", lse_out, {"q": q, "k": k, "v": v, "out": out})
-    _prompt(q, k, v, (B, Hq, k.shape[1], N, D), (q.stride(), k.stride(), v.stride()), attn_mask, causal, scale, out,
+        _no_overlap("lse_out", lse_out, {**ins, "out": out})
+    _prompt(q, k, v, (B, Hq, k.shape[1], N, D), (q.stride(), k.stride(), v.stride()), mask, causal, scale, out,
             out.stride(), lse_out, lse_out.stride(), fill, lens=lens)
     return out, lse_out
 
@@ -217,18 +226,19 @@ def attention_varlen(q, k, v, cu_seqlens, max_seqlen=None, causal=False, scale=N
         cu_h = cu_seqlens.detach().to("cpu", torch.int64)
         max_seqlen = int((cu_h[1:] - cu_h[:-1]).max())
     cu = _int32_on(cu_seqlens, q.device, "cu_seqlens")
+    ins = {"q": q, "k": k, "v": v, "cu_seqlens": cu}
     fill = out is None and lse_out is None
     if out is None:
         out = q.new_empty((T, Hq, D)) if fill else q.new_zeros((T, Hq, D))
     else:
         _check_out("out", out, q.shape, q.dtype, q.device)
-        _no_overlap("out", out, {"q": q, "k": k, "v": v})
+        _no_overlap("out", out, ins)
     if lse_out is None:
         lse_out = q.new_empty((Hq, T), dtype=torch.float32) if fill else \
             torch.full((Hq, T), float("-inf"), dtype=torch.float32, device=q.device)
     else:
         _check_out("lse_out", lse_out, (Hq, T), torch.float32, q.device)
-        _no_overlap("lse_out", lse_out, {"q": q, "k": k, "v": v, "out": out})
+        _no_overlap("lse_out", lse_out, {**ins, "out": out})
     _prompt(q, k, v, (cu.shape[0] - 1, Hq, Hkv, max(int(max_seqlen), 1), D),
             tuple((0, t.stride(1), t.stride(0), t.stride(2)) for t in (q, k, v)), None, causal, scale, out,
             (0, out.stride(1), out.stride(0), out.stride(2)), lse_out, (0, lse_out.stride(0), lse_out.stride(1)), fill,
@@ -312,6 +322,7 @@ def _cached_args(q, k_cache, v_cache, block_table, seq_lens, tree_mask, log_offs
     if table is not None:
         a.block_table, a.block_table_stride = table.data_ptr(), table.stride(0)
     a.seq_lens = lens.data_ptr()
+    m = t = None
     if tree_mask is not None:
         m = _as_mask(tree_mask, q.device)
         if m.dim() == 2:
@@ -336,9 +347,8 @@ def _cached_args(q, k_cache, v_cache, block_table, seq_lens, tree_mask, log_offs
             weights_out = weights
         wo, a.weights_out_bstride, a.weights_out_hstride = _per_key("weights_out", weights_out, B, Hkv, L, q.device, True)
         _check_out("weights_out", wo, wo.shape, wo.dtype, wo.device)
-        ins = {"q": q, "k_cache": k_cache, "v_cache": v_cache}
-        if log_offsets is not None:
-            ins["log_offsets"] = t
+        ins = {"q": q, "k_cache": k_cache, "v_cache": v_cache, "block_table": table, "seq_lens": lens, "tree_mask": m,
+               "log_offsets": t}
         if weights is weights_out:
             a.weights, a.weights_bstride, a.weights_hstride = wo.data_ptr(), a.weights_out_bstride, a.weights_out_hstride
         else:
@@ -354,11 +364,8 @@ def _cached_args(q, k_cache, v_cache, block_table, seq_lens, tree_mask, log_offs
         keep.append(wo)
     a.scale = float(1.0 / D ** 0.5 if scale is None else scale)
     if out is not None or lse_out is not None:
-        ins = {"q": q, "k_cache": k_cache, "v_cache": v_cache}
-        if log_offsets is not None:
-            ins["log_offsets"] = t
-        if weights is not None:
-            ins["weights"], ins["weights_out"] = weights, weights_out
+        ins = {"q": q, "k_cache": k_cache, "v_cache": v_cache, "block_table": table, "seq_lens": lens, "tree_mask": m,
+               "log_offsets": t, "weights": weights, "weights_out": weights_out}
     if out is None:
         out = q.new_empty((B, Hq, T, D))
     else:

@@ -94,7 +94,8 @@ def evict_cache(k_cache, v_cache, block_table, seq_lens, weights, budget, *, n_s
             raise ValueError(f"out holds {cap} slots per sequence, budget={budget}, capacity={capacity}")
         for name, t in (("out k", ko), ("out v", vo)):
             _check_out(name, t, (B, cap, Hkv, D), k_cache.dtype, dev)
-            _no_overlap(name, t, {"k_cache": k_cache, "v_cache": v_cache, "weights": w})
+            _no_overlap(name, t, {"k_cache": k_cache, "v_cache": v_cache, "weights": w, "block_table": table,
+                                  "seq_lens": lens})
         _no_overlap("out v", vo, {"out k": ko})
     a = _lib.EvictArgs()
     a.k_cache, a.v_cache, a.k_out, a.v_out = k_cache.data_ptr(), v_cache.data_ptr(), ko.data_ptr(), vo.data_ptr()

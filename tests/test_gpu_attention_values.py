@@ -347,3 +347,39 @@ def test_decoding_on_after_evictions(cuda_device, dtype, shared):
                 check(lse[b, i], l, lt, f"tree lse[{b},{i}]")
         if shared:
             w = w.sum(1, keepdim=True)
+
+
+def test_outputs_over_small_inputs(cuda_device):
+    """Outputs over lengths, offsets, tables and masks are refused, as those over q, k and v are."""
+    dev = cuda_device
+    c = Case([40, 20], 16, 4, 2, 64, 1, torch.bfloat16, dev)
+    room = torch.zeros(2, 8, 64, device=dev)  # 4 KB to be shared
+    ints, bits = room.view(torch.int32).flatten(), room.view(torch.bool).flatten()
+    out = room.view(torch.bfloat16).flatten()[:512].view(2, 4, 1, 64)
+    lse = room.flatten()[:8].view(2, 4, 1)
+    lens, table = ints[2:4].copy_(c.seq_lens), ints[4:4 + c.table.numel()].view(c.table.shape)
+    off = room.flatten()[:2 * c.L].view(2, 1, c.L)
+    w = room.flatten()[:4 * c.L].view(2, 2, c.L)
+    keep = bits[:1].view(1, 1)
+    q, k, v = _inputs(2, 4, 2, 1, 64, torch.bfloat16, 61, dev)
+    qp, kp, vp = (t[:, :, 0] for t in (q, k, v))
+    call = lambda ln=c.seq_lens, tb=c.table, **kw: kb.attention_cached(c.q, c.k, c.v, tb, ln, **kw)  # noqa: E731
+    bad = [
+        lambda: kb.attention_b200(q, k, v, seq_lens=lens, out=out),
+        lambda: kb.attention_b200(q, k, v, seq_lens=lens, lse_out=lse),
+        lambda: kb.attention_b200(q, k, v, attn_mask=bits[:2].view(2, 1, 1), out=out),
+        lambda: kb.attention_varlen(qp, kp, vp, ints[:3], 1, out=out[:, :, 0]),
+        lambda: kb.attention_varlen(qp, kp, vp, ints[:3], 1, lse_out=room.flatten()[:8].view(4, 2)),
+        lambda: call(ln=lens, out=out),
+        lambda: call(tb=table, lse_out=lse),
+        lambda: call(tree_mask=keep, out=out),
+        lambda: call(log_offsets=off, out=out),
+        lambda: call(ln=lens, weights=w),
+        lambda: call(tb=table, weights=torch.zeros_like(w), weights_out=w),
+        lambda: kb.evict_cache(c.k, c.v, c.table, lens, torch.zeros(2, 2, c.L, device=dev), 2, n_sinks=1, recency=1,
+                               out=(room.view(torch.bfloat16).flatten()[:512].view(2, 2, 2, 64), torch.empty_like(c.k)[:2, :2])),
+    ]
+    for i, f in enumerate(bad):
+        with pytest.raises(ValueError):
+            f()
+            raise AssertionError(f"call {i} was accepted")
