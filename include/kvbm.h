@@ -490,7 +490,8 @@ KVBM_API int kvbm_design(const kvbm_design_args* d, const kvbm_design_out* out, 
  * a row past a sequence's end) holds, NaN and infinities included, reaches no
  * result.  A NaN in v of a kept key makes its column NaN; an infinity makes it
  * infinite, or NaN where the key's weight rounds to 0 (float32's and bfloat16's
- * smallest value, 2^-32 of the row's largest weight in float16).  lse is what kvbm_block_mass_lse and kvbm_options.lse take.
+ * smallest value, 2^-32 of the row's largest weight in float16).  Sums over v
+ * are float32 ones with weights of up to 2^8 (float16: 2^15).  lse is what kvbm_block_mass_lse and kvbm_options.lse take.
  *
  * float32, bfloat16 or float16 (out in the same type; sums, maxima, lse and
  * scale in float32: a smaller scale is 0, a larger one KVBM_ERR_SHAPE),
@@ -585,7 +586,10 @@ typedef struct kvbm_cached_args {
 
 KVBM_API int kvbm_validate_cached_attention(const kvbm_cached_args* a);
 
-/* Workspace bytes of kvbm_cached_attention (0 on invalid arguments). */
+/* Workspace bytes of kvbm_cached_attention (0 on invalid arguments): some tens
+ * of MB at most for split units; with `weights`, also the scores of every slot
+ * of the table, B * H_q * max_pages * page_size * 4 bytes whatever the lengths
+ * (pass a table as wide as the longest sequence needs). */
 KVBM_API size_t kvbm_cached_attention_workspace_bytes(const kvbm_cached_args* a);
 
 /* `workspace`: 256-byte aligned device memory; its contents on entry do not

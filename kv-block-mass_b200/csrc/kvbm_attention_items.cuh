@@ -1,5 +1,4 @@
-// Work items of the tensor-core prompt kernels: how CTAs (or CTA pairs) find
-// their row tiles, and the rows that belong to no sequence.
+// Work items of the tensor-core prompt kernel: how CTAs find their row tiles, and the rows that belong to no sequence.
 #pragma once
 
 #include "kvbm_attention.cuh"

@@ -20,11 +20,13 @@
 // S/P and O of both tiles: 2 * 128 + 2 * 128 columns.
 //
 // Measured (bf16, D = 128, 32 q heads on 8, causal): one prompt of 16384 tokens
-// 1.89 ms, 1.16 PFLOP/s, 70 % of cuBLAS' rate for the same work, and 2.17 ms
-// called without pause (power); packed prompts of 217 to 2100 tokens, 0.22
-// TFLOP, 0.27 ms.  Bound by the chain score - maximum - weights of a tile: about
-// 3600 cycles, of which the other tile's tensor work fills 2048.  Without any
-// softmax the loop took 1.62 ms.  A pair of CTAs on one tile of 256 rows
+// 1.90 ms, 1.16 PFLOP/s, 70 % of cuBLAS' rate for the same work, and 2.21 ms
+// called without pause (power); packed prompts of 1 to 4044 tokens, 0.22
+// TFLOP, 0.28 ms.  Bound by the chain score - maximum - weights of a tile: about
+// 3500 cycles, of which the other tile's tensor work fills 2048.  Of the packed
+// call that chain is 187 us (102 steps of two tiles in the longest CTA); the rest
+// lies between a CTA's 7 or 8 items, some 20000 cycles each.  Without any
+// softmax the long prompt's loop took 1.62 ms.  A pair of CTAs on one tile of 256 rows
 // (cta_group::2) took 2.66 ms: each step waits on the other CTA's softmax too.
 //
 // The CTAs are persistent (one per SM, items from the longest in a snake over

@@ -4,14 +4,15 @@
 //
 // Bound by reading k and v once per 16 rows.  Every CTA gets the same number of
 // 64-key tiles (kvbm_attention.cu describes the split and the joining); three
-// CTAs an SM with two tiles each in flight (32 sequences of 4-8k keys: 156 us,
-// 5.2 TB/s) hide a tile's chain of products and shuffles better than two CTAs
-// with three (174 us).  A CTA of four warps keeps kStages tiles of k and v in
-// flight with 16-byte cp.async (page lookups one tile ahead), rows swizzled so
-// that ldmatrix meets no bank conflict; warp w takes keys 16 w .. 16 w + 15 of
-// each tile with mma.m16n8k16: one A tile holds 16 rows, so every k and v
-// element leaves shared memory once for them.  Each warp has a running maximum and sum of its own;
-// the four are joined once per unit.  mma.sync rather than tcgen05: 16 rows
+// CTAs an SM with rings of two tiles (32 sequences of 4-8k keys: 158 us, 5.2
+// TB/s) hide a tile's chain of products and shuffles better than two CTAs with
+// three (174 us).  A CTA of four warps has a ring of kStages tiles of k and v:
+// while one is computed, kStages - 1 are in flight with 16-byte cp.async (page
+// lookups one tile further ahead), rows swizzled so that ldmatrix meets no bank
+// conflict; warp w takes keys 16 w .. 16 w + 15 of each tile with mma.m16n8k16:
+// one A tile holds 16 rows, so every k and v element leaves shared memory once
+// for them.  Each warp has a running maximum and sum of its own; the four are
+// joined once per unit.  mma.sync rather than tcgen05: 16 rows
 // would fill an eighth of a tcgen05 tile, and at 64 FLOP a byte at most the
 // tensor work of a tile is a third of the time its bytes take.
 #include <cuda_bf16.h>

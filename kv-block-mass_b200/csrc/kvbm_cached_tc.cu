@@ -10,7 +10,7 @@
 //          ones, and with log offsets all);
 //   else:  any page size: all three warps read the rows with 16-byte cp.async
 //          into the layout TMA would write, page ids looked up one tile ahead.
-//          (32768 keys x 4 sequences, 64 tokens: 358 us this way.)
+//          (32768 keys x 4 sequences, 64 tokens: 358 us this way, 219 the other.)
 //   kPair (R > 128): the streams are two tiles of 128 rows that share every
 //                    key tile;
 //   else:            one tile of rows, the streams take the even and the odd
@@ -18,9 +18,11 @@
 // Either way the tensor pipe works for one stream while the other's softmax
 // runs.  With 256 rows a key tile of 64 KB takes 2048 tensor cycles, about as
 // long as its bytes take from DRAM.  Measured: 4 sequences of 32768 keys, 64
-// tokens, 32 q heads on 8, D = 128: 178 us with the joining (16 us of it), 3.1
-// TB/s and 0.77 PFLOP/s.  Bound as the prompt kernel by the softmax chain, 3600
-// cycles a key tile.
+// tokens, 32 q heads on 8, D = 128: 174 us with the joining (16 us of it), 3.0
+// TB/s and 0.77 PFLOP/s: 53 key tiles a CTA at about 5800 cycles.  The prompt
+// kernel's loop of the same two streams takes 3500 (its softmax chain), so about
+// 2300 cycles a tile are this kernel's own; which wait holds them has not been
+// measured (K and V share kSlots slots, and a tile is up to 16 box loads).
 //
 // Log offsets are added in the natural-log domain, and subtracted from before
 // the conversion to base 2, so that offsets of float32's lowest value act like

@@ -6,14 +6,15 @@
 // Kept tokens keep their order.
 //
 // Two kernels.  evict_select_kernel finds the threshold weight with a radix
-// select (most significant byte first) over order-preserving 32-bit keys and
-// turns the choice into slots with one scan: 4 * len bytes of weights are all
-// it reads from DRAM (once, into shared memory, where the CTAs' share of a row
-// fits).  evict_gather_kernel moves the kept k and v rows, 16 bytes a thread:
-// 4 * budget * D elements a head.  Measured: 8 sequences of up to 16384 tokens cut
-// to 4096 per head (8 heads of 128, bf16): 74 us, the choice 25 of it (the latency
-// of four passes) and the move 49, 5.5 TB/s; one sequence of 32768 cut to 8192
-// for all heads alike: 31 us.
+// select over order-preserving 32-bit keys (three histogram passes, of the top
+// 11, the next 11 and the last 10 bits) and turns the choice into slots with two
+// walks over the row: 4 * len bytes of weights are all it reads from DRAM (once,
+// into shared memory, where the CTAs' share of a row fits).  evict_gather_kernel
+// moves the kept k and v rows, 16 bytes a thread: 4 * budget * D elements a head.
+// Measured: 8 sequences of up to 16384 tokens cut to 4096 per head (8 heads of 128,
+// bf16): 74 us, the choice 25 of it (the latency of three passes with three
+// cluster barriers each and of the walks) and the move 49, 5.5 TB/s; one sequence
+// of 32768 cut to 8192 for all heads alike: 31 us.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 

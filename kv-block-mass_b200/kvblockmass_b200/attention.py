@@ -165,7 +165,9 @@ def attention_b200(q, k, v, attn_mask=None, causal=False, scale=None, *, seq_len
     N]``). A row that keeps no key gets ``out`` 0 and ``lse`` -inf, and so do
     rows past a sequence's end, unless ``out=`` or ``lse_out=`` is given: those
     rows of both are then left as they were. What masked keys and rows past the
-    end hold (NaN included) reaches no result.
+    end hold (NaN included) reaches no result; a non-finite value of a kept key
+    makes its column of ``out`` non-finite.  At most 65535 heads in all (``B *
+    H_q``) and 2^28 positions.
     """
     _check_qkv(q, k, v, "attention_b200")
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
@@ -415,7 +417,8 @@ def attention_cached(q, k_cache, v_cache, block_table, seq_lens, *, tree_mask=No
     ``weights [B, H_kv, max_pages * page_size]`` (float32, ``T == 1``): the
     softmax weight of every key, summed over the heads of its group, is added
     to it, into ``weights_out`` if given, else in place; slots past a
-    sequence's end are not touched.
+    sequence's end are not touched.  The call then holds ``B * H_q * max_pages
+    * page_size`` float32 scores in its workspace, whatever the lengths.
 
     A page id outside ``[0, num_pages)`` is not read (its keys count as zero
     vectors); ``check_device_errors()`` reports it.  ``workspace`` (uint8,
