@@ -172,17 +172,15 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 
-// The non-finite v elements of slots [lo, hi) that token `tok` keeps, added to
-// four output columns from d.  (Drafted tokens': the matrix products took them
-// as zeros.  All slots': repairs a column whose products made NaN of an
-// infinity.)
+// The non-finite v elements of drafted tokens [lo, hi) that token `tok` keeps,
+// added to four output columns from d (the matrix products took them as zeros).
 template <typename T>
 __device__ __noinline__ void add_nonfinite(const CachedArgs& a, int b, int g, int tok, int lo, int hi, int pre,
                                                  int d, float4& acc) {
   const uint8_t* tree = a.tree ? a.tree + b * a.tb : nullptr;
   const float* off = a.off ? a.off + b * a.ob + g * a.oh : nullptr;
   for (int c = lo; c < hi; ++c) {
-    if (c >= pre && !(tree ? tree[tok * a.tr + (c - pre)] != 0 : c - pre <= tok)) continue;
+    if (!(tree ? tree[tok * a.tr + (c - pre)] != 0 : c - pre <= tok)) continue;
     if (off != nullptr && off[c] == -INFINITY) continue;
     const int page = a.pg.page(b, a.pg.page_index(c));
     if (page < 0 || page >= a.pg.num_pages) continue;
