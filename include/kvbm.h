@@ -500,6 +500,7 @@ KVBM_API int kvbm_design(const kvbm_design_args* d, const kvbm_design_out* out, 
  * cu_seqlens (q, k, v, out and lse packed alike, [total_tokens, H, D]: strides
  * {unused, head, row, d}).  fill_outside != 0: rows of `out` and `lse` that
  * belong to no sequence are written (0, -inf); 0: they are left as they were.
+ * Offsets must not decrease: a row that two sequences name holds either's result.
  * `out` must not overlap the inputs.  No workspace; asynchronous on `stream`;
  * the same inputs give the same bits. */
 typedef struct kvbm_attention_args {

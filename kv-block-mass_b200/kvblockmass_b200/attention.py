@@ -206,7 +206,9 @@ def attention_varlen(q, k, v, cu_seqlens, max_seqlen=None, causal=False, scale=N
     """Attention of a packed batch: ``(out [T, H_q, D], lse [H_q, T])``.
 
     ``q [T, H_q, D]``, ``k`` and ``v [T, H_kv, D]``; sequence ``b`` is rows
-    ``[cu_seqlens[b], cu_seqlens[b + 1])`` and attends to itself alone.
+    ``[cu_seqlens[b], cu_seqlens[b + 1])`` and attends to itself alone
+    (``cu_seqlens`` must not decrease: a row that two sequences name holds the
+    result of either).  At most 65535 heads in all (``B * H_q``).
     ``max_seqlen`` (host int; read from ``cu_seqlens`` when omitted, which
     synchronises): the longest sequence; rows past a sequence's first
     ``max_seqlen`` count as outside it.  ``lse`` has the layout
